@@ -14,10 +14,19 @@ from .interface import (
     rope,
     swiglu, swiglu_fused,
 )
+from .logprobs import TokenLogprobs, token_logprobs
+from .paged import (
+    copy_pages,
+    page_width,
+    paged_attention,
+    paged_kv_append,
+)
 from .reference import rope_cache
 
 __all__ = [
-    "adamw_step", "can_flash_attention", "flash_attention",
-    "fused_cross_entropy", "get_ext", "has_ext", "l2norm_sq",
+    "TokenLogprobs", "adamw_step", "can_flash_attention", "copy_pages",
+    "flash_attention", "fused_cross_entropy", "get_ext", "has_ext",
+    "l2norm_sq", "page_width", "paged_attention", "paged_kv_append",
     "reference", "rmsnorm", "rope", "rope_cache", "swiglu", "swiglu_fused",
+    "token_logprobs",
 ]

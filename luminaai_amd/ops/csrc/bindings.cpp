@@ -3,10 +3,13 @@
 // reached through extern "C" launchers taking hipStream_t.
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
+#include <c10/core/DeviceGuard.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <optional>
 #include <tuple>
+#include <vector>
 
 namespace {
 
@@ -72,6 +75,11 @@ hipError_t lumina_moe_dispatch_bwd(const void*, const int64_t*, void*, int64_t, 
 hipError_t lumina_moe_combine_fwd(const void*, const float*, const int64_t*, void*, int64_t, int, int, int64_t, int, hipStream_t);
 hipError_t lumina_moe_combine_bwd_y(const void*, const float*, const int64_t*, const int64_t*, const bool*, void*, int64_t, int64_t, int, int, hipStream_t);
 hipError_t lumina_moe_combine_bwd_w(const void*, const void*, const int64_t*, float*, int64_t, int, int, int64_t, int, hipStream_t);
+hipError_t lumina_paged_attn(const void*, const void*, const void*, void*, const int*, const int*, float*, float*, const int64_t*, int64_t, int, int, int, int, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_paged_append(const void*, const void*, void*, void*, const int*, const int*, const int*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int, int, hipStream_t);
+hipError_t lumina_copy_pages(void* const*, int, const int64_t*, const int64_t*, int, int64_t, const int*, const int*, int64_t, hipStream_t);
+hipError_t lumina_logprob_fwd(const void*, int, const void*, int, float*, float*, float*, float*, int64_t*, int64_t, int, int64_t, int, int64_t, hipStream_t);
+hipError_t lumina_logprob_bwd(const void*, int, const void*, int, const float*, const float*, const float*, const float*, void*, int64_t, int, int64_t, int64_t, hipStream_t);
 }
 
 // ---- RMSNorm -------------------------------------------------------------
@@ -705,6 +713,295 @@ at::Tensor gemv(const at::Tensor& x, const at::Tensor& w) {
   return y;
 }
 
+// ---- paged cache -----------------------------------------------------------
+namespace {
+
+void check_same_device(const at::Tensor& t, const at::Tensor& first,
+                       const char* name) {
+  TORCH_CHECK_VALUE(t.device() == first.device(), name, " is on ", t.device(),
+                    ", not on ", first.device());
+}
+
+// Pages [P, HKV, page, W]; returns log2(page).
+int check_pages(const at::Tensor& t, const at::Tensor& like, const char* name,
+                int64_t heads, int64_t dim) {
+  TORCH_CHECK_VALUE(t.dim() == 4, name, " must be [pages, kv_heads, page, width]");
+  check_same_device(t, like, name);
+  TORCH_CHECK_TYPE(t.scalar_type() == like.scalar_type(), name, " is ",
+                   t.scalar_type(), ", not ", like.scalar_type());
+  const int64_t page = t.size(2), W = t.size(3);
+  TORCH_CHECK_VALUE(t.size(1) == heads, name, " has ", t.size(1),
+                    " heads, not ", heads);
+  TORCH_CHECK_VALUE(page >= 16 && page <= 4096 && (page & (page - 1)) == 0,
+                    "page size must be a power of two from 16 to 4096, got ",
+                    page);
+  TORCH_CHECK_VALUE(W % 8 == 0 && W >= dim && W < dim + 8, name,
+                    " must be head_dim rounded up to a multiple of 8 wide "
+                    "(head_dim ", dim, ", got ", W, ")");
+  TORCH_CHECK_VALUE(t.stride(3) == 1 && t.stride(2) % 8 == 0 &&
+                    t.stride(1) % 8 == 0 && t.stride(0) % 8 == 0 &&
+                    (uintptr_t)t.data_ptr() % 16 == 0,
+                    name, " rows must be contiguous and 16-byte aligned");
+  TORCH_CHECK_VALUE(t.size(0) <= INT32_MAX, name, " has too many pages");
+  int shift = 0;
+  while ((1ll << shift) < page) ++shift;
+  return shift;
+}
+
+void check_int32(const at::Tensor& t, const at::Tensor& like, int64_t dims,
+                 const char* name) {
+  check_same_device(t, like, name);
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " must be int32, got ",
+                   t.scalar_type());
+  TORCH_CHECK_VALUE(t.dim() == dims && (t.numel() == 0 ||
+                    t.stride(dims - 1) == 1), name, " must be a ", dims,
+                    "-dimensional tensor with contiguous rows");
+}
+
+}  // namespace
+
+at::Tensor paged_attn(const at::Tensor& q_, const at::Tensor& kp,
+                      const at::Tensor& vp, const at::Tensor& table,
+                      const at::Tensor& lens, double scale) {
+  TORCH_CHECK_VALUE(q_.dim() == 3, "q must be [batch, heads, head_dim]");
+  TORCH_CHECK_TYPE(is_bf16(q_), "paged_attention on the GPU takes bf16, got ",
+                   q_.scalar_type());
+  TORCH_CHECK(!(at::GradMode::is_enabled() && q_.requires_grad()),
+              "paged_attention has no gradient: call it under torch.no_grad()");
+  const c10::DeviceGuard guard(q_.device());
+  const at::Tensor q = q_.stride(2) == 1 || q_.size(2) == 1
+      ? q_ : q_.contiguous();
+  const int64_t B = q.size(0), H = q.size(1), D = q.size(2);
+  TORCH_CHECK_VALUE(kp.dim() == 4 && kp.sizes() == vp.sizes(),
+                    "k_pages and v_pages must be [pages, kv_heads, page, "
+                    "width], of one shape");
+  const int64_t HKV = kp.size(1);
+  TORCH_CHECK_VALUE(D >= 1 && D <= 192, "head_dim must be 1 to 192, got ", D);
+  TORCH_CHECK_VALUE(HKV > 0 && H > 0 && H % HKV == 0, "heads (", H,
+                    ") must be a multiple of kv_heads (", HKV, ")");
+  const int shift = check_pages(kp, q, "k_pages", HKV, D);
+  check_pages(vp, q, "v_pages", HKV, D);
+  check_int32(table, q, 2, "block_table");
+  check_int32(lens, q, 1, "seq_lens");
+  TORCH_CHECK_VALUE(table.size(0) == B && lens.size(0) == B,
+                    "block_table and seq_lens need a row for each of the ", B,
+                    " sequences");
+  const int64_t M = table.size(1), cap = M << shift;
+  TORCH_CHECK_VALUE(cap < (1ll << 31) - 4096, "block_table holds ", cap,
+                    " tokens: fewer than 2^31 - 4096 are supported");
+  auto o = at::empty({B, H, D}, q.options());
+  if (B == 0) return o;
+  if (cap == 0 || kp.size(0) == 0) return o.zero_();
+  // Chunks of the context, a workgroup each: about 1024 workgroups (four on
+  // each of the 256 units, 16 waves) where there is that much, and no fewer
+  // than 128 tokens (one step of each of its four waves).
+  const int64_t G = H / HKV, rows = B * HKV * ((G + 15) / 16);
+  int64_t chunk = 128;
+  while (chunk < 1024 && rows * cap > chunk * 1024) chunk *= 2;
+  const int64_t S = (cap + chunk - 1) / chunk;
+  at::Tensor ws;
+  float* part = nullptr;
+  float* ml = nullptr;
+  if (S > 1) {
+    ws = at::empty({B * H * S * (D + 2)}, q.options().dtype(at::kFloat));
+    ml = ws.data_ptr<float>();
+    part = ml + B * H * S * 2;
+  }
+  const int64_t strides[9] = {q.stride(0), q.stride(1), kp.stride(0),
+                              kp.stride(1), kp.stride(2), vp.stride(0),
+                              vp.stride(1), vp.stride(2), table.stride(0)};
+  check_hip(lumina_paged_attn(q.data_ptr(), kp.data_ptr(), vp.data_ptr(),
+                              o.data_ptr(), table.data_ptr<int>(),
+                              lens.data_ptr<int>(), part, ml, strides,
+                              kp.size(0), (int)B, (int)H, (int)HKV, (int)D,
+                              (int)kp.size(3), shift, (int)M, (int)chunk,
+                              (int)S, (float)scale, cur_stream()),
+            "paged_attention");
+  return o;
+}
+
+void paged_append(const at::Tensor& k_, const at::Tensor& v_,
+                  const at::Tensor& kp, const at::Tensor& vp,
+                  const at::Tensor& table, const at::Tensor& pos,
+                  const std::optional<at::Tensor>& ids) {
+  TORCH_CHECK_VALUE(k_.dim() == 3 && v_.sizes() == k_.sizes(),
+                    "k and v must be [tokens, kv_heads, head_dim]");
+  TORCH_CHECK_TYPE(k_.scalar_type() == at::kBFloat16 ||
+                   k_.scalar_type() == at::kHalf ||
+                   k_.scalar_type() == at::kFloat,
+                   "k must be bf16, fp16 or fp32, got ", k_.scalar_type());
+  check_same_device(v_, k_, "v");
+  TORCH_CHECK_TYPE(v_.scalar_type() == k_.scalar_type(), "v is ",
+                   v_.scalar_type(), ", not ", k_.scalar_type());
+  const c10::DeviceGuard guard(k_.device());
+  const int64_t T = k_.size(0), HKV = k_.size(1), D = k_.size(2);
+  const at::Tensor k = k_.stride(2) == 1 || D == 1 ? k_ : k_.contiguous();
+  const at::Tensor v = v_.stride(2) == 1 || D == 1 ? v_ : v_.contiguous();
+  TORCH_CHECK_VALUE(HKV > 0 && D > 0, "k has no heads or no channels");
+  TORCH_CHECK_VALUE(kp.sizes() == vp.sizes(),
+                    "k_pages and v_pages must be of one shape");
+  const int shift = check_pages(kp, k, "k_pages", HKV, D);
+  check_pages(vp, k, "v_pages", HKV, D);
+  check_int32(table, k, 2, "block_table");
+  check_int32(pos, k, 1, "positions");
+  TORCH_CHECK_VALUE(pos.size(0) == T, "positions has ", pos.size(0),
+                    " entries for ", T, " tokens");
+  if (ids.has_value()) {
+    check_int32(*ids, k, 1, "seq_ids");
+    TORCH_CHECK_VALUE(ids->size(0) == T, "seq_ids has ", ids->size(0),
+                      " entries for ", T, " tokens");
+  } else {
+    TORCH_CHECK_VALUE(table.size(0) == T, "without seq_ids there is one token "
+                      "for each sequence: ", T, " tokens, ", table.size(0),
+                      " sequences");
+  }
+  if (T == 0) return;
+  const int64_t strides[11] = {k.stride(0), k.stride(1), v.stride(0),
+                               v.stride(1), kp.stride(0), kp.stride(1),
+                               kp.stride(2), vp.stride(0), vp.stride(1),
+                               vp.stride(2), table.stride(0)};
+  check_hip(lumina_paged_append(k.data_ptr(), v.data_ptr(), kp.data_ptr(),
+                                vp.data_ptr(), table.data_ptr<int>(),
+                                pos.data_ptr<int>(),
+                                ids.has_value() ? ids->data_ptr<int>()
+                                                : nullptr,
+                                strides, kp.size(0), T, (int)table.size(0),
+                                (int)HKV, (int)D, (int)kp.size(3), shift,
+                                (int)table.size(1), (int)k.element_size(),
+                                cur_stream()),
+            "paged_kv_append");
+}
+
+void copy_pages(const std::vector<at::Tensor>& pools,
+                const std::vector<int64_t>& src,
+                const std::vector<int64_t>& dst) {
+  TORCH_CHECK_VALUE(src.size() == dst.size(), "src names ", src.size(),
+                    " pages, dst ", dst.size());
+  TORCH_CHECK_VALUE(!pools.empty(), "no pool was given");
+  std::vector<int64_t> s(src), d(dst);
+  std::sort(s.begin(), s.end());
+  std::sort(d.begin(), d.end());
+  for (size_t i = 1; i < d.size(); ++i)
+    TORCH_CHECK_VALUE(d[i] != d[i - 1], "page ", d[i], " is written twice");
+  for (int64_t p : d)
+    TORCH_CHECK_VALUE(!std::binary_search(s.begin(), s.end(), p), "page ", p,
+                      " is both read and written");
+  for (const auto& t : pools) {
+    TORCH_CHECK_VALUE(t.dim() >= 3, "a pool must be [layers, pages, ...]");
+    check_same_device(t, pools[0], "pool");
+    TORCH_CHECK_VALUE(t.size(0) > 0 && t.size(1) > 0 && t.numel() > 0,
+                      "a pool is empty");
+    TORCH_CHECK_VALUE(t[0][0].is_contiguous(), "a pool's pages must be "
+                      "contiguous");
+    TORCH_CHECK_VALUE(t.size(1) <= INT32_MAX, "a pool has too many pages");
+    if (!d.empty())
+      TORCH_CHECK_VALUE(s.front() >= 0 && d.front() >= 0 &&
+                        s.back() < t.size(1) && d.back() < t.size(1),
+                        "page numbers must be in 0 to ", t.size(1) - 1);
+  }
+  if (d.empty()) return;
+  const std::vector<int> si(src.begin(), src.end()), di(dst.begin(), dst.end());
+  const c10::DeviceGuard guard(pools[0].device());
+  auto page_bytes = [](const at::Tensor& t) {
+    return (int64_t)(t.numel() / (t.size(0) * t.size(1)) * t.element_size());
+  };
+  for (size_t i = 0; i < pools.size();) {
+    // two pools of the same size (keys and values) share a launch
+    const bool two = i + 1 < pools.size() &&
+        pools[i].size(0) == pools[i + 1].size(0) &&
+        page_bytes(pools[i]) == page_bytes(pools[i + 1]);
+    void* ptr[2];
+    int64_t layer[2], page[2];
+    const int n = two ? 2 : 1;
+    for (int j = 0; j < n; ++j) {
+      const auto& t = pools[i + j];
+      ptr[j] = t.data_ptr();
+      layer[j] = t.stride(0) * t.element_size();
+      page[j] = t.stride(1) * t.element_size();
+    }
+    check_hip(lumina_copy_pages(ptr, n, layer, page, (int)pools[i].size(0),
+                                page_bytes(pools[i]), si.data(), di.data(),
+                                (int64_t)si.size(), cur_stream()),
+              "copy_pages");
+    i += n;
+  }
+}
+
+// ---- token log probabilities -------------------------------------------------
+namespace {
+int logit_dtype(const at::Tensor& t) {
+  if (t.scalar_type() == at::kBFloat16) return 0;
+  if (t.scalar_type() == at::kHalf) return 1;
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat,
+                   "logits must be bf16, fp16 or fp32, got ", t.scalar_type());
+  return 2;
+}
+}  // namespace
+
+// logits [N, V] with contiguous rows. stat [N, 2] (row maximum, log2 of the sum)
+// is what the gradient needs; empty where want_stat is false.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+logprob_fwd(const at::Tensor& x, const at::Tensor& tok, int64_t k,
+            int64_t ignore, bool want_stat) {
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) > 0 &&
+                    (x.stride(1) == 1 || x.size(1) == 1),
+                    "logits must be [rows, vocab] with contiguous rows");
+  const int dtype = logit_dtype(x);
+  check_same_device(tok, x, "tokens");
+  TORCH_CHECK_TYPE(tok.scalar_type() == at::kLong ||
+                   tok.scalar_type() == at::kInt,
+                   "tokens must be int64 or int32, got ", tok.scalar_type());
+  const int64_t N = x.size(0), V = x.size(1);
+  TORCH_CHECK_VALUE(tok.dim() == 1 && tok.size(0) == N && tok.is_contiguous(),
+                    "tokens must hold one token for each of the ", N, " rows");
+  TORCH_CHECK_VALUE(V <= INT32_MAX - 8 && N <= INT32_MAX,
+                    "logits of ", N, " x ", V, " are not supported");
+  TORCH_CHECK_VALUE(k >= 0 && k <= 64 && k <= V, "top_k must be 0 to 64 and at "
+                    "most the vocabulary's ", V, ", got ", k);
+  const c10::DeviceGuard guard(x.device());
+  const auto f32 = x.options().dtype(at::kFloat);
+  auto lp = at::empty({N}, f32), ent = at::empty({N}, f32);
+  auto stat = at::empty({want_stat ? N : 0, 2}, f32);
+  auto tl = at::empty({N, k}, f32);
+  auto ti = at::empty({N, k}, x.options().dtype(at::kLong));
+  if (N > 0)
+    check_hip(lumina_logprob_fwd(x.data_ptr(), dtype, tok.data_ptr(),
+                                 tok.scalar_type() == at::kLong,
+                                 lp.data_ptr<float>(), ent.data_ptr<float>(),
+                                 want_stat ? stat.data_ptr<float>() : nullptr,
+                                 tl.data_ptr<float>(), ti.data_ptr<int64_t>(),
+                                 N, (int)V, x.stride(0), (int)k, ignore,
+                                 cur_stream()), "token_logprobs");
+  return {lp, ent, tl, ti, stat};
+}
+
+at::Tensor logprob_bwd(const at::Tensor& x, const at::Tensor& tok,
+                       const at::Tensor& stat, const at::Tensor& ent,
+                       const std::optional<at::Tensor>& g_lp,
+                       const std::optional<at::Tensor>& g_ent,
+                       int64_t ignore) {
+  const int dtype = logit_dtype(x);
+  const int64_t N = x.size(0), V = x.size(1);
+  const c10::DeviceGuard guard(x.device());
+  auto grad = [&](const std::optional<at::Tensor>& g) -> const float* {
+    if (!g.has_value()) return nullptr;
+    TORCH_CHECK_VALUE(g->scalar_type() == at::kFloat && g->is_contiguous() &&
+                      g->numel() == N && g->device() == x.device(),
+                      "a gradient must be fp32 and contiguous, one for each row");
+    return g->data_ptr<float>();
+  };
+  auto dx = at::empty({N, V}, x.options());
+  if (N > 0)
+    check_hip(lumina_logprob_bwd(x.data_ptr(), dtype, tok.data_ptr(),
+                                 tok.scalar_type() == at::kLong,
+                                 stat.data_ptr<float>(),
+                                 ent.data_ptr<float>(), grad(g_lp),
+                                 grad(g_ent), dx.data_ptr(), N, (int)V,
+                                 x.stride(0), ignore, cur_stream()),
+              "token_logprobs gradient");
+  return dx;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("attn_fwd", &attn_fwd,
           "causal GQA flash attention forward -> (O, LSE2) (gfx950)");
@@ -760,4 +1057,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("ce_bwd", &ce_bwd, "fused CE backward (gfx950)");
   mod.def("l2norm_sq", &l2norm_sq, "flat L2 norm squared (gfx950)");
   mod.def("adamw_step", &adamw_step, "fused clip+AdamW on flat buffers (gfx950)");
+  mod.def("paged_attn", &paged_attn, "single-token attention over pages");
+  mod.def("paged_append", &paged_append, "append keys and values to pages");
+  mod.def("copy_pages", &copy_pages, "copy pages within pools");
+  mod.def("logprob_fwd", &logprob_fwd, "token log probabilities and entropy");
+  mod.def("logprob_bwd", &logprob_bwd, "gradient of logprob_fwd");
 }

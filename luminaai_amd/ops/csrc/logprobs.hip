@@ -1,0 +1,376 @@
+// Log probabilities of given tokens, entropy and the most likely
+// alternatives of each row of logits, and the gradient, for CDNA4 (gfx950).
+//
+//   lp = x_t - lse      H = lse - sum_j p_j x_j      p_j = exp(x_j - lse)
+//   dx_j = g_lp (1[j = t] - p_j) - g_H p_j (log p_j + H)
+//
+// A workgroup takes a row and reads it once: each thread keeps a running
+// maximum m, the sum of 2^y and the sum of y 2^y with y = (x - m) log2(e). The
+// difference is taken first: it is exact near the maximum and cannot overflow
+// at a mask of the type's lowest value. The kernel is bound by the bytes of the
+// logits, with the exponentials close behind.
+//
+// Alternatives: the k-th largest of 64 group maxima is a lower bound of
+// the k-th largest logit, so only threads whose own maximum reaches it look at
+// their elements again (from L2) and put the candidates into LDS, where each is
+// ranked by counting. Ties go to the lowest index: value and index make one
+// 64-bit key. Rows with more candidates than fit (many equal logits) take
+// k rounds of a maximum over the row.
+#include "common.h"
+
+#define LOG2E 1.4426950408889634f
+#define LN2 0.6931471805599453f
+#define LP_MAX_K 64
+#define LP_CAP 1024            // candidates that fit into LDS
+
+template <typename S> struct Vec8;
+template <> struct Vec8<uint16_t> { uint16_t v[8]; };
+template <> struct Vec8<float> { float v[8]; };
+
+struct BF16In {
+  using S = uint16_t;
+  static DEV_INLINE float get(uint16_t u) { return bf16_to_f32(u); }
+  static DEV_INLINE uint16_t put(float f) { return f32_to_bf16(f); }
+};
+struct F16In {
+  using S = uint16_t;
+  static DEV_INLINE float get(uint16_t u) {
+    return (float)__builtin_bit_cast(_Float16, u);
+  }
+  static DEV_INLINE uint16_t put(float f) {
+    return __builtin_bit_cast(uint16_t, (_Float16)f);
+  }
+};
+struct F32In {
+  using S = float;
+  static DEV_INLINE float get(float f) { return f; }
+  static DEV_INLINE float put(float f) { return f; }
+};
+
+// rows start at any element: memcpy leaves the choice of the load to the
+// compiler, which takes 16-byte loads (global memory takes any alignment)
+template <typename S>
+DEV_INLINE Vec8<S> load8(const S* p) {
+  Vec8<S> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+
+// orders floats as unsigned numbers; NaN above all, the two zeros equal
+DEV_INLINE uint32_t order_key(float f) {
+  if (f != f) return 0xffffffffu;
+  const uint32_t u = __builtin_bit_cast(uint32_t, f + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+DEV_INLINE uint64_t pair_key(float f, int idx) {
+  return ((uint64_t)order_key(f) << 32) | (uint32_t)~idx;
+}
+
+struct RowState { float m, s, t; };   // maximum, sum 2^y, sum y 2^y
+
+DEV_INLINE RowState join(RowState a, RowState b) {
+  if (b.s == 0.f) return a;
+  if (a.s == 0.f) return b;
+  RowState r;
+  r.m = fmaxf(a.m, b.m);
+  const float da = (a.m - r.m) * LOG2E, db = (b.m - r.m) * LOG2E;
+  const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+  r.s = a.s * fa + b.s * fb;
+  // a difference past the type's range has factor 0: -1e30 keeps 0 * inf out
+  r.t = fa * (a.t + a.s * fmaxf(da, -1e30f))
+        + fb * (b.t + b.s * fmaxf(db, -1e30f));
+  return r;
+}
+
+struct LogprobArgs {
+  const void* x;
+  const void* tok;
+  float* lp;
+  float* ent;
+  float* stat;                 // [N, 2]: row maximum, log2 of sum exp(x - max)
+  float* top_lp;
+  int64_t* top_id;
+  int64_t N, row_stride;
+  int64_t ignore;
+  int V, k, tok64;
+};
+
+DEV_INLINE int64_t token_of(const void* tok, int is64, int64_t row) {
+  return is64 ? reinterpret_cast<const int64_t*>(tok)[row]
+              : (int64_t)reinterpret_cast<const int32_t*>(tok)[row];
+}
+
+template <typename E, int BLOCK, bool TOP>
+__global__ __launch_bounds__(BLOCK)
+void logprob_fwd_kernel(const LogprobArgs a) {
+  using S = typename E::S;
+  constexpr int NW = BLOCK / 64;
+  __shared__ float red[NW][3];
+  __shared__ float gmax[TOP ? NW : 1][64];
+  __shared__ uint64_t cand[TOP ? LP_CAP : 1];
+  __shared__ uint64_t best[NW];
+  __shared__ int n_cand;
+  __shared__ float thr;
+
+  const int64_t row = blockIdx.x;
+  const S* x = reinterpret_cast<const S*>(a.x) + row * a.row_stride;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int nvec = a.V >> 3;
+
+  float mx = -INFINITY, ref = 0.f, s = 0.f, t = 0.f;
+  auto take = [&](const float* f, int n) {
+    float cm = f[0];
+    #pragma unroll
+    for (int j = 1; j < n; ++j) cm = fmaxf(cm, f[j]);
+    if (cm > mx) {
+      // the reference is 0 while all is -inf (inf - inf otherwise): s is 0
+      if (mx > -INFINITY) {
+        const float d = (mx - cm) * LOG2E, sc = __builtin_amdgcn_exp2f(d);
+        t = sc * (t + s * fmaxf(d, -1e30f));
+        s *= sc;
+      }
+      ref = mx = cm;
+    }
+    #pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const float y = (f[j] - ref) * LOG2E;
+      const float e = __builtin_amdgcn_exp2f(y);
+      s += e;
+      t = __builtin_fmaf(e, fmaxf(y, -200.f), t);   // 0 * -inf is 0 here
+    }
+  };
+  constexpr int U = sizeof(S) == 2 ? 4 : 2;
+  int i = threadIdx.x;
+  for (; i + (U - 1) * BLOCK < nvec; i += U * BLOCK) {
+    Vec8<S> v[U];
+    #pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = load8(x + 8 * (int64_t)(i + u * BLOCK));
+    float f[8 * U];
+    #pragma unroll
+    for (int u = 0; u < U; ++u)
+      #pragma unroll
+      for (int j = 0; j < 8; ++j) f[8 * u + j] = E::get(v[u].v[j]);
+    take(f, 8 * U);
+  }
+  for (; i < nvec; i += BLOCK) {
+    const Vec8<S> v = load8(x + 8 * (int64_t)i);
+    float f[8];
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = E::get(v.v[j]);
+    take(f, 8);
+  }
+  const int tail = 8 * nvec + threadIdx.x;
+  if (tail < a.V) {
+    const float f = E::get(x[tail]);
+    take(&f, 1);
+  }
+
+  // ---- the row's state, joined in a fixed order
+  RowState st = {mx, s, t};
+  #pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    RowState b = {__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64),
+                  __shfl_xor(st.t, o, 64)};
+    st = lane & o ? join(b, st) : join(st, b);
+  }
+  if (lane == 0) {
+    red[wave][0] = st.m; red[wave][1] = st.s; red[wave][2] = st.t;
+  }
+  if (TOP) gmax[wave][lane] = mx;
+  if (threadIdx.x == 0) n_cand = 0;
+  __syncthreads();
+  RowState r = {red[0][0], red[0][1], red[0][2]};
+  #pragma unroll
+  for (int w = 1; w < NW; ++w)
+    r = join(r, RowState{red[w][0], red[w][1], red[w][2]});
+  // a row of nothing but -inf has no distribution: NaN, as -inf - -inf
+  if (r.s == 0.f) r.s = __builtin_nanf("");
+  const float ls = __builtin_log2f(r.s);
+  if (threadIdx.x == 0) {
+    const int64_t tk = token_of(a.tok, a.tok64, row);
+    float lp = __builtin_nanf("");         // a token outside the vocabulary
+    if (tk == a.ignore) lp = 0.f;
+    else if (tk >= 0 && tk < a.V)
+      lp = E::get(x[tk]) - r.m - LN2 * ls;
+    a.lp[row] = lp;
+    a.ent[row] = LN2 * (ls - r.t / r.s);
+    if (a.stat) {
+      a.stat[2 * row] = r.m;
+      a.stat[2 * row + 1] = ls;
+    }
+  }
+  if (!TOP) return;
+
+  if (wave == 0) {
+    float g = gmax[0][lane];
+    #pragma unroll
+    for (int w = 1; w < NW; ++w) g = fmaxf(g, gmax[w][lane]);
+    int rank = 0;
+    for (int j = 0; j < 64; ++j) {
+      const float o = __shfl(g, j, 64);
+      rank += (o > g || (o == g && j < lane)) ? 1 : 0;
+    }
+    if (rank == a.k - 1) thr = g;
+  }
+  __syncthreads();
+  const float T = thr;
+  if (mx >= T || s != s) {
+    for (int q = threadIdx.x; q < nvec; q += BLOCK) {
+      const Vec8<S> v = load8(x + 8 * (int64_t)q);
+      #pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float f = E::get(v.v[j]);
+        if (!(f < T)) {
+          const int at = atomicAdd(&n_cand, 1);
+          if (at < LP_CAP) cand[at] = pair_key(f, 8 * q + j);
+        }
+      }
+    }
+    if (tail < a.V) {
+      const float f = E::get(x[tail]);
+      if (!(f < T)) {
+        const int at = atomicAdd(&n_cand, 1);
+        if (at < LP_CAP) cand[at] = pair_key(f, tail);
+      }
+    }
+  }
+  __syncthreads();
+  auto put = [&](int rank, uint64_t key) {
+    const int idx = (int)~(uint32_t)key;
+    a.top_id[row * a.k + rank] = idx;
+    a.top_lp[row * a.k + rank] =
+        E::get(x[idx]) - r.m - LN2 * ls;
+  };
+  const int n = n_cand;
+  if (n <= LP_CAP) {
+    for (int c = threadIdx.x; c < n; c += BLOCK) {
+      const uint64_t key = cand[c];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += cand[j] > key ? 1 : 0;
+      if (rank < a.k) put(rank, key);
+    }
+    return;
+  }
+  uint64_t prev = ~0ull;                 // above every key: indexes are >= 0
+  for (int rank = 0; rank < a.k; ++rank) {
+    uint64_t b = 0;
+    for (int q = threadIdx.x; q < a.V; q += BLOCK) {
+      const uint64_t key = pair_key(E::get(x[q]), q);
+      if (key < prev && key > b) b = key;
+    }
+    #pragma unroll
+    for (int o = 32; o; o >>= 1) {
+      const uint64_t other = __shfl_xor((unsigned long long)b, o, 64);
+      b = other > b ? other : b;
+    }
+    __syncthreads();                     // the last round's reads are done
+    if (lane == 0) best[wave] = b;
+    __syncthreads();
+    #pragma unroll
+    for (int w = 0; w < NW; ++w) b = best[w] > b ? best[w] : b;
+    prev = b;
+    if (threadIdx.x == 0) put(rank, b);
+  }
+}
+
+struct LogprobBwdArgs {
+  const void* x;
+  const void* tok;
+  const float* stat;
+  const float* ent;
+  const float* g_lp;           // null: zero
+  const float* g_ent;          // null: zero
+  void* dx;                    // [N, V]
+  int64_t N, row_stride, ignore;
+  int V, pieces, tok64;
+};
+
+#define LP_BWD_VECS 1024       // vectors of 8 that a workgroup takes
+
+// Elementwise over a row's saved maximum and sum: reads x once, writes dx once.
+template <typename E>
+__global__ __launch_bounds__(256)
+void logprob_bwd_kernel(const LogprobBwdArgs a) {
+  using S = typename E::S;
+  const int64_t row = blockIdx.x / a.pieces;
+  const int piece = (int)(blockIdx.x - row * a.pieces);
+  const S* x = reinterpret_cast<const S*>(a.x) + row * a.row_stride;
+  S* dx = reinterpret_cast<S*>(a.dx) + row * (int64_t)a.V;
+  const float mx = a.stat[2 * row], ls = a.stat[2 * row + 1];
+  const float H = a.ent[row];
+  const int64_t tk = token_of(a.tok, a.tok64, row);
+  float gl = a.g_lp ? a.g_lp[row] : 0.f;
+  const float ge = a.g_ent ? a.g_ent[row] : 0.f;
+  int hot = -1;
+  if (tk == a.ignore) gl = 0.f;
+  else if (tk >= 0 && tk < a.V) hot = (int)tk;
+  else gl = __builtin_nanf("");
+  // -p (gl + ge (ln2 y + H)) with y = log2 p
+  const float c0 = -(gl + ge * H), c1 = -ge * LN2;
+  auto grad = [&](float f, int idx) {
+    const float y = __builtin_fmaf(f - mx, LOG2E, -ls);
+    const float p = __builtin_amdgcn_exp2f(y);
+    const float d = p * __builtin_fmaf(c1, fmaxf(y, -200.f), c0);
+    return idx == hot ? d + gl : d;
+  };
+  const int nvec = a.V >> 3;
+  const int v0 = piece * LP_BWD_VECS;
+  const int v1 = v0 + LP_BWD_VECS < nvec ? v0 + LP_BWD_VECS : nvec;
+  for (int i = v0 + threadIdx.x; i < v1; i += 256) {
+    const Vec8<S> v = load8(x + 8 * (int64_t)i);
+    Vec8<S> o;
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) o.v[j] = E::put(grad(E::get(v.v[j]), 8 * i + j));
+    __builtin_memcpy(dx + 8 * (int64_t)i, &o, sizeof(o));
+  }
+  const int tail = 8 * nvec + threadIdx.x;
+  if (piece == a.pieces - 1 && tail < a.V)
+    dx[tail] = E::put(grad(E::get(x[tail]), tail));
+}
+
+template <typename E, int BLOCK>
+static void fwd_launch(const LogprobArgs& a, hipStream_t stream) {
+  const dim3 grid((uint32_t)a.N), block(BLOCK);
+  if (a.k > 0)
+    logprob_fwd_kernel<E, BLOCK, true><<<grid, block, 0, stream>>>(a);
+  else
+    logprob_fwd_kernel<E, BLOCK, false><<<grid, block, 0, stream>>>(a);
+}
+
+// dtype: 0 bf16, 1 fp16, 2 fp32
+extern "C" hipError_t lumina_logprob_fwd(
+    const void* x, int dtype, const void* tok, int tok64, float* lp,
+    float* ent, float* stat, float* top_lp, int64_t* top_id, int64_t N, int V,
+    int64_t row_stride, int k, int64_t ignore, hipStream_t stream) {
+  if (N > 0x7fffffff || k > LP_MAX_K) return hipErrorInvalidValue;
+  LogprobArgs a;
+  a.x = x; a.tok = tok; a.lp = lp; a.ent = ent; a.stat = stat;
+  a.top_lp = top_lp; a.top_id = top_id; a.N = N; a.row_stride = row_stride;
+  a.ignore = ignore; a.V = V; a.k = k; a.tok64 = tok64;
+  if (dtype == 0) fwd_launch<BF16In, 512>(a, stream);
+  else if (dtype == 1) fwd_launch<F16In, 512>(a, stream);
+  else if (dtype == 2) fwd_launch<F32In, 512>(a, stream);
+  else return hipErrorInvalidValue;
+  HIP_CHECK_LAST();
+  return hipSuccess;
+}
+
+extern "C" hipError_t lumina_logprob_bwd(
+    const void* x, int dtype, const void* tok, int tok64, const float* stat,
+    const float* ent, const float* g_lp, const float* g_ent, void* dx,
+    int64_t N, int V, int64_t row_stride, int64_t ignore, hipStream_t stream) {
+  LogprobBwdArgs a;
+  a.x = x; a.tok = tok; a.stat = stat; a.ent = ent; a.g_lp = g_lp;
+  a.g_ent = g_ent; a.dx = dx; a.N = N; a.row_stride = row_stride;
+  a.ignore = ignore; a.V = V; a.tok64 = tok64;
+  const int nvec = V / 8;
+  a.pieces = nvec > LP_BWD_VECS ? (nvec + LP_BWD_VECS - 1) / LP_BWD_VECS : 1;
+  if (N * a.pieces > 0x7fffffff) return hipErrorInvalidValue;
+  const dim3 grid((uint32_t)(N * a.pieces)), block(256);
+  if (dtype == 0) logprob_bwd_kernel<BF16In><<<grid, block, 0, stream>>>(a);
+  else if (dtype == 1) logprob_bwd_kernel<F16In><<<grid, block, 0, stream>>>(a);
+  else if (dtype == 2) logprob_bwd_kernel<F32In><<<grid, block, 0, stream>>>(a);
+  else return hipErrorInvalidValue;
+  HIP_CHECK_LAST();
+  return hipSuccess;
+}

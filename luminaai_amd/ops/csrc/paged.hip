@@ -1,0 +1,538 @@
+// Paged key/value cache for CDNA4 (gfx950): single-token attention over pages,
+// appending new keys and values, and copying pages.
+//
+// A pool holds pages [P, HKV, page, W] (bf16 for attention): W is head_dim
+// padded to a multiple of 8, `page` a power of two >= 16. A sequence is a
+// row of page numbers and a length. Strides are arguments, so a layer's slice
+// of a pool over all layers works as it is.
+#include "common.h"
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) float  floatx2;
+
+#define LOG2E 1.4426950408889634f
+
+// Eight elements from an address that is only element-aligned; elements at
+// and after n are zero. The full load is one 16-byte global load: gfx950 takes
+// any alignment there.
+DEV_INLINE ushortx8 load8_guarded(const uint16_t* p, int n) {
+  ushortx8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (n >= 8) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+    #pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) v[j] = p[j];
+  }
+  return v;
+}
+
+DEV_INLINE uint32_t pack_bf16(float lo, float hi) {
+  floatx2 f = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
+}
+
+// ===========================================================================
+// Attention of one new token per sequence.
+//
+//   o[h] = sum_t softmax_t(scale * q[h] . k[t]) v[t],  t < seq_len
+//
+// Bound by the bytes of K and V, so nothing is staged: a wave takes 32 tokens
+// a step straight from global memory into matrix operands.
+//   S^T = K Q^T   mfma 16x16x32, A = 16 tokens x 32 channels (a lane's 16-byte
+//                 load is its fragment), B = the group's heads (G <= 16).
+//                 The result has head = lane & 15 and tokens in registers,
+//                 4 g + r of each 16-token tile (g = lane >> 4).
+//   O^T = V^T P^T contracts over tokens, whose order is free as long as P and
+//                 V agree: lane group g takes tokens {4g..4g+3} of both tiles,
+//                 which is what it already holds of P. V rows are loaded
+//                 whole (16 lanes x NDW dwords) and the eight tokens of one
+//                 channel are put together with one byte permute per two.
+// Softmax state and the O accumulator are lane-local in the head. The running
+// maximum moves only when it grew by more than 2^8, so most steps need no
+// cross-lane traffic. P enters the product as a bf16 pair hi + lo (16 bits of
+// mantissa): the matrix pipe is idle anyway, and the result's error is
+// that of its own rounding.
+//
+// Work is split over the context in chunks of `chunk` tokens; a sequence that
+// fits one chunk is finished here, the others are joined by
+// paged_attn_join_kernel in the order of their chunks.
+// ===========================================================================
+struct PagedAttnArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* o;
+  const int* table;
+  const int* lens;
+  float* part;                 // [B, H, S, D] unnormalised partial outputs
+  float* ml;                   // [B, H, S, 2] their maximum and sum
+  int64_t q_sb, q_sh;          // strides in elements
+  int64_t k_sp, k_sh, k_st;
+  int64_t v_sp, v_sh, v_st;
+  int64_t table_sb;
+  int64_t P;
+  int B, H, HKV, D, W, page_shift, M, chunk, S, HG;
+  float scale2;                // scale * log2(e)
+};
+
+DEV_INLINE int clampi(int x, int lo, int hi) {
+  return x < lo ? lo : (x > hi ? hi : x);
+}
+
+template <int NDW>             // W <= 32 * NDW
+__global__ __launch_bounds__(256, 2)
+void paged_attn_kernel(const PagedAttnArgs a) {
+  extern __shared__ float lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = a.H / a.HKV;
+
+  // workgroup -> (sequence, chunk, kv head, group of 16 heads); neighbours
+  // share a chunk's pages
+  int64_t id = blockIdx.x;
+  const int hg = (int)(id % a.HG);
+  id /= a.HG;
+  const int hkv = (int)(id % a.HKV);
+  id /= a.HKV;
+  const int split = (int)(id % a.S);
+  const int b = (int)(id / a.S);
+
+  // a length longer than the table's row is cut to it
+  const int cap = a.M << a.page_shift;
+  const int len = clampi(a.lens[b], 0, cap);
+  const int t_begin = split * a.chunk;
+  if (t_begin >= len && split > 0) return;
+  const int t_end = len < t_begin + a.chunk ? len : t_begin + a.chunk;
+
+  const int g = lane >> 4, c16 = lane & 15;
+  const int gh = hg * 16 + c16;            // this lane's head in the group
+  const bool head_ok = gh < G;
+  const int h = hkv * G + (head_ok ? gh : 0);
+
+  bf16x8 qf[NDW];
+  {
+    const uint16_t* qp = a.q + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh;
+    #pragma unroll
+    for (int ks = 0; ks < NDW; ++ks) {
+      const int d0 = 32 * ks + 8 * g;
+      qf[ks] = __builtin_bit_cast(
+          bf16x8, load8_guarded(qp + (d0 < a.D ? d0 : 0),
+                                head_ok ? a.D - d0 : 0));
+    }
+  }
+  // channels past head_dim in K's last 8 may hold anything: cut them
+  uintx4 kmask;
+  #pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int left = a.D - (a.D & ~7) - 2 * j;
+    kmask[j] = left >= 2 ? 0xffffffffu : (left == 1 ? 0xffffu : 0u);
+  }
+
+  // channels of O: this lane loads dwords [off, off + NDW) of a V row; lanes
+  // past the row's end repeat its last ones
+  const int off = clampi(NDW * c16, 0, a.W / 2 - NDW);
+
+  floatx4 oacc[2 * NDW];
+  #pragma unroll
+  for (int i = 0; i < 2 * NDW; ++i) oacc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float m = -1e30f, l = 0.f;
+  const int* tb = a.table + (int64_t)b * a.table_sb;
+  const int pmask = (1 << a.page_shift) - 1;
+  const uint16_t* kh = a.k + hkv * a.k_sh;
+  const uint16_t* vh = a.v + hkv * a.v_sh;
+
+  for (int t0 = t_begin + 32 * wave; t0 < t_end; t0 += 128) {
+    // tokens at and after the end repeat the last live one: nothing behind
+    // a sequence is read, and its score is set to -inf below
+    uintx4 kr[2][NDW];
+    uint32_t vr[8][NDW];
+    bool ok[2];
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int last = t_end - 1;
+      const int tt = t0 + 16 * i <= last ? t0 + 16 * i : (last & ~15);
+      const int pg = tb[tt >> a.page_shift];
+      ok[i] = pg >= 0 && pg < a.P;
+      const int64_t pgc = ok[i] ? pg : 0;
+      const uint16_t* kp = kh + pgc * a.k_sp;
+      const uint16_t* vp = vh + pgc * a.v_sp;
+      const int tk = tt + c16 <= last ? tt + c16 : last;
+      const uint16_t* krow = kp + (int64_t)(tk & pmask) * a.k_st;
+      #pragma unroll
+      for (int ks = 0; ks < NDW; ++ks) {
+        const int d0 = 32 * ks + 8 * g;
+        kr[i][ks] = *reinterpret_cast<const uintx4*>(
+            krow + (d0 < a.W ? d0 : 0));
+      }
+      #pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int tv = tt + 4 * g + r <= last ? tt + 4 * g + r : last;
+        const uint16_t* vrow = vp + (int64_t)(tv & pmask) * a.v_st + 2 * off;
+        __builtin_memcpy(vr[4 * i + r], __builtin_assume_aligned(vrow, 4),
+                         4 * NDW);
+      }
+    }
+    floatx4 st[2];
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      st[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+      #pragma unroll
+      for (int ks = 0; ks < NDW; ++ks) {
+        const int d0 = 32 * ks + 8 * g;
+        uintx4 kf = kr[i][ks];
+        if (d0 >= a.D) kf = uintx4{0u, 0u, 0u, 0u};
+        else if (d0 + 8 > a.D) kf &= kmask;
+        st[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8, kf), qf[ks], st[i], 0, 0, 0);
+      }
+    }
+    float s[8];
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int t = t0 + 16 * (j >> 2) + 4 * g + (j & 3);
+      const float x = st[j >> 2][j & 3] * a.scale2;
+      s[j] = t < t_end && ok[j >> 2] ? x : -INFINITY;
+    }
+    if (!(ok[0] && ok[1])) {
+      // a page number outside the pool: its tokens are left out
+      #pragma unroll
+      for (int j = 0; j < 8; ++j)
+        #pragma unroll
+        for (int w = 0; w < NDW; ++w)
+          vr[j][w] = ok[j >> 2] ? vr[j][w] : 0u;
+    }
+    float pm = s[0];
+    #pragma unroll
+    for (int j = 1; j < 8; ++j) pm = fmaxf(pm, s[j]);
+    if (__any(pm > m + 8.f)) {
+      pm = fmaxf(pm, __shfl_xor(pm, 16, 64));
+      pm = fmaxf(pm, __shfl_xor(pm, 32, 64));
+      const float mn = fmaxf(m, pm);
+      const float alpha = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+      #pragma unroll
+      for (int i = 0; i < 2 * NDW; ++i) oacc[i] *= alpha;
+    }
+    uint32_t ph[4], pl[4];
+    #pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(s[j] - m), p1 = __builtin_amdgcn_exp2f(s[j + 1] - m);
+      l += p0 + p1;
+      const uint32_t u = pack_bf16(p0, p1);
+      ph[j / 2] = u;
+      pl[j / 2] = pack_bf16(p0 - __builtin_bit_cast(float, u << 16),
+                            p1 - __builtin_bit_cast(float, u & 0xffff0000u));
+    }
+    const bf16x8 pfh = __builtin_bit_cast(bf16x8, uintx4{ph[0], ph[1], ph[2], ph[3]});
+    const bf16x8 pfl = __builtin_bit_cast(bf16x8, uintx4{pl[0], pl[1], pl[2], pl[3]});
+    #pragma unroll
+    for (int w = 0; w < NDW; ++w) {
+      #pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uintx4 u;
+        #pragma unroll
+        for (int j = 0; j < 4; ++j)
+          u[j] = __builtin_amdgcn_perm(vr[2 * j + 1][w], vr[2 * j][w],
+                                       e ? 0x07060302u : 0x05040100u);
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, u);
+        oacc[2 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            vf, pfl, oacc[2 * w + e], 0, 0, 0);
+        oacc[2 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            vf, pfh, oacc[2 * w + e], 0, 0, 0);
+      }
+    }
+  }
+
+  // ---- join the four waves: LDS holds [wave][head of 16][2 + D]
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  const int nh = G - hg * 16 < 16 ? G - hg * 16 : 16;
+  const int rowf = a.D + 2;
+  if (c16 < nh) {
+    float* row = lds + ((int64_t)wave * nh + c16) * rowf;
+    if (g == 0) { row[0] = m; row[1] = l; }
+    #pragma unroll
+    for (int i = 0; i < 2 * NDW; ++i)
+      #pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 2 * clampi(NDW * (4 * g + r), 0, a.W / 2 - NDW) + i;
+        if (d < a.D) row[2 + d] = oacc[i][r];
+      }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nh * a.D; i += 256) {
+    const int hh = i / a.D, d = i - hh * a.D;
+    float mw[4], mm = -1e30f;
+    #pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      mw[w] = lds[(w * nh + hh) * rowf];
+      mm = fmaxf(mm, mw[w]);
+    }
+    float ls = 0.f, os = 0.f;
+    #pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(mw[w] - mm);
+      ls += f * lds[(w * nh + hh) * rowf + 1];
+      os += f * lds[(w * nh + hh) * rowf + 2 + d];
+    }
+    const int head = hkv * G + hg * 16 + hh;
+    const int64_t bh = (int64_t)b * a.H + head;
+    if (len <= a.chunk) {
+      // an empty sequence gives zeros
+      a.o[bh * a.D + d] = f32_to_bf16(ls == 0.f ? 0.f : os / ls);
+    } else {
+      a.part[(bh * a.S + split) * a.D + d] = os;
+      if (d == 0) {
+        a.ml[(bh * a.S + split) * 2] = mm;
+        a.ml[(bh * a.S + split) * 2 + 1] = ls;
+      }
+    }
+  }
+}
+
+// Joins the chunks of one (sequence, head), always in the same order.
+__global__ __launch_bounds__(256)
+void paged_attn_join_kernel(const PagedAttnArgs a) {
+  __shared__ float so[4][192], sl[4];
+  const int64_t bh = blockIdx.x;
+  const int b = (int)(bh / a.H);
+  const int len = clampi(a.lens[b], 0, a.M << a.page_shift);
+  if (len <= a.chunk) return;                  // finished by its only chunk
+  const int n = (len + a.chunk - 1) / a.chunk;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float* ml = a.ml + bh * a.S * 2;
+  const float* part = a.part + bh * a.S * a.D;
+  float m = -1e30f;
+  for (int s = lane; s < n; s += 64) m = fmaxf(m, ml[2 * s]);
+  #pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  float l = 0.f, acc[3] = {0.f, 0.f, 0.f};
+  for (int s = wave; s < n; s += 4) {
+    const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m);
+    l += f * ml[2 * s + 1];
+    #pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const int d = lane + 64 * i;
+      if (d < a.D) acc[i] += f * part[(int64_t)s * a.D + d];
+    }
+  }
+  #pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (lane + 64 * i < a.D) so[wave][lane + 64 * i] = acc[i];
+  if (lane == 0) sl[wave] = l;
+  __syncthreads();
+  const float ls = ((sl[0] + sl[1]) + sl[2]) + sl[3];
+  for (int d = threadIdx.x; d < a.D; d += 256) {
+    const float os = ((so[0][d] + so[1][d]) + so[2][d]) + so[3][d];
+    a.o[bh * a.D + d] = f32_to_bf16(ls == 0.f ? 0.f : os / ls);
+  }
+}
+
+extern "C" hipError_t lumina_paged_attn(
+    const void* q, const void* k, const void* v, void* o, const int* table,
+    const int* lens, float* part, float* ml, const int64_t* strides, int64_t P,
+    int B, int H, int HKV, int D, int W, int page_shift, int M, int chunk,
+    int S, float scale, hipStream_t stream) {
+  PagedAttnArgs a;
+  a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
+  a.o = (uint16_t*)o; a.table = table; a.lens = lens; a.part = part; a.ml = ml;
+  a.q_sb = strides[0]; a.q_sh = strides[1];
+  a.k_sp = strides[2]; a.k_sh = strides[3]; a.k_st = strides[4];
+  a.v_sp = strides[5]; a.v_sh = strides[6]; a.v_st = strides[7];
+  a.table_sb = strides[8];
+  a.P = P; a.B = B; a.H = H; a.HKV = HKV; a.D = D; a.W = W;
+  a.page_shift = page_shift; a.M = M; a.chunk = chunk; a.S = S;
+  const int G = H / HKV;
+  a.HG = (G + 15) / 16;
+  a.scale2 = scale * LOG2E;
+  const int64_t blocks = (int64_t)B * S * HKV * a.HG;
+  if (blocks > 0x7fffffff || (int64_t)B * H > 0x7fffffff)
+    return hipErrorInvalidValue;
+  const int nh = G < 16 ? G : 16;
+  const size_t lds = 4 * (size_t)nh * (D + 2) * sizeof(float);
+  const dim3 grid((uint32_t)blocks), block(256);
+  switch ((W + 31) / 32) {
+    case 1:
+    case 2: paged_attn_kernel<2><<<grid, block, lds, stream>>>(a); break;
+    case 3: paged_attn_kernel<3><<<grid, block, lds, stream>>>(a); break;
+    case 4: paged_attn_kernel<4><<<grid, block, lds, stream>>>(a); break;
+    case 5: paged_attn_kernel<5><<<grid, block, lds, stream>>>(a); break;
+    case 6: paged_attn_kernel<6><<<grid, block, lds, stream>>>(a); break;
+    default: return hipErrorInvalidValue;
+  }
+  HIP_CHECK_LAST();
+  if (S > 1) {
+    paged_attn_join_kernel<<<dim3((uint32_t)((int64_t)B * H)), block, 0,
+                             stream>>>(a);
+    HIP_CHECK_LAST();
+  }
+  return hipSuccess;
+}
+
+// ===========================================================================
+// Appending: k_pages[page(t), h, row(t), :] = k[t, h, :], zero past head_dim,
+// and the same for v. A thread writes 8 elements of a row. Bound by bytes;
+// small calls by the launch.
+// ===========================================================================
+struct PagedAppendArgs {
+  const char* src[2];
+  char* dst[2];
+  const int* table;
+  const int* pos;
+  const int* ids;              // null: token t belongs to sequence t
+  int64_t s_t[2], s_h[2];      // source strides in elements
+  int64_t d_p[2], d_h[2], d_t[2];
+  int64_t table_sb;
+  int64_t P, total;            // total: threads of one of the two tensors
+  int B, HKV, D, chunks, page_shift, M;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256)
+void paged_append_kernel(const PagedAppendArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.total) return;
+  const int which = blockIdx.y;
+  const int64_t row = i / a.chunks;
+  const int c = (int)(i - row * a.chunks);
+  const int64_t t = row / a.HKV;
+  const int h = (int)(row - t * a.HKV);
+  const int seq = a.ids ? a.ids[t] : (int)t;
+  const int pos = a.pos[t];
+  // tokens without a place (negative position, past the table, a page number
+  // outside the pool) are not written
+  if (seq < 0 || seq >= a.B || pos < 0) return;
+  const int pi = pos >> a.page_shift;
+  if (pi >= a.M) return;
+  const int pg = a.table[seq * a.table_sb + pi];
+  if (pg < 0 || pg >= a.P) return;
+  const T* src = reinterpret_cast<const T*>(a.src[which]) + t * a.s_t[which]
+                 + h * a.s_h[which] + 8 * c;
+  T* dst = reinterpret_cast<T*>(a.dst[which]) + pg * a.d_p[which]
+           + h * a.d_h[which]
+           + (pos & ((1 << a.page_shift) - 1)) * a.d_t[which] + 8 * c;
+  T v[8];
+  const int n = a.D - 8 * c;
+  if (n >= 8) {
+    __builtin_memcpy(v, src, sizeof(v));
+  } else {
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? src[j] : (T)0;
+  }
+  __builtin_memcpy(__builtin_assume_aligned(dst, 16), v, sizeof(v));
+}
+
+extern "C" hipError_t lumina_paged_append(
+    const void* k, const void* v, void* kp, void* vp, const int* table,
+    const int* pos, const int* ids, const int64_t* strides, int64_t P,
+    int64_t T, int B, int HKV, int D, int W, int page_shift, int M,
+    int elem_size, hipStream_t stream) {
+  PagedAppendArgs a;
+  a.src[0] = (const char*)k; a.src[1] = (const char*)v;
+  a.dst[0] = (char*)kp; a.dst[1] = (char*)vp;
+  a.table = table; a.pos = pos; a.ids = ids;
+  for (int i = 0; i < 2; ++i) {
+    a.s_t[i] = strides[2 * i]; a.s_h[i] = strides[2 * i + 1];
+    a.d_p[i] = strides[4 + 3 * i]; a.d_h[i] = strides[5 + 3 * i];
+    a.d_t[i] = strides[6 + 3 * i];
+  }
+  a.table_sb = strides[10];
+  a.P = P; a.B = B; a.HKV = HKV; a.D = D; a.chunks = W / 8;
+  a.page_shift = page_shift; a.M = M;
+  a.total = T * HKV * a.chunks;
+  const int64_t blocks = (a.total + 255) / 256;
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  const dim3 grid((uint32_t)blocks, 2), block(256);
+  if (elem_size == 2)
+    paged_append_kernel<uint16_t><<<grid, block, 0, stream>>>(a);
+  else if (elem_size == 4)
+    paged_append_kernel<uint32_t><<<grid, block, 0, stream>>>(a);
+  else
+    return hipErrorInvalidValue;
+  HIP_CHECK_LAST();
+  return hipSuccess;
+}
+
+// ===========================================================================
+// Copying pages: pool[l, dst[i]] = pool[l, src[i]] for every layer l, for up to
+// two pools at once. The page numbers travel in the kernel's arguments, so a
+// call copies nothing to the device and may be captured. A workgroup moves
+// COPY_PIECE bytes of one page.
+// ===========================================================================
+#define COPY_PAIRS 256
+#define COPY_PIECE 16384
+
+struct CopyPagesArgs {
+  char* pool[2];
+  int64_t layer_bytes[2], page_stride[2];   // strides in bytes
+  int64_t page_bytes;
+  int layers, pieces, n;
+  int src[COPY_PAIRS], dst[COPY_PAIRS];
+};
+
+template <typename V>
+__global__ __launch_bounds__(256)
+void copy_pages_kernel(const CopyPagesArgs a) {
+  const int which = blockIdx.z;
+  const int pair = blockIdx.y;
+  const int layer = blockIdx.x / a.pieces;
+  const int piece = blockIdx.x - layer * a.pieces;
+  char* base = a.pool[which] + layer * a.layer_bytes[which];
+  const char* src = base + a.src[pair] * a.page_stride[which];
+  char* dst = base + a.dst[pair] * a.page_stride[which];
+  const int64_t at = (int64_t)piece * COPY_PIECE;
+  const int64_t left = a.page_bytes - at;
+  const int bytes = left < COPY_PIECE ? (int)left : COPY_PIECE;
+  const V* s = reinterpret_cast<const V*>(src + at);
+  V* d = reinterpret_cast<V*>(dst + at);
+  const int nv = bytes / (int)sizeof(V);
+  constexpr int U = 4;
+  for (int i = threadIdx.x; i < nv; i += 256 * U) {
+    V v[U];
+    #pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + 256 * u < nv) v[u] = __builtin_nontemporal_load(s + i + 256 * u);
+    #pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + 256 * u < nv) __builtin_nontemporal_store(v[u], d + i + 256 * u);
+  }
+}
+
+// src and dst are host arrays of n page numbers that the caller has checked.
+extern "C" hipError_t lumina_copy_pages(
+    void* const* pools, int n_pools, const int64_t* layer_bytes,
+    const int64_t* page_stride, int layers, int64_t page_bytes,
+    const int* src, const int* dst, int64_t n, hipStream_t stream) {
+  CopyPagesArgs a;
+  if (n_pools < 1 || n_pools > 2) return hipErrorInvalidValue;
+  a.page_bytes = page_bytes;
+  a.layers = layers;
+  const int64_t pieces = (page_bytes + COPY_PIECE - 1) / COPY_PIECE;
+  if (pieces * layers > 0x7fffffff) return hipErrorInvalidValue;
+  a.pieces = (int)pieces;
+  bool wide = page_bytes % 16 == 0;
+  for (int i = 0; i < n_pools; ++i) {
+    a.pool[i] = (char*)pools[i];
+    a.layer_bytes[i] = layer_bytes[i];
+    a.page_stride[i] = page_stride[i];
+    wide = wide && (uintptr_t)pools[i] % 16 == 0 && layer_bytes[i] % 16 == 0
+           && page_stride[i] % 16 == 0;
+  }
+  for (int64_t at = 0; at < n; at += COPY_PAIRS) {
+    a.n = (int)(n - at < COPY_PAIRS ? n - at : COPY_PAIRS);
+    for (int i = 0; i < a.n; ++i) {
+      a.src[i] = src[at + i];
+      a.dst[i] = dst[at + i];
+    }
+    const dim3 grid((uint32_t)(pieces * layers), a.n, n_pools), block(256);
+    if (wide)
+      copy_pages_kernel<uintx4><<<grid, block, 0, stream>>>(a);
+    else
+      copy_pages_kernel<uint8_t><<<grid, block, 0, stream>>>(a);
+    HIP_CHECK_LAST();
+  }
+  return hipSuccess;
+}

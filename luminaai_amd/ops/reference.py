@@ -195,3 +195,182 @@ def load_balancing_loss(probs: torch.Tensor, topi: torch.Tensor, num_experts: in
         frac = counts / max(1, topi.numel())
     importance = probs.mean(0)
     return (frac * importance).sum() * num_experts
+
+
+# ---------------------------------------------------------- paged KV cache
+def _check_pages(k_pages, v_pages, heads, dim, like):
+    """Refusals shared with the GPU binding (csrc/bindings.cpp check_pages)."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must be [pages, kv_heads, page, "
+                         "width], of one shape")
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if t.device != like.device:
+            raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+        if t.dtype != like.dtype:
+            raise TypeError(f"{name} is {t.dtype}, not {like.dtype}")
+    _, hkv, page, width = k_pages.shape
+    if heads is not None and hkv != heads:
+        raise ValueError(f"k_pages has {hkv} heads, not {heads}")
+    if not 16 <= page <= 4096 or page & (page - 1):
+        raise ValueError("page size must be a power of two from 16 to 4096, "
+                         f"got {page}")
+    if width != (dim + 7) // 8 * 8:
+        raise ValueError("k_pages must be head_dim rounded up to a multiple of "
+                         f"8 wide (head_dim {dim}, got {width})")
+
+
+def _check_int32(t, like, dims, name):
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if t.dim() != dims or (t.numel() and t.stride(-1) != 1):
+        raise ValueError(f"{name} must be a {dims}-dimensional tensor with "
+                         "contiguous rows")
+
+
+def paged_attention(q, k_pages, v_pages, block_table, seq_lens, scale):
+    """Sequence by sequence over gathered pages, fp32 (fp64 for fp64 input)."""
+    if q.dim() != 3:
+        raise ValueError("q must be [batch, heads, head_dim]")
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise RuntimeError("paged_attention has no gradient: call it under "
+                           "torch.no_grad()")
+    B, H, D = q.shape
+    if not 1 <= D <= 192:
+        raise ValueError(f"head_dim must be 1 to 192, got {D}")
+    _check_pages(k_pages, v_pages, None, D, q)
+    P, HKV, page, _ = k_pages.shape
+    if HKV == 0 or H == 0 or H % HKV:
+        raise ValueError(f"heads ({H}) must be a multiple of kv_heads ({HKV})")
+    _check_int32(block_table, q, 2, "block_table")
+    _check_int32(seq_lens, q, 1, "seq_lens")
+    if block_table.shape[0] != B or seq_lens.shape[0] != B:
+        raise ValueError("block_table and seq_lens need a row for each of the "
+                         f"{B} sequences")
+    wide = torch.promote_types(q.dtype, torch.float32)
+    out = torch.zeros(B, H, D, dtype=q.dtype, device=q.device)
+    cap = block_table.shape[1] * page
+    for b, n in enumerate(seq_lens.tolist()):
+        n = min(max(n, 0), cap)
+        pages = block_table[b, :(n + page - 1) // page].long()
+        live = ((pages >= 0) & (pages < P)).repeat_interleave(page)[:n]
+        if not bool(live.any()):
+            continue
+        pages = torch.where((pages >= 0) & (pages < P), pages, 0)
+        kv = [t[pages].transpose(0, 1).reshape(HKV, -1, t.shape[-1])
+              [:, :n, :D][:, live].to(wide) for t in (k_pages, v_pages)]
+        qg = q[b].to(wide).view(HKV, H // HKV, D)
+        s = torch.matmul(qg, kv[0].transpose(1, 2).contiguous()) * scale
+        out[b] = torch.matmul(s.softmax(-1), kv[1]).view(H, D).to(q.dtype)
+    return out
+
+
+def paged_kv_append(k, v, k_pages, v_pages, block_table, positions, seq_ids):
+    if k.dim() != 3 or v.shape != k.shape:
+        raise ValueError("k and v must be [tokens, kv_heads, head_dim]")
+    if v.dtype != k.dtype:
+        raise TypeError(f"v is {v.dtype}, not {k.dtype}")
+    T, HKV, D = k.shape
+    if not HKV or not D:
+        raise ValueError("k has no heads or no channels")
+    _check_pages(k_pages, v_pages, HKV, D, k)
+    _check_int32(block_table, k, 2, "block_table")
+    _check_int32(positions, k, 1, "positions")
+    if positions.shape[0] != T:
+        raise ValueError(f"positions has {positions.shape[0]} entries for {T} "
+                         "tokens")
+    if seq_ids is not None:
+        _check_int32(seq_ids, k, 1, "seq_ids")
+        if seq_ids.shape[0] != T:
+            raise ValueError(f"seq_ids has {seq_ids.shape[0]} entries for {T} "
+                             "tokens")
+    elif block_table.shape[0] != T:
+        raise ValueError("without seq_ids there is one token for each "
+                         f"sequence: {T} tokens, {block_table.shape[0]} "
+                         "sequences")
+    B, M = block_table.shape
+    if not T or not B or not M:
+        return
+    page, width = k_pages.shape[2:]
+    seq = torch.arange(T, device=k.device) if seq_ids is None \
+        else seq_ids.long()
+    pos = positions.long()
+    slot = torch.div(pos, page, rounding_mode="floor")
+    ok = (seq >= 0) & (seq < B) & (pos >= 0) & (slot < M)
+    pages = block_table.long()[seq.clamp(0, B - 1), slot.clamp(0, M - 1)]
+    ok &= (pages >= 0) & (pages < k_pages.shape[0])
+    pad = width - D
+    for new, pool in ((k, k_pages), (v, v_pages)):
+        pool[pages[ok], :, pos[ok] % page] = F.pad(new[ok], (0, pad))
+
+
+def copy_pages(pools, src, dst):
+    if len(src) != len(dst):
+        raise ValueError(f"src names {len(src)} pages, dst {len(dst)}")
+    if not len(pools):
+        raise ValueError("no pool was given")
+    written = set(dst)
+    if len(written) < len(dst):
+        raise ValueError("a page is written twice")
+    if written & set(src):
+        raise ValueError("a page is both read and written")
+    for t in pools:
+        if t.dim() < 3:
+            raise ValueError("a pool must be [layers, pages, ...]")
+        if t.device != pools[0].device:
+            raise ValueError(f"pool is on {t.device}, not on "
+                             f"{pools[0].device}")
+        if not t.numel():
+            raise ValueError("a pool is empty")
+        if not t[0, 0].is_contiguous():
+            raise ValueError("a pool's pages must be contiguous")
+        if any(not 0 <= p < t.shape[1] for p in (*src, *dst)):
+            raise ValueError(f"page numbers must be in 0 to {t.shape[1] - 1}")
+    if not len(src):
+        return
+    s = torch.tensor(src, device=pools[0].device)
+    d = torch.tensor(dst, device=pools[0].device)
+    for t in pools:
+        t[:, d] = t[:, s]
+
+
+# ---------------------------------------------------- token log probabilities
+def token_logprobs(logits, tokens, top_k, ignore_index):
+    """Autograd runs through these operations; see ops/logprobs.py for the
+    meaning of each result."""
+    V = logits.shape[-1]
+    if V == 0:
+        raise ValueError("logits must be [rows, vocab] with contiguous rows")
+    if not logits.is_floating_point():
+        raise TypeError(f"logits must be bf16, fp16 or fp32, got "
+                        f"{logits.dtype}")
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"tokens must be int64 or int32, got {tokens.dtype}")
+    if tokens.device != logits.device:
+        raise ValueError(f"tokens is on {tokens.device}, not on "
+                         f"{logits.device}")
+    if not 0 <= top_k <= min(64, V):
+        raise ValueError("top_k must be 0 to 64 and at most the vocabulary's "
+                         f"{V}, got {top_k}")
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    logp = F.log_softmax(x, dim=-1)
+    # exp(-inf) * -inf is 0 here, in the value and in the gradient
+    ent = -(logp.exp() * logp.masked_fill(logp == float("-inf"), 0)).sum(-1)
+    tok = tokens.long()
+    inside = (tok >= 0) & (tok < V)
+    lp = logp.gather(1, torch.where(inside, tok, 0)[:, None])[:, 0]
+    lp = torch.where(tok == ignore_index, torch.zeros_like(lp), lp)
+    bad = ~inside & (tok != ignore_index)
+    lp = lp * torch.ones_like(lp).masked_fill(bad, float("nan"))
+    with torch.no_grad():
+        key = x.masked_fill(x.isnan(), float("inf"))
+        # NaN above +inf, then falling values, ties to the lowest index
+        ids = torch.sort(key, dim=-1, descending=True, stable=True).indices
+        if bool(x.isnan().any()):
+            order = torch.sort(x.isnan().gather(1, ids).int(), dim=-1,
+                               descending=True, stable=True).indices
+            ids = ids.gather(1, order)
+        ids = ids[:, :top_k].contiguous()
+        top = logp.gather(1, ids)
+    return lp, ent, top, ids
