@@ -15,6 +15,7 @@ from .interface import (
     swiglu, swiglu_fused,
 )
 from .logprobs import TokenLogprobs, token_logprobs
+from .packed import flash_attention_packed, packed_positions
 from .paged import (
     copy_pages,
     page_width,
@@ -25,8 +26,9 @@ from .reference import rope_cache
 
 __all__ = [
     "TokenLogprobs", "adamw_step", "can_flash_attention", "copy_pages",
-    "flash_attention", "fused_cross_entropy", "get_ext", "has_ext",
-    "l2norm_sq", "page_width", "paged_attention", "paged_kv_append",
+    "flash_attention", "flash_attention_packed", "fused_cross_entropy",
+    "get_ext", "has_ext", "l2norm_sq", "packed_positions", "page_width",
+    "paged_attention", "paged_kv_append",
     "reference", "rmsnorm", "rope", "rope_cache", "swiglu", "swiglu_fused",
     "token_logprobs",
 ]

@@ -75,6 +75,8 @@ hipError_t lumina_moe_dispatch_bwd(const void*, const int64_t*, void*, int64_t, 
 hipError_t lumina_moe_combine_fwd(const void*, const float*, const int64_t*, void*, int64_t, int, int, int64_t, int, hipStream_t);
 hipError_t lumina_moe_combine_bwd_y(const void*, const float*, const int64_t*, const int64_t*, const bool*, void*, int64_t, int64_t, int, int, hipStream_t);
 hipError_t lumina_moe_combine_bwd_w(const void*, const void*, const int64_t*, float*, int64_t, int, int, int64_t, int, hipStream_t);
+hipError_t lumina_packed_attn_fwd(const void*, const void*, const void*, void*, float*, const int*, const int64_t*, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_packed_attn_bwd(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, const int*, const int64_t*, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_paged_attn(const void*, const void*, const void*, void*, const int*, const int*, float*, float*, const int64_t*, int64_t, int, int, int, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_paged_append(const void*, const void*, void*, void*, const int*, const int*, const int*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int, int, hipStream_t);
 hipError_t lumina_copy_pages(void* const*, int, const int64_t*, const int64_t*, int, int64_t, const int*, const int*, int64_t, hipStream_t);
@@ -1002,6 +1004,91 @@ at::Tensor logprob_bwd(const at::Tensor& x, const at::Tensor& tok,
   return dx;
 }
 
+// ---- packed attention ------------------------------------------------------
+namespace {
+// channels beside each other; heads and tokens may lie anywhere
+at::Tensor dense_channels(const at::Tensor& t) {
+  return t.stride(2) == 1 || t.size(2) == 1 ? t : t.contiguous();
+}
+}  // namespace
+
+// -> (o, lse2); lse2 is empty where want_lse is false
+std::tuple<at::Tensor, at::Tensor> packed_attn_fwd(
+    const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
+    const at::Tensor& cu, double scale, bool want_lse) {
+  TORCH_CHECK_VALUE(q_.dim() == 3 && k_.dim() == 3 && v_.sizes() == k_.sizes(),
+                    "q must be [tokens, heads, head_dim], k and v [tokens, "
+                    "kv_heads, head_dim]");
+  TORCH_CHECK_TYPE(is_bf16(q_), "flash_attention_packed on the GPU takes bf16, "
+                   "got ", q_.scalar_type());
+  for (const auto& t : {k_, v_}) {
+    check_same_device(t, q_, "k or v");
+    TORCH_CHECK_TYPE(t.scalar_type() == q_.scalar_type(), "k or v is ",
+                     t.scalar_type(), ", not ", q_.scalar_type());
+  }
+  const int64_t T = q_.size(0), H = q_.size(1), D = q_.size(2);
+  const int64_t HKV = k_.size(1);
+  TORCH_CHECK_VALUE(k_.size(0) == T && k_.size(2) == D,
+                    "q, k and v need the same tokens and head_dim");
+  TORCH_CHECK_VALUE(D >= 1 && D <= 192, "head_dim must be 1 to 192, got ", D);
+  TORCH_CHECK_VALUE(HKV > 0 && H > 0 && H % HKV == 0, "heads (", H,
+                    ") must be a multiple of kv_heads (", HKV, ")");
+  TORCH_CHECK_VALUE(T <= (1 << 30), "at most 2^30 tokens, got ", T);
+  check_int32(cu, q_, 1, "cu_seqlens");
+  TORCH_CHECK_VALUE(cu.size(0) >= 1 && cu.size(0) <= (1 << 24),
+                    "cu_seqlens needs one entry more than there are sequences");
+  TORCH_CHECK_VALUE(scale > 0 && scale < INFINITY, "scale must be positive, got ",
+                    scale);
+  const c10::DeviceGuard guard(q_.device());
+  const auto q = dense_channels(q_), k = dense_channels(k_),
+             v = dense_channels(v_);
+  auto o = at::empty({T, H, D}, q.options());
+  auto lse = at::empty({want_lse ? H : 0, T}, q.options().dtype(at::kFloat));
+  if (T == 0) return {o, lse};
+  const int64_t strides[8] = {q.stride(0), q.stride(1), k.stride(0),
+                              k.stride(1), v.stride(0), v.stride(1), 0, 0};
+  check_hip(lumina_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                   o.data_ptr(),
+                                   want_lse ? lse.data_ptr<float>() : nullptr,
+                                   cu.data_ptr<int>(), strides, (int)T,
+                                   (int)cu.size(0) - 1, (int)H, (int)HKV,
+                                   (int)D, (float)scale, cur_stream()),
+            "flash_attention_packed");
+  return {o, lse};
+}
+
+// Takes what packed_attn_fwd took and gave.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
+    const at::Tensor& go_, const at::Tensor& q_, const at::Tensor& k_,
+    const at::Tensor& v_, const at::Tensor& o, const at::Tensor& lse,
+    const at::Tensor& cu, double scale) {
+  TORCH_CHECK_VALUE(go_.sizes() == q_.sizes() && go_.device() == q_.device(),
+                    "the gradient must be of q's shape and device");
+  TORCH_CHECK_TYPE(is_bf16(go_), "the gradient must be bf16");
+  const c10::DeviceGuard guard(q_.device());
+  const auto q = dense_channels(q_), k = dense_channels(k_),
+             v = dense_channels(v_), go = dense_channels(go_);
+  const int64_t T = q.size(0), H = q.size(1), D = q.size(2), HKV = k.size(1);
+  auto dq = at::empty({T, H, D}, q.options());
+  auto dk = at::empty({T, HKV, D}, q.options());
+  auto dv = at::empty({T, HKV, D}, q.options());
+  if (T == 0) return {dq, dk, dv};
+  auto delta = at::empty({H, T}, lse.options());
+  const int64_t strides[8] = {q.stride(0), q.stride(1), k.stride(0),
+                              k.stride(1), v.stride(0), v.stride(1),
+                              go.stride(0), go.stride(1)};
+  check_hip(lumina_packed_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                   o.data_ptr(), go.data_ptr(),
+                                   lse.data_ptr<float>(),
+                                   delta.data_ptr<float>(), dq.data_ptr(),
+                                   dk.data_ptr(), dv.data_ptr(),
+                                   cu.data_ptr<int>(), strides, (int)T,
+                                   (int)cu.size(0) - 1, (int)H, (int)HKV,
+                                   (int)D, (float)scale, cur_stream()),
+            "flash_attention_packed gradient");
+  return {dq, dk, dv};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("attn_fwd", &attn_fwd,
           "causal GQA flash attention forward -> (O, LSE2) (gfx950)");
@@ -1057,6 +1144,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("ce_bwd", &ce_bwd, "fused CE backward (gfx950)");
   mod.def("l2norm_sq", &l2norm_sq, "flat L2 norm squared (gfx950)");
   mod.def("adamw_step", &adamw_step, "fused clip+AdamW on flat buffers (gfx950)");
+  mod.def("packed_attn_fwd", &packed_attn_fwd, "packed causal attention");
+  mod.def("packed_attn_bwd", &packed_attn_bwd, "gradient of packed_attn_fwd");
   mod.def("paged_attn", &paged_attn, "single-token attention over pages");
   mod.def("paged_append", &paged_append, "append keys and values to pages");
   mod.def("copy_pages", &copy_pages, "copy pages within pools");

@@ -1,0 +1,702 @@
+// Causal GQA attention over packed sequences, forward and backward, for CDNA4
+// (gfx950).
+//
+// q [T, H, D], k and v [T, HKV, D] bf16 in any strides with contiguous
+// channels; sequence b is the tokens cu[b] .. cu[b+1]. D <= 192 is padded to a
+// multiple of 32 (DP) while a tile is staged, not in memory.
+//
+//   forward   S = scale Q K^T, P = softmax(S), O = P V, lse2 = log2 sum 2^S2
+//   backward  dP = dO V^T, delta = rowsum(dO O), dS = P (dP - delta)
+//             dV = P^T dO, dK = scale dS^T Q, dQ = scale dS K
+//
+// Bound by the matrix pipe, and beside it by the exponentials and the LDS reads
+// of the operands. What carries all three kernels:
+// - mfma 32x32x16 bf16 (C: column = lane & 31, row = 8 (r >> 2) + 4 (lane >> 5)
+//   + (r & 3) for register r). The softmax index runs along the lanes' columns
+//   where it can (forward, dQ), so maximum, sum and rescaling are lane-local.
+// - A product that contracts over C's rows takes them in the order they lie in:
+//   registers 8s .. 8s+7 are already the B fragment of step s, if the other
+//   operand supplies rows 16s + 4 hi + {0..3} and 16s + 8 + 4 hi + {0..3}. Two
+//   transposing LDS reads (ds_read_b64_tr_b16) at those rows do; P and dS never
+//   cross lanes.
+// - One LDS image per tile serves both row reads (16 bytes of a row) and
+//   transposing reads (4 rows x 64 bytes per half wave): row stride = 16 or 48
+//   mod 64 dwords and the 16-byte piece index xor (row >> 2) & 3, which keeps
+//   both free of bank conflicts.
+// - Tiles go global -> registers -> LDS, loaded one step ahead; two LDS buffers,
+//   one barrier a step.
+#include "common.h"
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(2))) float floatx2;
+typedef __attribute__((ext_vector_type(2))) uint32_t uintx2;
+typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
+
+#define LOG2E 1.4426950408889634f
+
+struct PackedArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  const uint16_t* o;           // backward: forward's result [T, H, D]
+  const uint16_t* go;          // backward: its gradient
+  uint16_t* out;               // forward: [T, H, D]
+  uint16_t* dq;                // [T, H, D]
+  uint16_t* dk;                // [T, HKV, D]
+  uint16_t* dv;
+  float* lse;                  // [H, T], log2 units; +inf where nothing summed
+  float* delta;                // [H, T]
+  const int* cu;               // [B + 1]
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, go_st, go_sh;
+  int T, B, H, HKV, D;
+  float scale;
+};
+
+// ---- which rows a workgroup takes ------------------------------------------
+struct Work {
+  int start;                   // the sequence's first token
+  int len;                     // its length; 0: nothing to do
+  int block;                   // block of rows inside it, the last ones first
+  int tail;                    // >= 0: rows behind the last sequence start here
+};
+
+// Block `id` of all sequences' blocks of `rows` rows, then the blocks of the
+// rows behind the last sequence. cu[0] counts as 0 and the rest is cut to [0, T],
+// so that no content of it leads outside the tensors. Every wave scans it: 64
+// sequences a step, from L2.
+DEV_INLINE Work find_work(const int* cu, int B, int T, int id, int rows) {
+  const int lane = threadIdx.x & 63;
+  Work w = {0, 0, 0, -1};
+  int before = 0;
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    const int b = b0 + lane;
+    int s = 0, n = 0;
+    if (b < B) {
+      s = b ? cu[b] : 0;
+      s = s < 0 ? 0 : (s > T ? T : s);
+      int e = cu[b + 1];
+      e = e > T ? T : e;
+      n = e > s ? e - s : 0;
+    }
+    const int nb = (n + rows - 1) / rows;
+    int sum = nb;                         // inclusive prefix sum
+    #pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += x;
+    }
+    const int at = id - before - (sum - nb);
+    const unsigned long long hit = __ballot(at >= 0 && at < nb);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      w.start = __builtin_amdgcn_readlane(s, src);
+      w.len = __builtin_amdgcn_readlane(n, src);
+      w.block = __builtin_amdgcn_readlane(nb - 1 - at, src);
+      return w;
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+  }
+  int end = B > 0 ? cu[B] : 0;
+  end = end < 0 ? 0 : (end > T ? T : end);
+  const int64_t tail = end + (int64_t)(id - before) * rows;
+  w.tail = tail < T ? (int)tail : T;
+  return w;
+}
+
+// Heads that share keys and values are given to one XCD (workgroups go round
+// the eight of them), so that its L2 holds them once.
+DEV_INLINE int head_of(int local, int heads) {
+  return heads & 7 ? local : (local & 7) * (heads >> 3) + (local >> 3);
+}
+
+// ---- staging ---------------------------------------------------------------
+template <int DP> struct Img {
+  // dwords of a row: 16 or 48 mod 64
+  static constexpr int ROW = (DP / 2) % 64 == 16 || (DP / 2) % 64 == 48
+                                 ? DP / 2 : DP / 2 + 16;
+  static constexpr int BYTES = ROW * 4;
+  static_assert(ROW % 64 == 16 || ROW % 64 == 48, "bank layout");
+  static DEV_INLINE int at(int row, int piece) {     // 16-byte pieces
+    return row * BYTES + ((piece ^ ((row >> 2) & 3)) << 4);
+  }
+};
+
+// 8 channels from 8 c on of a row of D: zero past D. Rows may start at any
+// element. A row's last, partial piece is read as the last 8 channels and
+// moved down.
+DEV_INLINE uintx4 load_piece(const uint16_t* row, int c, int D) {
+  uintx4 v = {0, 0, 0, 0};
+  const int off = 8 * c;
+  if (D >= 8) {
+    if (off < D) {
+      const int o = off < D - 8 ? off : D - 8;
+      __builtin_memcpy(&v, row + o, 16);
+      const int e = (8 - (D & 7)) & 7;
+      if (e) {                                       // uniform
+        uint32_t t[8] = {v[0], v[1], v[2], v[3], 0, 0, 0, 0};
+        if (e & 1) {
+          #pragma unroll
+          for (int i = 0; i < 4; ++i)
+            t[i] = __builtin_amdgcn_alignbit(t[i + 1], t[i], 16);
+        }
+        if (e & 2) {
+          #pragma unroll
+          for (int i = 0; i < 4; ++i) t[i] = t[i + 1];
+        }
+        if (e & 4) {
+          #pragma unroll
+          for (int i = 0; i < 4; ++i) t[i] = t[i + 2];
+        }
+        if (off != o) v = uintx4{t[0], t[1], t[2], t[3]};
+      }
+    }
+  } else {
+    #pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (off + j < D) v[j >> 1] |= (uint32_t)row[off + j] << (16 * (j & 1));
+  }
+  return v;
+}
+
+// A tile of ROWS rows in registers, NT threads.
+template <int DP, int ROWS, int NT>
+struct Stage {
+  static constexpr int PIECES = ROWS * DP / 8;
+  static constexpr int N = (PIECES + NT - 1) / NT;
+  uintx4 v[N];
+  // rows past `last` repeat it: nothing outside the sequence is read
+  DEV_INLINE void load(const uint16_t* base, int64_t st, int row0, int last,
+                       int D) {
+    #pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = threadIdx.x + i * NT;
+      if (PIECES % NT == 0 || p < PIECES) {
+        const int row = p / (DP / 8), c = p - row * (DP / 8);
+        const int r = row0 + row < last ? row0 + row : last;
+        v[i] = load_piece(base + r * st, c, D);
+      }
+    }
+  }
+  DEV_INLINE void store(char* img) const {
+    #pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = threadIdx.x + i * NT;
+      if (PIECES % NT == 0 || p < PIECES) {
+        const int row = p / (DP / 8), c = p - row * (DP / 8);
+        *reinterpret_cast<uintx4*>(img + Img<DP>::at(row, c)) = v[i];
+      }
+    }
+  }
+};
+
+// A or B fragment of step ks: row lane & 31 (+ row0), channels 16 ks + 8 hi ..
+template <int DP>
+DEV_INLINE bf16x8 row_frag(const char* img, int row0, int lane, int ks) {
+  return *reinterpret_cast<const bf16x8*>(
+      img + Img<DP>::at(row0 + (lane & 31), 2 * ks + (lane >> 5)));
+}
+
+// A fragment of the transposed tile: channel 32 dt + (lane & 31), rows
+// r0 + 4 hi + {0..3} and r0 + 8 + 4 hi + {0..3}. ds_read_b64_tr_b16 hands lane
+// l of 16 the l-th channel of the four rows whose 8-byte pieces the lanes
+// address: lane l points at row l >> 2, channels 4 (l & 3) ..
+template <int DP>
+DEV_INLINE bf16x8 col_frag(const char* img, int r0, int lane, int dt) {
+  const int l = lane & 15;
+  const int row = r0 + 4 * (lane >> 5) + (l >> 2);
+  const int ch = 32 * dt + (lane & 16) + 4 * (l & 3);
+  const int sub = (ch & 4) * 2;
+  union { bf16x4 h[2]; bf16x8 v; } u;
+  u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+      (lds_bf16x4*)(img + Img<DP>::at(row, ch >> 3) + sub));
+  u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+      (lds_bf16x4*)(img + Img<DP>::at(row + 8, ch >> 3) + sub));
+  return u.v;
+}
+
+DEV_INLINE uint32_t pack2(float lo, float hi) {
+  floatx2 f = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
+}
+
+// C's registers 8 s .. 8 s + 7 as the B fragment of step s
+DEV_INLINE bf16x8 pack_frag(const float* p) {
+  const uintx4 u = {pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]),
+                    pack2(p[6], p[7])};
+  return __builtin_bit_cast(bf16x8, u);
+}
+
+DEV_INLINE f32x16 zero16() {
+  f32x16 z;
+  #pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+DEV_INLINE f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// A column of a transposed result: this lane's row of memory takes channels
+// 8 g + 4 hi + {0..3}, g = 0 .. 4 DT - 1.
+template <int DT>
+DEV_INLINE void store_col(uint16_t* row, const f32x16* acc, float f, int hi,
+                          int D) {
+  #pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+    #pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * dt + 8 * g + 4 * hi;
+      const uintx2 u = {pack2(acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f),
+                        pack2(acc[dt][4 * g + 2] * f, acc[dt][4 * g + 3] * f)};
+      if (d + 4 <= D) {
+        __builtin_memcpy(row + d, &u, 8);
+      } else {
+        #pragma unroll
+        for (int j = 0; j < 3; ++j)
+          if (d + j < D) row[d + j] = (uint16_t)(u[j >> 1] >> (16 * (j & 1)));
+      }
+    }
+}
+
+// Rows behind the last sequence belong to nothing: zero.
+DEV_INLINE void zero_rows(uint16_t* out, int heads, int head, int D, int from,
+                          int T, int rows) {
+  const int n = T - from < rows ? T - from : rows;
+  for (int i = threadIdx.x; i < n * D; i += blockDim.x) {
+    const int r = i / D;
+    out[((int64_t)(from + r) * heads + head) * D + i - r * D] = 0;
+  }
+}
+
+// ===========================================================================
+// Forward: a workgroup takes FQ rows of one head, a wave 32 of them.
+// ===========================================================================
+#define FW 8                   // waves
+#define FQ (32 * FW)           // query rows of a workgroup
+#define FK 64                  // keys of a step
+
+template <int DP>
+__global__ __launch_bounds__(64 * FW, 2)
+void packed_fwd_kernel(const PackedArgs a) {
+  constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * FW;
+  constexpr int IMG = FK * Img<DP>::BYTES;
+  __shared__ char lds[4 * IMG];              // [2][K image, V image]
+  const int h = head_of(blockIdx.x % a.H, a.H);
+  const Work w = find_work(a.cu, a.B, a.T, blockIdx.x / a.H, FQ);
+  if (w.tail >= 0) {
+    zero_rows(a.out, a.H, h, a.D, w.tail, a.T, FQ);
+    return;
+  }
+  const int lane = threadIdx.x & 63, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hk = h / (a.H / a.HKV);
+  const int q0 = w.block * FQ, qw = q0 + 32 * wave;
+  const int last = w.len - 1;
+  const uint16_t* kb = a.k + w.start * a.k_st + hk * a.k_sh;
+  const uint16_t* vb = a.v + w.start * a.v_st + hk * a.v_sh;
+  const int qi = qw + (lane & 31);           // this lane's query
+
+  bf16x8 qf[KS];
+  {
+    const uint16_t* qr = a.q + (int64_t)(w.start + (qi < last ? qi : last))
+                         * a.q_st + h * a.q_sh;
+    #pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qf[ks] = __builtin_bit_cast(bf16x8, load_piece(qr, 2 * ks + hi, a.D));
+  }
+  f32x16 o[DT];
+  #pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = zero16();
+  float m = -1e30f, l = 0.f;
+  const float c2 = a.scale * LOG2E;
+
+  // keys up to the last query of the workgroup, or of the sequence
+  const int kend = q0 + FQ < w.len ? q0 + FQ : w.len;
+  const int steps = (kend + FK - 1) / FK;
+  Stage<DP, FK, NT> sk, sv;
+  sk.load(kb, a.k_st, 0, last, a.D);
+  sv.load(vb, a.v_st, 0, last, a.D);
+  sk.store(lds);
+  sv.store(lds + IMG);
+  __syncthreads();
+  for (int t = 0; t < steps; ++t) {
+    const char* ki = lds + (t & 1) * 2 * IMG;
+    const char* vi = ki + IMG;
+    const bool more = t + 1 < steps;
+    if (more) {
+      sk.load(kb, a.k_st, (t + 1) * FK, last, a.D);
+      sv.load(vb, a.v_st, (t + 1) * FK, last, a.D);
+    }
+    const int k0 = t * FK;
+    if (k0 <= qw + 31) {                     // else all masked for this wave
+      float p[FK / 32][16];
+      #pragma unroll
+      for (int kk = 0; kk < FK / 32; ++kk) {
+        f32x16 s = zero16();
+        #pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          s = mfma(row_frag<DP>(ki, 32 * kk, lane, ks), qf[ks], s);
+        #pragma unroll
+        for (int r = 0; r < 16; ++r) p[kk][r] = s[r];
+      }
+      if (k0 + FK - 1 > qw) {                // touches the diagonal
+        #pragma unroll
+        for (int kk = 0; kk < FK / 32; ++kk)
+          #pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int kt = k0 + 32 * kk + 8 * (r >> 2) + 4 * hi + (r & 3);
+            if (kt > qi) p[kk][r] = -INFINITY;
+          }
+      }
+      float pm = p[0][0];
+      #pragma unroll
+      for (int kk = 0; kk < FK / 32; ++kk)
+        #pragma unroll
+        for (int r = 0; r < 16; ++r) pm = fmaxf(pm, p[kk][r]);
+      pm *= c2;                              // c2 > 0
+      // the maximum follows only when it grew by more than 2^8: sums and
+      // products of up to 2^8 lose nothing
+      if (__any(pm > m + 8.f)) {
+        pm = fmaxf(pm, __shfl_xor(pm, 32, 64));
+        const float mn = fmaxf(m, pm);
+        const float f = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+        #pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+      }
+      #pragma unroll
+      for (int kk = 0; kk < FK / 32; ++kk) {
+        #pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          p[kk][r] = __builtin_amdgcn_exp2f(
+              __builtin_fmaf(p[kk][r], c2, -m));
+          l += p[kk][r];
+        }
+        #pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const bf16x8 pf = pack_frag(&p[kk][8 * s]);
+          #pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+            o[dt] = mfma(col_frag<DP>(vi, 32 * kk + 16 * s, lane, dt), pf,
+                         o[dt]);
+        }
+      }
+    }
+    if (more) {
+      char* next = lds + ((t + 1) & 1) * 2 * IMG;
+      sk.store(next);
+      sv.store(next + IMG);
+    }
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (qi < w.len) {
+    const int64_t tok = w.start + qi;
+    store_col<DT>(a.out + (tok * a.H + h) * a.D, o, l == 0.f ? 0.f : 1.f / l,
+                  hi, a.D);
+    if (a.lse && hi == 0)
+      a.lse[(int64_t)h * a.T + tok] =
+          l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+  }
+}
+
+// ===========================================================================
+// dQ, and delta for the next kernel: the forward's arrangement, with P from the
+// saved lse2. K's image serves S (rows) and dQ (columns).
+// ===========================================================================
+#define BW 4                   // waves
+#define BQ (32 * BW)
+#define BK 32                  // keys of a step
+
+template <int DP>
+__global__ __launch_bounds__(64 * BW, DP <= 128 ? 2 : 1)
+void packed_dq_kernel(const PackedArgs a) {
+  constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * BW;
+  constexpr int IMG = BK * Img<DP>::BYTES;
+  __shared__ char lds[4 * IMG];
+  const int h = head_of(blockIdx.x % a.H, a.H);
+  const Work w = find_work(a.cu, a.B, a.T, blockIdx.x / a.H, BQ);
+  if (w.tail >= 0) {
+    zero_rows(a.dq, a.H, h, a.D, w.tail, a.T, BQ);
+    return;
+  }
+  const int lane = threadIdx.x & 63, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hk = h / (a.H / a.HKV);
+  const int q0 = w.block * BQ, qw = q0 + 32 * wave;
+  const int last = w.len - 1;
+  const uint16_t* kb = a.k + w.start * a.k_st + hk * a.k_sh;
+  const uint16_t* vb = a.v + w.start * a.v_st + hk * a.v_sh;
+  const int qi = qw + (lane & 31);
+  const int64_t tok = w.start + (qi < last ? qi : last);
+
+  bf16x8 qf[KS], gf[KS];
+  float delta = 0.f;
+  {
+    const uint16_t* qr = a.q + tok * a.q_st + h * a.q_sh;
+    const uint16_t* gr = a.go + tok * a.go_st + h * a.go_sh;
+    const uint16_t* orow = a.o + (tok * a.H + h) * a.D;
+    #pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks] = __builtin_bit_cast(bf16x8, load_piece(qr, 2 * ks + hi, a.D));
+      gf[ks] = __builtin_bit_cast(bf16x8, load_piece(gr, 2 * ks + hi, a.D));
+      const bf16x8 of = __builtin_bit_cast(
+          bf16x8, load_piece(orow, 2 * ks + hi, a.D));
+      #pragma unroll
+      for (int j = 0; j < 8; ++j)
+        delta = __builtin_fmaf((float)gf[ks][j], (float)of[j], delta);
+    }
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  const float lse = a.lse[(int64_t)h * a.T + tok];
+  if (hi == 0 && qi < w.len) a.delta[(int64_t)h * a.T + tok] = delta;
+  f32x16 dq[DT];
+  #pragma unroll
+  for (int dt = 0; dt < DT; ++dt) dq[dt] = zero16();
+  const float c2 = a.scale * LOG2E;
+
+  const int kend = q0 + BQ < w.len ? q0 + BQ : w.len;
+  const int steps = (kend + BK - 1) / BK;
+  Stage<DP, BK, NT> sk, sv;
+  sk.load(kb, a.k_st, 0, last, a.D);
+  sv.load(vb, a.v_st, 0, last, a.D);
+  sk.store(lds);
+  sv.store(lds + IMG);
+  __syncthreads();
+  for (int t = 0; t < steps; ++t) {
+    const char* ki = lds + (t & 1) * 2 * IMG;
+    const char* vi = ki + IMG;
+    const bool more = t + 1 < steps;
+    if (more) {
+      sk.load(kb, a.k_st, (t + 1) * BK, last, a.D);
+      sv.load(vb, a.v_st, (t + 1) * BK, last, a.D);
+    }
+    const int k0 = t * BK;
+    if (k0 <= qw + 31) {
+      f32x16 s = zero16(), dp = zero16();
+      #pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        s = mfma(row_frag<DP>(ki, 0, lane, ks), qf[ks], s);
+        dp = mfma(row_frag<DP>(vi, 0, lane, ks), gf[ks], dp);
+      }
+      float ds[16];
+      #pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lse));
+        const int kt = k0 + 8 * (r >> 2) + 4 * hi + (r & 3);
+        if (kt > qi) p = 0.f;
+        ds[r] = p * (dp[r] - delta);
+      }
+      #pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const bf16x8 f = pack_frag(&ds[8 * st]);
+        #pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          dq[dt] = mfma(col_frag<DP>(ki, 16 * st, lane, dt), f, dq[dt]);
+      }
+    }
+    if (more) {
+      char* next = lds + ((t + 1) & 1) * 2 * IMG;
+      sk.store(next);
+      sv.store(next + IMG);
+    }
+    __syncthreads();
+  }
+  if (qi < w.len)
+    store_col<DT>(a.dq + (tok * a.H + h) * a.D, dq, a.scale, hi, a.D);
+}
+
+// ===========================================================================
+// dK and dV: a workgroup takes BKV keys of one kv head, a wave 32 of them, and
+// goes over the queries of all heads that share it, so the sum over the heads
+// stays in registers and has one order. S has rows = queries (registers),
+// columns = keys (lanes): P and dS are then B fragments of dV^T = dO^T P and
+// dK^T = Q^T dS, and the images of Q and dO serve rows and columns.
+// ===========================================================================
+#define BKV (32 * BW)
+#define BQT 32                 // queries of a step
+
+template <int DP>
+__global__ __launch_bounds__(64 * BW, DP <= 96 ? 2 : 1)
+void packed_dkdv_kernel(const PackedArgs a) {
+  constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * BW;
+  constexpr int IMG = BQT * Img<DP>::BYTES;
+  constexpr int BUF = 2 * IMG + 2 * BQT * 4;   // Q, dO, lse2, delta
+  __shared__ char lds[2 * BUF];
+  const int hk = head_of(blockIdx.x % a.HKV, a.HKV);
+  const Work w = find_work(a.cu, a.B, a.T, blockIdx.x / a.HKV, BKV);
+  if (w.tail >= 0) {
+    zero_rows(a.dk, a.HKV, hk, a.D, w.tail, a.T, BKV);
+    zero_rows(a.dv, a.HKV, hk, a.D, w.tail, a.T, BKV);
+    return;
+  }
+  const int lane = threadIdx.x & 63, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = a.H / a.HKV;
+  // the first keys have the most queries: they go first
+  const int blocks = (w.len + BKV - 1) / BKV;
+  const int kv0 = (blocks - 1 - w.block) * BKV, kw = kv0 + 32 * wave;
+  const int last = w.len - 1;
+  const int ki = kw + (lane & 31);             // this lane's key
+  const int64_t tok = w.start + (ki < last ? ki : last);
+
+  bf16x8 kf[KS], vf[KS];
+  {
+    const uint16_t* kr = a.k + tok * a.k_st + hk * a.k_sh;
+    const uint16_t* vr = a.v + tok * a.v_st + hk * a.v_sh;
+    #pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      kf[ks] = __builtin_bit_cast(bf16x8, load_piece(kr, 2 * ks + hi, a.D));
+      vf[ks] = __builtin_bit_cast(bf16x8, load_piece(vr, 2 * ks + hi, a.D));
+    }
+  }
+  f32x16 dk[DT], dv[DT];
+  #pragma unroll
+  for (int dt = 0; dt < DT; ++dt) { dk[dt] = zero16(); dv[dt] = zero16(); }
+  const float c2 = a.scale * LOG2E;
+
+  const int per = (w.len - kv0 + BQT - 1) / BQT;   // steps of one head
+  const int steps = per * G;
+  Stage<DP, BQT, NT> sq, sg;
+  float slab = 0.f;
+  auto load = [&](int t) {
+    const int g = t / per, qt = kv0 + (t - g * per) * BQT;
+    const int h = hk * G + g;
+    sq.load(a.q + w.start * a.q_st + h * a.q_sh, a.q_st, qt, last, a.D);
+    sg.load(a.go + w.start * a.go_st + h * a.go_sh, a.go_st, qt, last, a.D);
+    if (threadIdx.x < 2 * BQT) {
+      // lse2 = +inf makes P zero for rows past the end
+      const int r = qt + (threadIdx.x & (BQT - 1));
+      const float* src = threadIdx.x < BQT ? a.lse : a.delta;
+      slab = r <= last ? src[(int64_t)h * a.T + w.start + r]
+                       : (threadIdx.x < BQT ? INFINITY : 0.f);
+    }
+  };
+  auto store = [&](char* buf) {
+    sq.store(buf);
+    sg.store(buf + IMG);
+    if (threadIdx.x < 2 * BQT)
+      reinterpret_cast<float*>(buf + 2 * IMG)[threadIdx.x] = slab;
+  };
+  load(0);
+  store(lds);
+  __syncthreads();
+  for (int t = 0; t < steps; ++t) {
+    const char* qi = lds + (t & 1) * BUF;
+    const char* gi = qi + IMG;
+    const float* ls = reinterpret_cast<const float*>(qi + 2 * IMG);
+    const bool more = t + 1 < steps;
+    if (more) load(t + 1);
+    const int qt = kv0 + (t % per) * BQT;
+    if (qt + BQT - 1 >= kw) {                  // else all masked for this wave
+      f32x16 s = zero16(), dp = zero16();
+      #pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        s = mfma(row_frag<DP>(qi, 0, lane, ks), kf[ks], s);
+        dp = mfma(row_frag<DP>(gi, 0, lane, ks), vf[ks], dp);
+      }
+      float p[16], ds[16];
+      #pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const floatx4 le = *reinterpret_cast<const floatx4*>(ls + 8 * g + 4 * hi);
+        const floatx4 de = *reinterpret_cast<const floatx4*>(
+            ls + BQT + 8 * g + 4 * hi);
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * g + j;
+          float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -le[j]));
+          if (ki > qt + 8 * g + 4 * hi + j) x = 0.f;
+          p[r] = x;
+          ds[r] = x * (dp[r] - de[j]);
+        }
+      }
+      #pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const bf16x8 pf = pack_frag(&p[8 * st]), df = pack_frag(&ds[8 * st]);
+        #pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          dv[dt] = mfma(col_frag<DP>(gi, 16 * st, lane, dt), pf, dv[dt]);
+          dk[dt] = mfma(col_frag<DP>(qi, 16 * st, lane, dt), df, dk[dt]);
+        }
+      }
+    }
+    if (more) store(lds + ((t + 1) & 1) * BUF);
+    __syncthreads();
+  }
+  if (ki < w.len) {
+    store_col<DT>(a.dk + (tok * a.HKV + hk) * a.D, dk, a.scale, hi, a.D);
+    store_col<DT>(a.dv + (tok * a.HKV + hk) * a.D, dv, 1.f, hi, a.D);
+  }
+}
+
+// Blocks of `rows` rows that any cu can need: a partial one for each sequence
+// and one for the rows behind them.
+static int64_t max_blocks(const PackedArgs& a, int rows) {
+  return a.T / rows + a.B + 1;
+}
+
+template <int DP>
+static hipError_t run_fwd(const PackedArgs& a, hipStream_t stream) {
+  const int64_t n = max_blocks(a, FQ) * a.H;
+  if (n > 0x7fffffff) return hipErrorInvalidValue;
+  packed_fwd_kernel<DP><<<dim3((uint32_t)n), dim3(64 * FW), 0, stream>>>(a);
+  HIP_CHECK_LAST();
+  return hipSuccess;
+}
+
+template <int DP>
+static hipError_t run_bwd(const PackedArgs& a, hipStream_t stream) {
+  const int64_t n = max_blocks(a, BQ) * a.H;
+  if (n > 0x7fffffff) return hipErrorInvalidValue;
+  packed_dq_kernel<DP><<<dim3((uint32_t)n), dim3(64 * BW), 0, stream>>>(a);
+  HIP_CHECK_LAST();
+  const int64_t m = max_blocks(a, BKV) * a.HKV;
+  packed_dkdv_kernel<DP><<<dim3((uint32_t)m), dim3(64 * BW), 0, stream>>>(a);
+  HIP_CHECK_LAST();
+  return hipSuccess;
+}
+
+static void fill(PackedArgs& a, const int64_t* st, const int* cu, int T, int B,
+                 int H, int HKV, int D, float scale) {
+  a.q_st = st[0]; a.q_sh = st[1]; a.k_st = st[2]; a.k_sh = st[3];
+  a.v_st = st[4]; a.v_sh = st[5]; a.go_st = st[6]; a.go_sh = st[7];
+  a.cu = cu; a.T = T; a.B = B; a.H = H; a.HKV = HKV; a.D = D; a.scale = scale;
+}
+
+#define DISPATCH_DP(D, FN)                                                   \
+  if ((D) <= 64) return FN<64>(a, stream);                                   \
+  if ((D) <= 96) return FN<96>(a, stream);                                   \
+  if ((D) <= 128) return FN<128>(a, stream);                                 \
+  if ((D) <= 160) return FN<160>(a, stream);                                 \
+  if ((D) <= 192) return FN<192>(a, stream);                                 \
+  return hipErrorInvalidValue;
+
+extern "C" hipError_t lumina_packed_attn_fwd(
+    const void* q, const void* k, const void* v, void* out, float* lse,
+    const int* cu, const int64_t* strides, int T, int B, int H, int HKV, int D,
+    float scale, hipStream_t stream) {
+  PackedArgs a = {};
+  a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
+  a.out = (uint16_t*)out; a.lse = lse;
+  fill(a, strides, cu, T, B, H, HKV, D, scale);
+  DISPATCH_DP(D, run_fwd)
+}
+
+extern "C" hipError_t lumina_packed_attn_bwd(
+    const void* q, const void* k, const void* v, const void* o, const void* go,
+    const float* lse, float* delta, void* dq, void* dk, void* dv,
+    const int* cu, const int64_t* strides, int T, int B, int H, int HKV, int D,
+    float scale, hipStream_t stream) {
+  PackedArgs a = {};
+  a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
+  a.o = (const uint16_t*)o; a.go = (const uint16_t*)go;
+  a.lse = const_cast<float*>(lse); a.delta = delta;
+  a.dq = (uint16_t*)dq; a.dk = (uint16_t*)dk; a.dv = (uint16_t*)dv;
+  fill(a, strides, cu, T, B, H, HKV, D, scale);
+  DISPATCH_DP(D, run_bwd)
+}

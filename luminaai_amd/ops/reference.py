@@ -374,3 +374,51 @@ def token_logprobs(logits, tokens, top_k, ignore_index):
         ids = ids[:, :top_k].contiguous()
         top = logp.gather(1, ids)
     return lp, ent, top, ids
+
+
+# ------------------------------------------------------- packed attention
+def flash_attention_packed(q, k, v, cu_seqlens, scale):
+    """Sequence by sequence, fp32 (fp64 for fp64 input); autograd runs through
+    these operations. See ops/packed.py for the refusals' meaning."""
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
+        raise ValueError("q must be [tokens, heads, head_dim], k and v [tokens,"
+                         " kv_heads, head_dim]")
+    for t in (k, v):
+        if t.device != q.device:
+            raise ValueError(f"k or v is on {t.device}, not on {q.device}")
+        if t.dtype != q.dtype:
+            raise TypeError(f"k or v is {t.dtype}, not {q.dtype}")
+    T, H, D = q.shape
+    HKV = k.shape[1]
+    if k.shape[0] != T or k.shape[2] != D:
+        raise ValueError("q, k and v need the same tokens and head_dim")
+    if not 1 <= D <= 192:
+        raise ValueError(f"head_dim must be 1 to 192, got {D}")
+    if HKV == 0 or H == 0 or H % HKV:
+        raise ValueError(f"heads ({H}) must be a multiple of kv_heads ({HKV})")
+    _check_int32(cu_seqlens, q, 1, "cu_seqlens")
+    if cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens needs one entry more than there are "
+                         "sequences")
+    if not 0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive, got {scale}")
+    cu = cu_seqlens.tolist()
+    if cu[0] != 0 or cu[-1] > T or any(b < a for a, b in zip(cu, cu[1:])):
+        raise ValueError("cu_seqlens must rise from 0 to at most the "
+                         f"{T} tokens")
+    wide = torch.promote_types(q.dtype, torch.float32)
+    outs = []
+    for a, b in zip(cu, cu[1:]):
+        if a == b:
+            continue
+        qs = q[a:b].to(wide).view(b - a, HKV, H // HKV, D).permute(1, 2, 0, 3)
+        ks, vs = (t[a:b].to(wide).transpose(0, 1)[:, None] for t in (k, v))
+        s = torch.matmul(qs, ks.transpose(-1, -2).contiguous()) * scale
+        tri = torch.ones(b - a, b - a, dtype=torch.bool, device=q.device).tril()
+        o = torch.matmul(s.masked_fill(~tri, float("-inf")).softmax(-1), vs)
+        outs.append(o.permute(2, 0, 1, 3).reshape(b - a, H, D).to(q.dtype))
+    # zeros, with gradients of zero for all three also where no sequence is
+    rest = q[cu[-1]:]
+    outs.append(rest.masked_fill(torch.ones_like(rest, dtype=torch.bool), 0)
+                + (k[:0].sum() + v[:0].sum()))
+    return torch.cat(outs)
