@@ -1006,9 +1006,12 @@ at::Tensor logprob_bwd(const at::Tensor& x, const at::Tensor& tok,
 
 // ---- packed attention ------------------------------------------------------
 namespace {
-// channels beside each other; heads and tokens may lie anywhere
+// Channels beside each other; heads and tokens may lie anywhere, the tokens not
+// further apart than a tile's 32-bit offsets reach.
 at::Tensor dense_channels(const at::Tensor& t) {
-  return t.stride(2) == 1 || t.size(2) == 1 ? t : t.contiguous();
+  const bool fine = (t.stride(2) == 1 || t.size(2) == 1) &&
+                    t.stride(0) >= 0 && t.stride(0) <= (1 << 23);
+  return fine ? t : t.contiguous();
 }
 }  // namespace
 
@@ -1040,6 +1043,14 @@ std::tuple<at::Tensor, at::Tensor> packed_attn_fwd(
   TORCH_CHECK_VALUE(scale > 0 && scale < INFINITY, "scale must be positive, got ",
                     scale);
   const c10::DeviceGuard guard(q_.device());
+  if (D < 8) {
+    // the kernels take 8 channels at least: zeros change no score
+    const auto r = packed_attn_fwd(at::constant_pad_nd(q_, {0, 8 - D}),
+                                   at::constant_pad_nd(k_, {0, 8 - D}),
+                                   at::constant_pad_nd(v_, {0, 8 - D}), cu,
+                                   scale, want_lse);
+    return {std::get<0>(r).narrow(2, 0, D).contiguous(), std::get<1>(r)};
+  }
   const auto q = dense_channels(q_), k = dense_channels(k_),
              v = dense_channels(v_);
   auto o = at::empty({T, H, D}, q.options());
@@ -1066,9 +1077,20 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
                     "the gradient must be of q's shape and device");
   TORCH_CHECK_TYPE(is_bf16(go_), "the gradient must be bf16");
   const c10::DeviceGuard guard(q_.device());
+  const int64_t T = q_.size(0), H = q_.size(1), D = q_.size(2);
+  const int64_t HKV = k_.size(1);
+  if (D < 8) {
+    auto wide = [D](const at::Tensor& t) {
+      return at::constant_pad_nd(t, {0, 8 - D});
+    };
+    const auto r = packed_attn_bwd(wide(go_), wide(q_), wide(k_), wide(v_),
+                                   wide(o), lse, cu, scale);
+    return {std::get<0>(r).narrow(2, 0, D).contiguous(),
+            std::get<1>(r).narrow(2, 0, D).contiguous(),
+            std::get<2>(r).narrow(2, 0, D).contiguous()};
+  }
   const auto q = dense_channels(q_), k = dense_channels(k_),
              v = dense_channels(v_), go = dense_channels(go_);
-  const int64_t T = q.size(0), H = q.size(1), D = q.size(2), HKV = k.size(1);
   auto dq = at::empty({T, H, D}, q.options());
   auto dk = at::empty({T, HKV, D}, q.options());
   auto dv = at::empty({T, HKV, D}, q.options());

@@ -2,7 +2,7 @@
 // (gfx950).
 //
 // q [T, H, D], k and v [T, HKV, D] bf16 in any strides with contiguous
-// channels; sequence b is the tokens cu[b] .. cu[b+1]. D <= 192 is padded to a
+// channels; sequence b is the tokens cu[b] .. cu[b+1]. 8 <= D <= 192 is padded to a
 // multiple of 32 (DP) while a tile is staged, not in memory.
 //
 //   forward   S = scale Q K^T, P = softmax(S), O = P V, lse2 = log2 sum 2^S2
@@ -24,7 +24,8 @@
 //   mod 64 dwords and the 16-byte piece index xor (row >> 2) & 3, which keeps
 //   both free of bank conflicts.
 // - Tiles go global -> registers -> LDS, loaded one step ahead; two LDS buffers,
-//   one barrier a step.
+//   one barrier a step. The last step loads its own tile once more: where a
+//   branch skipped the loads, their registers would be waited for at its end.
 #include "common.h"
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -124,70 +125,98 @@ template <int DP> struct Img {
   }
 };
 
-// 8 channels from 8 c on of a row of D: zero past D. Rows may start at any
+// 8 channels from 8 c on of a row of D >= 8: zero past D. Rows may start at any
 // element. A row's last, partial piece is read as the last 8 channels and
 // moved down.
 DEV_INLINE uintx4 load_piece(const uint16_t* row, int c, int D) {
   uintx4 v = {0, 0, 0, 0};
   const int off = 8 * c;
-  if (D >= 8) {
-    if (off < D) {
-      const int o = off < D - 8 ? off : D - 8;
-      __builtin_memcpy(&v, row + o, 16);
-      const int e = (8 - (D & 7)) & 7;
-      if (e) {                                       // uniform
-        uint32_t t[8] = {v[0], v[1], v[2], v[3], 0, 0, 0, 0};
-        if (e & 1) {
-          #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            t[i] = __builtin_amdgcn_alignbit(t[i + 1], t[i], 16);
-        }
-        if (e & 2) {
-          #pragma unroll
-          for (int i = 0; i < 4; ++i) t[i] = t[i + 1];
-        }
-        if (e & 4) {
-          #pragma unroll
-          for (int i = 0; i < 4; ++i) t[i] = t[i + 2];
-        }
-        if (off != o) v = uintx4{t[0], t[1], t[2], t[3]};
+  if (off < D) {
+    const int o = off < D - 8 ? off : D - 8;
+    __builtin_memcpy(&v, row + o, 16);
+    const int e = off - o;
+    if (e) {
+      uint16_t t[16] = {};
+      __builtin_memcpy(t, &v, 16);
+      #pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint16_t x = 0;
+        #pragma unroll
+        for (int f = 1; f < 8; ++f)
+          if (f == e && j + f < 8) x = t[j + f];
+        v[j >> 1] = j & 1 ? (v[j >> 1] & 0xffffu) | ((uint32_t)x << 16)
+                          : (v[j >> 1] & 0xffff0000u) | x;
       }
     }
-  } else {
-    #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (off + j < D) v[j >> 1] |= (uint32_t)row[off + j] << (16 * (j & 1));
   }
   return v;
 }
 
-// A tile of ROWS rows in registers, NT threads.
-template <int DP, int ROWS, int NT>
+// A tile of ROWS rows on its way from memory to LDS, in the registers of NT
+// threads. Channels past D are not cleared: they meet zeros in the other
+// operand's fragment (load_piece), or columns that are not stored. They repeat
+// the row's own channels, never what lies behind it.
+template <int DP, int ROWS, int NT, bool ODD>   // ODD: D % 8 != 0
 struct Stage {
   static constexpr int PIECES = ROWS * DP / 8;
   static constexpr int N = (PIECES + NT - 1) / NT;
   uintx4 v[N];
-  // rows past `last` repeat it: nothing outside the sequence is read
-  DEV_INLINE void load(const uint16_t* base, int64_t st, int row0, int last,
-                       int D) {
+  uint32_t roff[N], coff[N];                 // bytes of the row and in it
+
+  static DEV_INLINE int piece(int i) {
+    // threads past the end repeat the last piece
+    const int p = threadIdx.x + i * NT;
+    return PIECES % NT == 0 || p < PIECES ? p : PIECES - 1;
+  }
+  DEV_INLINE void init(int64_t st, int D) {
     #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int p = threadIdx.x + i * NT;
-      if (PIECES % NT == 0 || p < PIECES) {
-        const int row = p / (DP / 8), c = p - row * (DP / 8);
-        const int r = row0 + row < last ? row0 + row : last;
-        v[i] = load_piece(base + r * st, c, D);
-      }
+      const int row = piece(i) / (DP / 8), c = piece(i) - row * (DP / 8);
+      roff[i] = 2 * (uint32_t)(row * (int)st);
+      coff[i] = 2 * (8 * c < D - 8 ? 8 * c : D - 8);
     }
   }
-  DEV_INLINE void store(char* img) const {
+  // base: the tile's first row; rows past `lim` repeat that one, so that
+  // nothing outside the sequence is read. No branch: a register that two paths
+  // load is waited for where they meet, which lays the latency bare.
+  DEV_INLINE void load(const uint16_t* base, int64_t st, int lim) {
+    const char* b = reinterpret_cast<const char*>(base);
+    const uint32_t most = 2 * (uint32_t)((lim < ROWS ? lim : ROWS) * (int)st);
+    #pragma unroll
+    for (int i = 0; i < N; ++i)
+      __builtin_memcpy(&v[i], b + ((roff[i] < most ? roff[i] : most) + coff[i]),
+                       16);
+  }
+  // a row's last, partial piece was read as its last 8 channels: move it down
+  DEV_INLINE void align(int D) {
+    if (!ODD) return;
+    const int e = 8 - (D & 7);
     #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int p = threadIdx.x + i * NT;
-      if (PIECES % NT == 0 || p < PIECES) {
-        const int row = p / (DP / 8), c = p - row * (DP / 8);
-        *reinterpret_cast<uintx4*>(img + Img<DP>::at(row, c)) = v[i];
+      const int c = piece(i) % (DP / 8);
+      uint32_t t[8] = {v[i][0], v[i][1], v[i][2], v[i][3], 0, 0, 0, 0};
+      if (e & 1) {
+        #pragma unroll
+        for (int j = 0; j < 4; ++j)
+          t[j] = __builtin_amdgcn_alignbit(t[j + 1], t[j], 16);
       }
+      if (e & 2) {
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = t[j + 1];
+      }
+      if (e & 4) {
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = t[j + 2];
+      }
+      if (c == D / 8) v[i] = uintx4{t[0], t[1], t[2], t[3]};
+    }
+  }
+  DEV_INLINE void store(char* img, int D) {
+    align(D);
+    #pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int row = piece(i) / (DP / 8), c = piece(i) - row * (DP / 8);
+      *reinterpret_cast<uintx4*>(img + Img<DP>::at(row, c)) = v[i];
     }
   }
 };
@@ -279,7 +308,7 @@ DEV_INLINE void zero_rows(uint16_t* out, int heads, int head, int D, int from,
 #define FQ (32 * FW)           // query rows of a workgroup
 #define FK 64                  // keys of a step
 
-template <int DP>
+template <int DP, bool ODD>
 __global__ __launch_bounds__(64 * FW, 2)
 void packed_fwd_kernel(const PackedArgs a) {
   constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * FW;
@@ -317,19 +346,21 @@ void packed_fwd_kernel(const PackedArgs a) {
   // keys up to the last query of the workgroup, or of the sequence
   const int kend = q0 + FQ < w.len ? q0 + FQ : w.len;
   const int steps = (kend + FK - 1) / FK;
-  Stage<DP, FK, NT> sk, sv;
-  sk.load(kb, a.k_st, 0, last, a.D);
-  sv.load(vb, a.v_st, 0, last, a.D);
-  sk.store(lds);
-  sv.store(lds + IMG);
+  Stage<DP, FK, NT, ODD> sk, sv;
+  sk.init(a.k_st, a.D);
+  sv.init(a.v_st, a.D);
+  sk.load(kb, a.k_st, last);
+  sv.load(vb, a.v_st, last);
+  sk.store(lds, a.D);
+  sv.store(lds + IMG, a.D);
   __syncthreads();
   for (int t = 0; t < steps; ++t) {
     const char* ki = lds + (t & 1) * 2 * IMG;
     const char* vi = ki + IMG;
-    const bool more = t + 1 < steps;
-    if (more) {
-      sk.load(kb, a.k_st, (t + 1) * FK, last, a.D);
-      sv.load(vb, a.v_st, (t + 1) * FK, last, a.D);
+    {
+      const int64_t r = (int64_t)(t + 1 < steps ? t + 1 : t) * FK;
+      sk.load(kb + r * a.k_st, a.k_st, last - (int)r);
+      sv.load(vb + r * a.v_st, a.v_st, last - (int)r);
     }
     const int k0 = t * FK;
     if (k0 <= qw + 31) {                     // else all masked for this wave
@@ -387,11 +418,9 @@ void packed_fwd_kernel(const PackedArgs a) {
         }
       }
     }
-    if (more) {
-      char* next = lds + ((t + 1) & 1) * 2 * IMG;
-      sk.store(next);
-      sv.store(next + IMG);
-    }
+    char* next = lds + ((t + 1) & 1) * 2 * IMG;
+    sk.store(next, a.D);
+    sv.store(next + IMG, a.D);
     __syncthreads();
   }
   l += __shfl_xor(l, 32, 64);
@@ -413,7 +442,7 @@ void packed_fwd_kernel(const PackedArgs a) {
 #define BQ (32 * BW)
 #define BK 32                  // keys of a step
 
-template <int DP>
+template <int DP, bool ODD>
 __global__ __launch_bounds__(64 * BW, DP <= 128 ? 2 : 1)
 void packed_dq_kernel(const PackedArgs a) {
   constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * BW;
@@ -462,19 +491,21 @@ void packed_dq_kernel(const PackedArgs a) {
 
   const int kend = q0 + BQ < w.len ? q0 + BQ : w.len;
   const int steps = (kend + BK - 1) / BK;
-  Stage<DP, BK, NT> sk, sv;
-  sk.load(kb, a.k_st, 0, last, a.D);
-  sv.load(vb, a.v_st, 0, last, a.D);
-  sk.store(lds);
-  sv.store(lds + IMG);
+  Stage<DP, BK, NT, ODD> sk, sv;
+  sk.init(a.k_st, a.D);
+  sv.init(a.v_st, a.D);
+  sk.load(kb, a.k_st, last);
+  sv.load(vb, a.v_st, last);
+  sk.store(lds, a.D);
+  sv.store(lds + IMG, a.D);
   __syncthreads();
   for (int t = 0; t < steps; ++t) {
     const char* ki = lds + (t & 1) * 2 * IMG;
     const char* vi = ki + IMG;
-    const bool more = t + 1 < steps;
-    if (more) {
-      sk.load(kb, a.k_st, (t + 1) * BK, last, a.D);
-      sv.load(vb, a.v_st, (t + 1) * BK, last, a.D);
+    {
+      const int64_t r = (int64_t)(t + 1 < steps ? t + 1 : t) * BK;
+      sk.load(kb + r * a.k_st, a.k_st, last - (int)r);
+      sv.load(vb + r * a.v_st, a.v_st, last - (int)r);
     }
     const int k0 = t * BK;
     if (k0 <= qw + 31) {
@@ -500,11 +531,9 @@ void packed_dq_kernel(const PackedArgs a) {
           dq[dt] = mfma(col_frag<DP>(ki, 16 * st, lane, dt), f, dq[dt]);
       }
     }
-    if (more) {
-      char* next = lds + ((t + 1) & 1) * 2 * IMG;
-      sk.store(next);
-      sv.store(next + IMG);
-    }
+    char* next = lds + ((t + 1) & 1) * 2 * IMG;
+    sk.store(next, a.D);
+    sv.store(next + IMG, a.D);
     __syncthreads();
   }
   if (qi < w.len)
@@ -521,7 +550,7 @@ void packed_dq_kernel(const PackedArgs a) {
 #define BKV (32 * BW)
 #define BQT 32                 // queries of a step
 
-template <int DP>
+template <int DP, bool ODD>
 __global__ __launch_bounds__(64 * BW, DP <= 96 ? 2 : 1)
 void packed_dkdv_kernel(const PackedArgs a) {
   constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * BW;
@@ -562,13 +591,14 @@ void packed_dkdv_kernel(const PackedArgs a) {
 
   const int per = (w.len - kv0 + BQT - 1) / BQT;   // steps of one head
   const int steps = per * G;
-  Stage<DP, BQT, NT> sq, sg;
+  Stage<DP, BQT, NT, ODD> sq, sg;
   float slab = 0.f;
   auto load = [&](int t) {
     const int g = t / per, qt = kv0 + (t - g * per) * BQT;
     const int h = hk * G + g;
-    sq.load(a.q + w.start * a.q_st + h * a.q_sh, a.q_st, qt, last, a.D);
-    sg.load(a.go + w.start * a.go_st + h * a.go_sh, a.go_st, qt, last, a.D);
+    const int64_t r = w.start + qt;
+    sq.load(a.q + r * a.q_st + h * a.q_sh, a.q_st, last - qt);
+    sg.load(a.go + r * a.go_st + h * a.go_sh, a.go_st, last - qt);
     if (threadIdx.x < 2 * BQT) {
       // lse2 = +inf makes P zero for rows past the end
       const int r = qt + (threadIdx.x & (BQT - 1));
@@ -578,11 +608,13 @@ void packed_dkdv_kernel(const PackedArgs a) {
     }
   };
   auto store = [&](char* buf) {
-    sq.store(buf);
-    sg.store(buf + IMG);
+    sq.store(buf, a.D);
+    sg.store(buf + IMG, a.D);
     if (threadIdx.x < 2 * BQT)
       reinterpret_cast<float*>(buf + 2 * IMG)[threadIdx.x] = slab;
   };
+  sq.init(a.q_st, a.D);
+  sg.init(a.go_st, a.D);
   load(0);
   store(lds);
   __syncthreads();
@@ -590,8 +622,7 @@ void packed_dkdv_kernel(const PackedArgs a) {
     const char* qi = lds + (t & 1) * BUF;
     const char* gi = qi + IMG;
     const float* ls = reinterpret_cast<const float*>(qi + 2 * IMG);
-    const bool more = t + 1 < steps;
-    if (more) load(t + 1);
+    load(t + 1 < steps ? t + 1 : t);
     const int qt = kv0 + (t % per) * BQT;
     if (qt + BQT - 1 >= kw) {                  // else all masked for this wave
       f32x16 s = zero16(), dp = zero16();
@@ -625,7 +656,7 @@ void packed_dkdv_kernel(const PackedArgs a) {
         }
       }
     }
-    if (more) store(lds + ((t + 1) & 1) * BUF);
+    store(lds + ((t + 1) & 1) * BUF);
     __syncthreads();
   }
   if (ki < w.len) {
@@ -640,23 +671,23 @@ static int64_t max_blocks(const PackedArgs& a, int rows) {
   return a.T / rows + a.B + 1;
 }
 
-template <int DP>
+template <int DP, bool ODD>
 static hipError_t run_fwd(const PackedArgs& a, hipStream_t stream) {
   const int64_t n = max_blocks(a, FQ) * a.H;
   if (n > 0x7fffffff) return hipErrorInvalidValue;
-  packed_fwd_kernel<DP><<<dim3((uint32_t)n), dim3(64 * FW), 0, stream>>>(a);
+  packed_fwd_kernel<DP, ODD><<<dim3((uint32_t)n), dim3(64 * FW), 0, stream>>>(a);
   HIP_CHECK_LAST();
   return hipSuccess;
 }
 
-template <int DP>
+template <int DP, bool ODD>
 static hipError_t run_bwd(const PackedArgs& a, hipStream_t stream) {
   const int64_t n = max_blocks(a, BQ) * a.H;
   if (n > 0x7fffffff) return hipErrorInvalidValue;
-  packed_dq_kernel<DP><<<dim3((uint32_t)n), dim3(64 * BW), 0, stream>>>(a);
+  packed_dq_kernel<DP, ODD><<<dim3((uint32_t)n), dim3(64 * BW), 0, stream>>>(a);
   HIP_CHECK_LAST();
   const int64_t m = max_blocks(a, BKV) * a.HKV;
-  packed_dkdv_kernel<DP><<<dim3((uint32_t)m), dim3(64 * BW), 0, stream>>>(a);
+  packed_dkdv_kernel<DP, ODD><<<dim3((uint32_t)m), dim3(64 * BW), 0, stream>>>(a);
   HIP_CHECK_LAST();
   return hipSuccess;
 }
@@ -669,11 +700,20 @@ static void fill(PackedArgs& a, const int64_t* st, const int* cu, int T, int B,
 }
 
 #define DISPATCH_DP(D, FN)                                                   \
-  if ((D) <= 64) return FN<64>(a, stream);                                   \
-  if ((D) <= 96) return FN<96>(a, stream);                                   \
-  if ((D) <= 128) return FN<128>(a, stream);                                 \
-  if ((D) <= 160) return FN<160>(a, stream);                                 \
-  if ((D) <= 192) return FN<192>(a, stream);                                 \
+  if ((D) < 8) return hipErrorInvalidValue;                                  \
+  if ((D) & 7) {                                                             \
+    if ((D) <= 64) return FN<64, true>(a, stream);                           \
+    if ((D) <= 96) return FN<96, true>(a, stream);                           \
+    if ((D) <= 128) return FN<128, true>(a, stream);                         \
+    if ((D) <= 160) return FN<160, true>(a, stream);                         \
+    if ((D) <= 192) return FN<192, true>(a, stream);                         \
+    return hipErrorInvalidValue;                                             \
+  }                                                                          \
+  if ((D) <= 64) return FN<64, false>(a, stream);                            \
+  if ((D) <= 96) return FN<96, false>(a, stream);                            \
+  if ((D) <= 128) return FN<128, false>(a, stream);                          \
+  if ((D) <= 160) return FN<160, false>(a, stream);                          \
+  if ((D) <= 192) return FN<192, false>(a, stream);                          \
   return hipErrorInvalidValue;
 
 extern "C" hipError_t lumina_packed_attn_fwd(
