@@ -34,6 +34,8 @@ typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(2))) float floatx2;
 typedef __attribute__((ext_vector_type(2))) uint32_t uintx2;
+// 16 bytes at any element: one load, gfx950 takes any alignment there
+typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t uintx4_any;
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 #define LOG2E 1.4426950408889634f
@@ -133,21 +135,15 @@ DEV_INLINE uintx4 load_piece(const uint16_t* row, int c, int D) {
   const int off = 8 * c;
   if (off < D) {
     const int o = off < D - 8 ? off : D - 8;
-    __builtin_memcpy(&v, row + o, 16);
+    v = *reinterpret_cast<const uintx4_any*>(row + o);
     const int e = off - o;
-    if (e) {
-      uint16_t t[16] = {};
-      __builtin_memcpy(t, &v, 16);
+    if (e & 1) {
       #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint16_t x = 0;
-        #pragma unroll
-        for (int f = 1; f < 8; ++f)
-          if (f == e && j + f < 8) x = t[j + f];
-        v[j >> 1] = j & 1 ? (v[j >> 1] & 0xffffu) | ((uint32_t)x << 16)
-                          : (v[j >> 1] & 0xffff0000u) | x;
-      }
+      for (int j = 0; j < 4; ++j)
+        v[j] = __builtin_amdgcn_alignbit(j < 3 ? v[j + 1] : 0, v[j], 16);
     }
+    if (e & 2) v = uintx4{v[1], v[2], v[3], 0};
+    if (e & 4) v = uintx4{v[2], v[3], 0, 0};
   }
   return v;
 }
@@ -184,31 +180,35 @@ struct Stage {
     const uint32_t most = 2 * (uint32_t)((lim < ROWS ? lim : ROWS) * (int)st);
     #pragma unroll
     for (int i = 0; i < N; ++i)
-      __builtin_memcpy(&v[i], b + ((roff[i] < most ? roff[i] : most) + coff[i]),
-                       16);
+      v[i] = *reinterpret_cast<const uintx4_any*>(
+          b + ((roff[i] < most ? roff[i] : most) + coff[i]));
   }
   // a row's last, partial piece was read as its last 8 channels: move it down
   DEV_INLINE void align(int D) {
     if (!ODD) return;
-    const int e = 8 - (D & 7);
+    const int e = 8 - (D & 7);               // by so many, the same everywhere
+    bool part[N];
     #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = piece(i) % (DP / 8);
-      uint32_t t[8] = {v[i][0], v[i][1], v[i][2], v[i][3], 0, 0, 0, 0};
-      if (e & 1) {
+    for (int i = 0; i < N; ++i) part[i] = piece(i) % (DP / 8) == D / 8;
+    if (e & 1) {
+      #pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t w[5] = {v[i][0], v[i][1], v[i][2], v[i][3], 0};
         #pragma unroll
         for (int j = 0; j < 4; ++j)
-          t[j] = __builtin_amdgcn_alignbit(t[j + 1], t[j], 16);
+          v[i][j] = part[i] ? __builtin_amdgcn_alignbit(w[j + 1], w[j], 16)
+                            : w[j];
       }
-      if (e & 2) {
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) t[j] = t[j + 1];
-      }
-      if (e & 4) {
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) t[j] = t[j + 2];
-      }
-      if (c == D / 8) v[i] = uintx4{t[0], t[1], t[2], t[3]};
+    }
+    if (e & 2) {
+      #pragma unroll
+      for (int i = 0; i < N; ++i)
+        v[i] = part[i] ? uintx4{v[i][1], v[i][2], v[i][3], 0} : v[i];
+    }
+    if (e & 4) {
+      #pragma unroll
+      for (int i = 0; i < N; ++i)
+        v[i] = part[i] ? uintx4{v[i][2], v[i][3], 0, 0} : v[i];
     }
   }
   DEV_INLINE void store(char* img, int D) {
