@@ -76,7 +76,7 @@ hipError_t lumina_moe_combine_fwd(const void*, const float*, const int64_t*, voi
 hipError_t lumina_moe_combine_bwd_y(const void*, const float*, const int64_t*, const int64_t*, const bool*, void*, int64_t, int64_t, int, int, hipStream_t);
 hipError_t lumina_moe_combine_bwd_w(const void*, const void*, const int64_t*, float*, int64_t, int, int, int64_t, int, hipStream_t);
 hipError_t lumina_packed_attn_fwd(const void*, const void*, const void*, void*, float*, const int*, const int64_t*, int, int, int, int, int, float, hipStream_t);
-hipError_t lumina_packed_attn_bwd(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, const int*, const int64_t*, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_packed_attn_bwd(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, float*, int, const int*, const int64_t*, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_paged_attn(const void*, const void*, const void*, void*, const int*, const int*, float*, float*, const int64_t*, int64_t, int, int, int, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_paged_append(const void*, const void*, void*, void*, const int*, const int*, const int*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int, int, hipStream_t);
 hipError_t lumina_copy_pages(void* const*, int, const int64_t*, const int64_t*, int, int64_t, const int*, const int*, int64_t, hipStream_t);
@@ -1096,6 +1096,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
   auto dv = at::empty({T, HKV, D}, q.options());
   if (T == 0) return {dq, dk, dv};
   auto delta = at::empty({H, T}, lse.options());
+  // dK / dV: a workgroup goes over at most T queries of its heads, and the causal
+  // half of all (query, key, head) pairs is spread over 256 units. Where the
+  // longest one alone takes more than such a share (T * HKV below 2 * 128 * 256
+  // pairs' worth), the group's heads are split, at the price of fp32 results
+  // that are written and read once more.
+  const int64_t G = H / HKV;
+  int64_t splits = 1;
+  while (splits < G && (G % splits != 0 || splits * HKV * T < 65536)) ++splits;
+  at::Tensor part;
+  if (splits > 1) part = at::empty({2, splits, T, HKV, D}, lse.options());
   const int64_t strides[8] = {q.stride(0), q.stride(1), k.stride(0),
                               k.stride(1), v.stride(0), v.stride(1),
                               go.stride(0), go.stride(1)};
@@ -1104,6 +1114,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
                                    lse.data_ptr<float>(),
                                    delta.data_ptr<float>(), dq.data_ptr(),
                                    dk.data_ptr(), dv.data_ptr(),
+                                   splits > 1 ? part.data_ptr<float>()
+                                              : nullptr, (int)splits,
                                    cu.data_ptr<int>(), strides, (int)T,
                                    (int)cu.size(0) - 1, (int)H, (int)HKV,
                                    (int)D, (float)scale, cur_stream()),

@@ -50,26 +50,45 @@ struct PackedArgs {
   uint16_t* dq;                // [T, H, D]
   uint16_t* dk;                // [T, HKV, D]
   uint16_t* dv;
+  float* part;                 // [2 (dk, dv), splits, T, HKV, D]
   float* lse;                  // [H, T], log2 units; +inf where nothing summed
   float* delta;                // [H, T]
   const int* cu;               // [B + 1]
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, go_st, go_sh;
   int T, B, H, HKV, D;
+  int splits;                  // parts of a group's heads in dK / dV
   float scale;
 };
 
 // ---- which rows a workgroup takes ------------------------------------------
 struct Work {
   int start;                   // the sequence's first token
-  int len;                     // its length; 0: nothing to do
-  int block;                   // block of rows inside it, the last ones first
+  int len;                     // its length
+  int level;                   // its blocks number 1 .. n by rising work
   int tail;                    // >= 0: rows behind the last sequence start here
 };
 
+// sum over the wave, the same in every lane
+DEV_INLINE int wave_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // row_bcast
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 // Block `id` of all sequences' blocks of `rows` rows, then the blocks of the
 // rows behind the last sequence. cu[0] counts as 0 and the rest is cut to [0, T],
-// so that no content of it leads outside the tensors. Every wave scans it: 64
-// sequences a step, from L2.
+// so that no content of it leads outside the tensors. Every wave finds its block
+// by itself, from L2.
+//
+// Up to 64 sequences: the blocks with the most work first, over all sequences,
+// so that the launch does not end with a few long ones. A sequence of n blocks
+// has one of each level 1 .. n, hence sum max(0, n - x + 1) blocks are of level
+// x or more, and the level is found by bisection. More sequences: one after the
+// other, each from its longest block on.
 DEV_INLINE Work find_work(const int* cu, int B, int T, int id, int rows) {
   const int lane = threadIdx.x & 63;
   Work w = {0, 0, 0, -1};
@@ -85,22 +104,43 @@ DEV_INLINE Work find_work(const int* cu, int B, int T, int id, int rows) {
       n = e > s ? e - s : 0;
     }
     const int nb = (n + rows - 1) / rows;
-    int sum = nb;                         // inclusive prefix sum
-    #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += x;
-    }
-    const int at = id - before - (sum - nb);
-    const unsigned long long hit = __ballot(at >= 0 && at < nb);
-    if (hit) {
-      const int src = __builtin_ctzll(hit);
-      w.start = __builtin_amdgcn_readlane(s, src);
-      w.len = __builtin_amdgcn_readlane(n, src);
-      w.block = __builtin_amdgcn_readlane(nb - 1 - at, src);
+    const int all = wave_sum(nb);
+    if (id - before < all) {
+      int at = id - before, level, rank = at;
+      if (B <= 64) {
+        int lo = 1, hi = (T + rows - 1) / rows + 1, above = 0;
+        while (hi - lo > 1) {                // blocks of level lo or more: > at
+          const int mid = (lo + hi) >> 1;
+          const int more = wave_sum(nb >= mid ? nb - mid + 1 : 0);
+          if (more > at) {
+            lo = mid;
+          } else {
+            hi = mid;
+            above = more;
+          }
+        }
+        level = lo;
+        rank = at - above;                   // among the sequences that have it
+        unsigned long long has = __ballot(nb >= level);
+        for (int i = 0; i < rank; ++i) has &= has - 1;
+        rank = __builtin_ctzll(has | (1ull << 63));
+      } else {
+        int sum = nb;                        // inclusive prefix sum
+        #pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int x = __shfl_up(sum, o, 64);
+          if (lane >= o) sum += x;
+        }
+        at -= sum - nb;
+        rank = __builtin_ctzll(__ballot(at >= 0 && at < nb) | (1ull << 63));
+        level = __builtin_amdgcn_readlane(nb - at, rank);
+      }
+      w.start = __builtin_amdgcn_readlane(s, rank);
+      w.len = __builtin_amdgcn_readlane(n, rank);
+      w.level = level;
       return w;
     }
-    before += __builtin_amdgcn_readlane(sum, 63);
+    before += all;
   }
   int end = B > 0 ? cu[B] : 0;
   end = end < 0 ? 0 : (end > T ? T : end);
@@ -323,7 +363,7 @@ void packed_fwd_kernel(const PackedArgs a) {
   const int lane = threadIdx.x & 63, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hk = h / (a.H / a.HKV);
-  const int q0 = w.block * FQ, qw = q0 + 32 * wave;
+  const int q0 = (w.level - 1) * FQ, qw = q0 + 32 * wave;
   const int last = w.len - 1;
   const uint16_t* kb = a.k + w.start * a.k_st + hk * a.k_sh;
   const uint16_t* vb = a.v + w.start * a.v_st + hk * a.v_sh;
@@ -457,7 +497,7 @@ void packed_dq_kernel(const PackedArgs a) {
   const int lane = threadIdx.x & 63, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hk = h / (a.H / a.HKV);
-  const int q0 = w.block * BQ, qw = q0 + 32 * wave;
+  const int q0 = (w.level - 1) * BQ, qw = q0 + 32 * wave;
   const int last = w.len - 1;
   const uint16_t* kb = a.k + w.start * a.k_st + hk * a.k_sh;
   const uint16_t* vb = a.v + w.start * a.v_st + hk * a.v_sh;
@@ -541,70 +581,94 @@ void packed_dq_kernel(const PackedArgs a) {
 }
 
 // ===========================================================================
-// dK and dV: a workgroup takes BKV keys of one kv head, a wave 32 of them, and
-// goes over the queries of all heads that share it, so the sum over the heads
-// stays in registers and has one order. S has rows = queries (registers),
-// columns = keys (lanes): P and dS are then B fragments of dV^T = dO^T P and
-// dK^T = Q^T dS, and the images of Q and dO serve rows and columns.
+// dK and dV: a workgroup takes BKV keys of one kv head and goes over the queries
+// of the heads that share it, so the sum over those heads stays in registers
+// and has one order. S has rows = queries (registers), columns = keys (lanes): P
+// and dS are then B fragments of dV^T = dO^T P and dK^T = Q^T dS, and the images
+// of Q and dO serve rows and columns.
+//
+// Two waves share 32 keys: one computes S, P and dV, the other dP, dS and dK,
+// a step behind, with P handed over in LDS (fp32, as it lies in the
+// registers). Each then holds one accumulator and one of K and V, which leaves
+// two waves a SIMD for every head_dim, and one's exponentials run under the
+// other's products. One wave for all of it took 1015 us for 8192 tokens of 32:8
+// heads x 128 (410 registers, one wave a SIMD).
+//
+// Where T * HKV / BKV workgroups of uneven length would not fill the chip, a
+// group's heads are split over `splits` workgroups, whose fp32 results
+// packed_join_kernel adds in order.
 // ===========================================================================
-#define BKV (32 * BW)
+#define BKV 128
 #define BQT 32                 // queries of a step
+#define BKW 8                  // waves: 4 of each kind
 
 template <int DP, bool ODD>
-__global__ __launch_bounds__(64 * BW, DP <= 96 ? 2 : 1)
+__global__ __launch_bounds__(64 * BKW, 2)
 void packed_dkdv_kernel(const PackedArgs a) {
-  constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * BW;
+  constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * BKW;
   constexpr int IMG = BQT * Img<DP>::BYTES;
   constexpr int BUF = 2 * IMG + 2 * BQT * 4;   // Q, dO, lse2, delta
-  __shared__ char lds[2 * BUF];
-  const int hk = head_of(blockIdx.x % a.HKV, a.HKV);
-  const Work w = find_work(a.cu, a.B, a.T, blockIdx.x / a.HKV, BKV);
+  constexpr int PB = 32 * 32 * 4;              // P of one pair of waves
+  __shared__ char lds[3 * BUF + 2 * 4 * PB];
+  int id = blockIdx.x;
+  const int hk = head_of(id % a.HKV, a.HKV);
+  id /= a.HKV;
+  const int split = id % a.splits;
+  const Work w = find_work(a.cu, a.B, a.T, id / a.splits, BKV);
   if (w.tail >= 0) {
-    zero_rows(a.dk, a.HKV, hk, a.D, w.tail, a.T, BKV);
-    zero_rows(a.dv, a.HKV, hk, a.D, w.tail, a.T, BKV);
+    if (split == 0) {
+      zero_rows(a.dk, a.HKV, hk, a.D, w.tail, a.T, BKV);
+      zero_rows(a.dv, a.HKV, hk, a.D, w.tail, a.T, BKV);
+    }
     return;
   }
   const int lane = threadIdx.x & 63, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int G = a.H / a.HKV;
-  // the first keys have the most queries: they go first
-  const int blocks = (w.len + BKV - 1) / BKV;
-  const int kv0 = (blocks - 1 - w.block) * BKV, kw = kv0 + 32 * wave;
+  const bool first = wave < 4;                 // S, P, dV; else dP, dS, dK
+  const int pair = wave & 3;
+  const int G = a.H / a.HKV, heads = G / a.splits;
+  const int h0 = hk * G + split * heads;
+  // the first keys have the most queries
+  const int kv0 = ((w.len + BKV - 1) / BKV - w.level) * BKV;
+  const int kw = kv0 + 32 * pair;
   const int last = w.len - 1;
   const int ki = kw + (lane & 31);             // this lane's key
   const int64_t tok = w.start + (ki < last ? ki : last);
 
-  bf16x8 kf[KS], vf[KS];
+  bf16x8 kvf[KS];                              // K's or V's rows
   {
-    const uint16_t* kr = a.k + tok * a.k_st + hk * a.k_sh;
-    const uint16_t* vr = a.v + tok * a.v_st + hk * a.v_sh;
+    const uint16_t* r = first ? a.k + tok * a.k_st + hk * a.k_sh
+                              : a.v + tok * a.v_st + hk * a.v_sh;
     #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      kf[ks] = __builtin_bit_cast(bf16x8, load_piece(kr, 2 * ks + hi, a.D));
-      vf[ks] = __builtin_bit_cast(bf16x8, load_piece(vr, 2 * ks + hi, a.D));
-    }
+    for (int ks = 0; ks < KS; ++ks)
+      kvf[ks] = __builtin_bit_cast(bf16x8, load_piece(r, 2 * ks + hi, a.D));
   }
-  f32x16 dk[DT], dv[DT];
+  f32x16 acc[DT];                              // dV^T or dK^T
   #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) { dk[dt] = zero16(); dv[dt] = zero16(); }
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = zero16();
   const float c2 = a.scale * LOG2E;
 
   const int per = (w.len - kv0 + BQT - 1) / BQT;   // steps of one head
-  const int steps = per * G;
+  const int steps = per * heads;
   Stage<DP, BQT, NT, ODD> sq, sg;
   float slab = 0.f;
-  auto load = [&](int t) {
-    const int g = t / per, qt = kv0 + (t - g * per) * BQT;
-    const int h = hk * G + g;
-    const int64_t r = w.start + qt;
-    sq.load(a.q + r * a.q_st + h * a.q_sh, a.q_st, last - qt);
-    sg.load(a.go + r * a.go_st + h * a.go_sh, a.go_st, last - qt);
-    if (threadIdx.x < 2 * BQT) {
-      // lse2 = +inf makes P zero for rows past the end
-      const int r = qt + (threadIdx.x & (BQT - 1));
-      const float* src = threadIdx.x < BQT ? a.lse : a.delta;
-      slab = r <= last ? src[(int64_t)h * a.T + w.start + r]
-                       : (threadIdx.x < BQT ? INFINITY : 0.f);
+  int lh = h0, lq = kv0;                       // head and query to load
+  auto load = [&]() {
+    const int64_t r = w.start + lq;
+    sq.load(a.q + r * a.q_st + lh * a.q_sh, a.q_st, last - lq);
+    sg.load(a.go + r * a.go_st + lh * a.go_sh, a.go_st, last - lq);
+    // lse2 = +inf makes P zero for rows past the end
+    const int i = threadIdx.x & (BQT - 1);
+    const float* src = threadIdx.x & BQT ? a.delta : a.lse;
+    const int row = lq + i;
+    slab = src[(int64_t)lh * a.T + w.start + (row < last ? row : last)];
+    if (row > last) slab = threadIdx.x & BQT ? 0.f : INFINITY;
+  };
+  auto next = [&](int& h, int& q) {
+    q += BQT;
+    if (q > last) {
+      q = kv0;
+      ++h;
     }
   };
   auto store = [&](char* buf) {
@@ -615,53 +679,122 @@ void packed_dkdv_kernel(const PackedArgs a) {
   };
   sq.init(a.q_st, a.D);
   sg.init(a.go_st, a.D);
-  load(0);
+  load();
   store(lds);
   __syncthreads();
-  for (int t = 0; t < steps; ++t) {
-    const char* qi = lds + (t & 1) * BUF;
+  int qt = kv0, dummy = 0;                     // the step's first query
+  int buf = 0;
+  // step t: the first kind takes tile t, the second tile t - 1, and tile t + 1
+  // is loaded; three buffers go round
+  for (int t = 0; t <= steps; ++t) {
+    if (t + 1 < steps) next(lh, lq);
+    load();
+    const int mine = first ? buf : (buf == 0 ? 2 : buf - 1);
+    const char* qi = lds + mine * BUF;
     const char* gi = qi + IMG;
     const float* ls = reinterpret_cast<const float*>(qi + 2 * IMG);
-    load(t + 1 < steps ? t + 1 : t);
-    const int qt = kv0 + (t % per) * BQT;
-    if (qt + BQT - 1 >= kw) {                  // else all masked for this wave
-      f32x16 s = zero16(), dp = zero16();
+    const bool live = first ? t < steps : t > 0;
+    if (live && qt + BQT - 1 >= kw) {          // else all masked for this pair
+      char* pb = lds + 3 * BUF + ((first ? t : t - 1) & 1) * 4 * PB + pair * PB
+                 + lane * 16;
+      const char* ri = first ? qi : gi;        // rows, then columns
+      const char* ci = first ? gi : qi;
+      f32x16 s = zero16();
       #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        s = mfma(row_frag<DP>(qi, 0, lane, ks), kf[ks], s);
-        dp = mfma(row_frag<DP>(gi, 0, lane, ks), vf[ks], dp);
-      }
-      float p[16], ds[16];
-      #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const floatx4 le = *reinterpret_cast<const floatx4*>(ls + 8 * g + 4 * hi);
-        const floatx4 de = *reinterpret_cast<const floatx4*>(
-            ls + BQT + 8 * g + 4 * hi);
+      for (int ks = 0; ks < KS; ++ks)
+        s = mfma(row_frag<DP>(ri, 0, lane, ks), kvf[ks], s);
+      float p[16];
+      if (first) {
         #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = 4 * g + j;
-          float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -le[j]));
-          if (ki > qt + 8 * g + 4 * hi + j) x = 0.f;
-          p[r] = x;
-          ds[r] = x * (dp[r] - de[j]);
+        for (int g = 0; g < 4; ++g) {
+          const floatx4 le = *reinterpret_cast<const floatx4*>(ls + 8 * g
+                                                               + 4 * hi);
+          #pragma unroll
+          for (int j = 0; j < 4; ++j)
+            p[4 * g + j] = __builtin_amdgcn_exp2f(
+                __builtin_fmaf(s[4 * g + j], c2, -le[j]));
+        }
+        if (qt < kw + 31) {                    // touches the diagonal
+          #pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (ki > qt + 8 * (r >> 2) + 4 * hi + (r & 3)) p[r] = 0.f;
+        }
+        #pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<floatx4*>(pb + 1024 * g) =
+              floatx4{p[4 * g], p[4 * g + 1], p[4 * g + 2], p[4 * g + 3]};
+      } else {
+        #pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const floatx4 de = *reinterpret_cast<const floatx4*>(
+              ls + BQT + 8 * g + 4 * hi);
+          const floatx4 x = *reinterpret_cast<const floatx4*>(pb + 1024 * g);
+          #pragma unroll
+          for (int j = 0; j < 4; ++j)
+            p[4 * g + j] = x[j] * (s[4 * g + j] - de[j]);
         }
       }
       #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        const bf16x8 pf = pack_frag(&p[8 * st]), df = pack_frag(&ds[8 * st]);
+        const bf16x8 pf = pack_frag(&p[8 * st]);
         #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          dv[dt] = mfma(col_frag<DP>(gi, 16 * st, lane, dt), pf, dv[dt]);
-          dk[dt] = mfma(col_frag<DP>(qi, 16 * st, lane, dt), df, dk[dt]);
-        }
+        for (int dt = 0; dt < DT; ++dt)
+          acc[dt] = mfma(col_frag<DP>(ci, 16 * st, lane, dt), pf, acc[dt]);
       }
     }
-    store(lds + ((t + 1) & 1) * BUF);
+    buf = buf == 2 ? 0 : buf + 1;
+    store(lds + buf * BUF);
+    if (live) next(dummy, qt);
     __syncthreads();
   }
   if (ki < w.len) {
-    store_col<DT>(a.dk + (tok * a.HKV + hk) * a.D, dk, a.scale, hi, a.D);
-    store_col<DT>(a.dv + (tok * a.HKV + hk) * a.D, dv, 1.f, hi, a.D);
+    const float f = first ? 1.f : a.scale;
+    if (a.splits == 1) {
+      store_col<DT>((first ? a.dv : a.dk) + (tok * a.HKV + hk) * a.D, acc, f,
+                    hi, a.D);
+    } else {
+      float* row = a.part + ((((int64_t)(first ? 1 : 0) * a.splits + split)
+                              * a.T + tok) * a.HKV + hk) * a.D;
+      #pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        #pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = 32 * dt + 8 * (r >> 2) + 4 * hi + (r & 3);
+          if (d < a.D) row[d] = acc[dt][r] * f;
+        }
+    }
+  }
+}
+
+// Adds the splits' results in order, for the rows of the sequences.
+__global__ __launch_bounds__(256)
+void packed_join_kernel(const PackedArgs a) {
+  int end = a.B > 0 ? a.cu[a.B] : 0;
+  end = end < 0 ? 0 : (end > a.T ? a.T : end);
+  const int64_t n = (int64_t)a.T * a.HKV * a.D;
+  const int64_t live = (int64_t)end * a.HKV * a.D;
+  const float* part = a.part + blockIdx.y * a.splits * n;
+  uint16_t* out = blockIdx.y ? a.dv : a.dk;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < live;
+       i += (int64_t)gridDim.x * 1024) {
+    const int m = live - i < 4 ? (int)(live - i) : 4;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) {
+      if (m == 4) {
+        floatx4 y;
+        __builtin_memcpy(&y, part + s * n + i, 16);
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += y[j];
+      } else {
+        for (int j = 0; j < m; ++j) x[j] += part[s * n + i + j];
+      }
+    }
+    if (m == 4) {
+      const uintx2 u = {pack2(x[0], x[1]), pack2(x[2], x[3])};
+      __builtin_memcpy(out + i, &u, 8);
+    } else {
+      for (int j = 0; j < m; ++j) out[i + j] = f32_to_bf16(x[j]);
+    }
   }
 }
 
@@ -686,9 +819,17 @@ static hipError_t run_bwd(const PackedArgs& a, hipStream_t stream) {
   if (n > 0x7fffffff) return hipErrorInvalidValue;
   packed_dq_kernel<DP, ODD><<<dim3((uint32_t)n), dim3(64 * BW), 0, stream>>>(a);
   HIP_CHECK_LAST();
-  const int64_t m = max_blocks(a, BKV) * a.HKV;
-  packed_dkdv_kernel<DP, ODD><<<dim3((uint32_t)m), dim3(64 * BW), 0, stream>>>(a);
+  const int64_t m = max_blocks(a, BKV) * a.HKV * a.splits;
+  if (m > 0x7fffffff) return hipErrorInvalidValue;
+  packed_dkdv_kernel<DP, ODD><<<dim3((uint32_t)m), dim3(64 * BKW), 0,
+                                stream>>>(a);
   HIP_CHECK_LAST();
+  if (a.splits > 1) {
+    const int64_t each = (int64_t)a.T * a.HKV * a.D;
+    packed_join_kernel<<<dim3(elementwise_grid(each, 256, 4), 2), dim3(256), 0,
+                         stream>>>(a);
+    HIP_CHECK_LAST();
+  }
   return hipSuccess;
 }
 
@@ -729,13 +870,14 @@ extern "C" hipError_t lumina_packed_attn_fwd(
 
 extern "C" hipError_t lumina_packed_attn_bwd(
     const void* q, const void* k, const void* v, const void* o, const void* go,
-    const float* lse, float* delta, void* dq, void* dk, void* dv,
-    const int* cu, const int64_t* strides, int T, int B, int H, int HKV, int D,
-    float scale, hipStream_t stream) {
+    const float* lse, float* delta, void* dq, void* dk, void* dv, float* part,
+    int splits, const int* cu, const int64_t* strides, int T, int B, int H,
+    int HKV, int D, float scale, hipStream_t stream) {
   PackedArgs a = {};
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
   a.o = (const uint16_t*)o; a.go = (const uint16_t*)go;
   a.lse = const_cast<float*>(lse); a.delta = delta;
+  a.part = part; a.splits = splits;
   a.dq = (uint16_t*)dq; a.dk = (uint16_t*)dk; a.dv = (uint16_t*)dv;
   fill(a, strides, cu, T, B, H, HKV, D, scale);
   DISPATCH_DP(D, run_bwd)
