@@ -483,11 +483,16 @@ void packed_fwd_kernel(const PackedArgs a) {
 #define BK 32                  // keys of a step
 
 template <int DP, bool ODD>
-__global__ __launch_bounds__(64 * BW, DP <= 128 ? 2 : 1)
+__global__ __launch_bounds__(64 * BW, DP <= 160 ? 2 : 1)
 void packed_dq_kernel(const PackedArgs a) {
   constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * BW;
   constexpr int IMG = BK * Img<DP>::BYTES;
-  __shared__ char lds[4 * IMG];
+  // Two waves a SIMD have 256 registers: at DP = 160 that leaves no room for
+  // dO's fragments, which go through an image of the wave's own instead. At 192
+  // the images would not fit twice; one wave a SIMD then has 512 registers.
+  constexpr bool GO_LDS = DP == 160;
+  constexpr int OWN = GO_LDS ? 32 * Img<DP>::BYTES : 0;
+  __shared__ char lds[4 * IMG + BW * OWN];
   const int h = head_of(blockIdx.x % a.H, a.H);
   const Work w = find_work(a.cu, a.B, a.T, blockIdx.x / a.H, BQ);
   if (w.tail >= 0) {
@@ -504,7 +509,8 @@ void packed_dq_kernel(const PackedArgs a) {
   const int qi = qw + (lane & 31);
   const int64_t tok = w.start + (qi < last ? qi : last);
 
-  bf16x8 qf[KS], gf[KS];
+  bf16x8 qf[KS], gf[GO_LDS ? 1 : KS];
+  char* own = lds + 4 * IMG + wave * OWN;
   float delta = 0.f;
   {
     const uint16_t* qr = a.q + tok * a.q_st + h * a.q_sh;
@@ -513,12 +519,18 @@ void packed_dq_kernel(const PackedArgs a) {
     #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qf[ks] = __builtin_bit_cast(bf16x8, load_piece(qr, 2 * ks + hi, a.D));
-      gf[ks] = __builtin_bit_cast(bf16x8, load_piece(gr, 2 * ks + hi, a.D));
+      const bf16x8 gk = __builtin_bit_cast(bf16x8,
+                                           load_piece(gr, 2 * ks + hi, a.D));
+      if (GO_LDS)
+        *reinterpret_cast<bf16x8*>(own + Img<DP>::at(lane & 31, 2 * ks + hi)) =
+            gk;
+      else
+        gf[ks] = gk;
       const bf16x8 of = __builtin_bit_cast(
           bf16x8, load_piece(orow, 2 * ks + hi, a.D));
       #pragma unroll
       for (int j = 0; j < 8; ++j)
-        delta = __builtin_fmaf((float)gf[ks][j], (float)of[j], delta);
+        delta = __builtin_fmaf((float)gk[j], (float)of[j], delta);
     }
     delta += __shfl_xor(delta, 32, 64);
   }
@@ -553,7 +565,9 @@ void packed_dq_kernel(const PackedArgs a) {
       #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         s = mfma(row_frag<DP>(ki, 0, lane, ks), qf[ks], s);
-        dp = mfma(row_frag<DP>(vi, 0, lane, ks), gf[ks], dp);
+        dp = mfma(row_frag<DP>(vi, 0, lane, ks),
+                  GO_LDS ? row_frag<DP>(own, 0, lane, ks) : gf[GO_LDS ? 0 : ks],
+                  dp);
       }
       float ds[16];
       #pragma unroll
