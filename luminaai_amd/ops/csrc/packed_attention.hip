@@ -223,68 +223,85 @@ struct Stage {
       v[i] = *reinterpret_cast<const uintx4_any*>(
           b + ((roff[i] < most ? roff[i] : most) + coff[i]));
   }
-  // a row's last, partial piece was read as its last 8 channels: move it down
-  DEV_INLINE void align(int D) {
-    if (!ODD) return;
-    const int e = 8 - (D & 7);               // by so many, the same everywhere
-    bool part[N];
+  DEV_INLINE void store(char* img, int D) const {
+    uintx4 x[N];
     #pragma unroll
-    for (int i = 0; i < N; ++i) part[i] = piece(i) % (DP / 8) == D / 8;
-    if (e & 1) {
+    for (int i = 0; i < N; ++i) x[i] = v[i];
+    if (ODD) {
+      // a row's last, partial piece was read as its last 8 channels: move it
+      // down by so many, the same everywhere
+      const int e = 8 - (D & 7);
+      bool part[N];
       #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t w[5] = {v[i][0], v[i][1], v[i][2], v[i][3], 0};
+      for (int i = 0; i < N; ++i) part[i] = piece(i) % (DP / 8) == D / 8;
+      if (e & 1) {
         #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          v[i][j] = part[i] ? __builtin_amdgcn_alignbit(w[j + 1], w[j], 16)
-                            : w[j];
+        for (int i = 0; i < N; ++i) {
+          const uint32_t w[5] = {x[i][0], x[i][1], x[i][2], x[i][3], 0};
+          #pragma unroll
+          for (int j = 0; j < 4; ++j)
+            x[i][j] = part[i] ? __builtin_amdgcn_alignbit(w[j + 1], w[j], 16)
+                              : w[j];
+        }
+      }
+      if (e & 2) {
+        #pragma unroll
+        for (int i = 0; i < N; ++i)
+          x[i] = part[i] ? uintx4{x[i][1], x[i][2], x[i][3], 0} : x[i];
+      }
+      if (e & 4) {
+        #pragma unroll
+        for (int i = 0; i < N; ++i)
+          x[i] = part[i] ? uintx4{x[i][2], x[i][3], 0, 0} : x[i];
       }
     }
-    if (e & 2) {
-      #pragma unroll
-      for (int i = 0; i < N; ++i)
-        v[i] = part[i] ? uintx4{v[i][1], v[i][2], v[i][3], 0} : v[i];
-    }
-    if (e & 4) {
-      #pragma unroll
-      for (int i = 0; i < N; ++i)
-        v[i] = part[i] ? uintx4{v[i][2], v[i][3], 0, 0} : v[i];
-    }
-  }
-  DEV_INLINE void store(char* img, int D) {
-    align(D);
     #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int row = piece(i) / (DP / 8), c = piece(i) - row * (DP / 8);
-      *reinterpret_cast<uintx4*>(img + Img<DP>::at(row, c)) = v[i];
+      *reinterpret_cast<uintx4*>(img + Img<DP>::at(row, c)) = x[i];
     }
   }
 };
 
-// A or B fragment of step ks: row lane & 31 (+ row0), channels 16 ks + 8 hi ..
+// A or B fragment of step ks: row lane & 31, channels 16 ks + 8 hi ..
+// A lane keeps two addresses, for even and odd ks; the rest is an offset that the
+// instruction holds.
 template <int DP>
-DEV_INLINE bf16x8 row_frag(const char* img, int row0, int lane, int ks) {
-  return *reinterpret_cast<const bf16x8*>(
-      img + Img<DP>::at(row0 + (lane & 31), 2 * ks + (lane >> 5)));
-}
+struct RowAddr {
+  uint32_t even, odd;
+  DEV_INLINE void init(int lane) {
+    even = Img<DP>::at(lane & 31, lane >> 5);
+    odd = Img<DP>::at(lane & 31, 2 + (lane >> 5));
+  }
+  DEV_INLINE bf16x8 get(const char* img, int ks) const {
+    return *reinterpret_cast<const bf16x8*>(img + (ks & 1 ? odd : even)
+                                            + 64 * (ks >> 1));
+  }
+};
 
 // A fragment of the transposed tile: channel 32 dt + (lane & 31), rows
-// r0 + 4 hi + {0..3} and r0 + 8 + 4 hi + {0..3}. ds_read_b64_tr_b16 hands lane
-// l of 16 the l-th channel of the four rows whose 8-byte pieces the lanes
-// address: lane l points at row l >> 2, channels 4 (l & 3) ..
+// r0 + 4 hi + {0..3} and r0 + 8 + 4 hi + {0..3}, r0 a multiple of 16.
+// ds_read_b64_tr_b16 hands lane l of 16 the l-th channel of the four rows whose
+// 8-byte pieces the lanes address: lane l points at row l >> 2, channels
+// 4 (l & 3) .. Two addresses again, for the two groups of rows.
 template <int DP>
-DEV_INLINE bf16x8 col_frag(const char* img, int r0, int lane, int dt) {
-  const int l = lane & 15;
-  const int row = r0 + 4 * (lane >> 5) + (l >> 2);
-  const int ch = 32 * dt + (lane & 16) + 4 * (l & 3);
-  const int sub = (ch & 4) * 2;
-  union { bf16x4 h[2]; bf16x8 v; } u;
-  u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-      (lds_bf16x4*)(img + Img<DP>::at(row, ch >> 3) + sub));
-  u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-      (lds_bf16x4*)(img + Img<DP>::at(row + 8, ch >> 3) + sub));
-  return u.v;
-}
+struct ColAddr {
+  uint32_t low, high;
+  DEV_INLINE void init(int lane) {
+    const int l = lane & 15;
+    const int row = 4 * (lane >> 5) + (l >> 2);
+    const int ch = (lane & 16) + 4 * (l & 3);
+    low = Img<DP>::at(row, ch >> 3) + (ch & 4) * 2;
+    high = Img<DP>::at(row + 8, ch >> 3) + (ch & 4) * 2;
+  }
+  DEV_INLINE bf16x8 get(const char* img, int r0, int dt) const {
+    const char* p = img + r0 * Img<DP>::BYTES + 64 * dt;
+    union { bf16x4 h[2]; bf16x8 v; } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p + low));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p + high));
+    return u.v;
+  }
+};
 
 DEV_INLINE uint32_t pack2(float lo, float hi) {
   floatx2 f = {lo, hi};
@@ -307,6 +324,21 @@ DEV_INLINE f32x16 zero16() {
 
 DEV_INLINE f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Order of the N products of a block whose operands come from LDS, READS reads
+// each: four products' reads ahead, then one more with each product. Left to
+// itself the compiler keeps one read in flight, whose latency is two products.
+template <int N, int READS>
+DEV_INLINE void reads_ahead() {
+  constexpr int AHEAD = N < 4 ? N : 4;
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);   // LDS reads
+  #pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // products
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
 }
 
 // A column of a transposed result: this lane's row of memory takes channels
@@ -369,6 +401,10 @@ void packed_fwd_kernel(const PackedArgs a) {
   const uint16_t* vb = a.v + w.start * a.v_st + hk * a.v_sh;
   const int qi = qw + (lane & 31);           // this lane's query
 
+  RowAddr<DP> rows;
+  ColAddr<DP> cols;
+  rows.init(lane);
+  cols.init(lane);
   bf16x8 qf[KS];
   {
     const uint16_t* qr = a.q + (int64_t)(w.start + (qi < last ? qi : last))
@@ -410,7 +446,7 @@ void packed_fwd_kernel(const PackedArgs a) {
         f32x16 s = zero16();
         #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-          s = mfma(row_frag<DP>(ki, 32 * kk, lane, ks), qf[ks], s);
+          s = mfma(rows.get(ki + 32 * kk * Img<DP>::BYTES, ks), qf[ks], s);
         #pragma unroll
         for (int r = 0; r < 16; ++r) p[kk][r] = s[r];
       }
@@ -453,8 +489,7 @@ void packed_fwd_kernel(const PackedArgs a) {
           const bf16x8 pf = pack_frag(&p[kk][8 * s]);
           #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
-            o[dt] = mfma(col_frag<DP>(vi, 32 * kk + 16 * s, lane, dt), pf,
-                         o[dt]);
+            o[dt] = mfma(cols.get(vi, 32 * kk + 16 * s, dt), pf, o[dt]);
         }
       }
     }
@@ -509,6 +544,10 @@ void packed_dq_kernel(const PackedArgs a) {
   const int qi = qw + (lane & 31);
   const int64_t tok = w.start + (qi < last ? qi : last);
 
+  RowAddr<DP> rows;
+  ColAddr<DP> cols;
+  rows.init(lane);
+  cols.init(lane);
   bf16x8 qf[KS], gf[GO_LDS ? 1 : KS];
   char* own = lds + 4 * IMG + wave * OWN;
   float delta = 0.f;
@@ -564,11 +603,11 @@ void packed_dq_kernel(const PackedArgs a) {
       f32x16 s = zero16(), dp = zero16();
       #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        s = mfma(row_frag<DP>(ki, 0, lane, ks), qf[ks], s);
-        dp = mfma(row_frag<DP>(vi, 0, lane, ks),
-                  GO_LDS ? row_frag<DP>(own, 0, lane, ks) : gf[GO_LDS ? 0 : ks],
-                  dp);
+        s = mfma(rows.get(ki, ks), qf[ks], s);
+        dp = mfma(rows.get(vi, ks),
+                  GO_LDS ? rows.get(own, ks) : gf[GO_LDS ? 0 : ks], dp);
       }
+      reads_ahead<2 * KS, 1>();
       float ds[16];
       #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -582,7 +621,7 @@ void packed_dq_kernel(const PackedArgs a) {
         const bf16x8 f = pack_frag(&ds[8 * st]);
         #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
-          dq[dt] = mfma(col_frag<DP>(ki, 16 * st, lane, dt), f, dq[dt]);
+          dq[dt] = mfma(cols.get(ki, 16 * st, dt), f, dq[dt]);
       }
     }
     char* next = lds + ((t + 1) & 1) * 2 * IMG;
@@ -649,6 +688,10 @@ void packed_dkdv_kernel(const PackedArgs a) {
   const int ki = kw + (lane & 31);             // this lane's key
   const int64_t tok = w.start + (ki < last ? ki : last);
 
+  RowAddr<DP> rows;
+  ColAddr<DP> cols;
+  rows.init(lane);
+  cols.init(lane);
   bf16x8 kvf[KS];                              // K's or V's rows
   {
     const uint16_t* r = first ? a.k + tok * a.k_st + hk * a.k_sh
@@ -666,24 +709,30 @@ void packed_dkdv_kernel(const PackedArgs a) {
   const int steps = per * heads;
   Stage<DP, BQT, NT, ODD> sq, sg;
   float slab = 0.f;
-  int lh = h0, lq = kv0;                       // head and query to load
+  // the tile to load: its first query and where its rows lie
+  int lq = kv0;
+  const uint16_t* qp = a.q + (int64_t)(w.start + kv0) * a.q_st + h0 * a.q_sh;
+  const uint16_t* gp = a.go + (int64_t)(w.start + kv0) * a.go_st + h0 * a.go_sh;
+  const int si = threadIdx.x & (BQT - 1);
+  const float* sp = (threadIdx.x & BQT ? a.delta : a.lse)
+                    + (int64_t)h0 * a.T + w.start;
+  const int64_t q_next = BQT * a.q_st, g_next = BQT * a.go_st;
+  const int64_t q_head = a.q_sh - (per - 1) * q_next;
+  const int64_t g_head = a.go_sh - (per - 1) * g_next;
   auto load = [&]() {
-    const int64_t r = w.start + lq;
-    sq.load(a.q + r * a.q_st + lh * a.q_sh, a.q_st, last - lq);
-    sg.load(a.go + r * a.go_st + lh * a.go_sh, a.go_st, last - lq);
+    sq.load(qp, a.q_st, last - lq);
+    sg.load(gp, a.go_st, last - lq);
     // lse2 = +inf makes P zero for rows past the end
-    const int i = threadIdx.x & (BQT - 1);
-    const float* src = threadIdx.x & BQT ? a.delta : a.lse;
-    const int row = lq + i;
-    slab = src[(int64_t)lh * a.T + w.start + (row < last ? row : last)];
+    const int row = lq + si;
+    slab = sp[row < last ? row : last];
     if (row > last) slab = threadIdx.x & BQT ? 0.f : INFINITY;
   };
-  auto next = [&](int& h, int& q) {
-    q += BQT;
-    if (q > last) {
-      q = kv0;
-      ++h;
-    }
+  auto advance = [&]() {
+    const bool wrap = lq + BQT > last;
+    lq = wrap ? kv0 : lq + BQT;
+    qp += wrap ? q_head : q_next;
+    gp += wrap ? g_head : g_next;
+    sp += wrap ? a.T : 0;
   };
   auto store = [&](char* buf) {
     sq.store(buf, a.D);
@@ -696,12 +745,12 @@ void packed_dkdv_kernel(const PackedArgs a) {
   load();
   store(lds);
   __syncthreads();
-  int qt = kv0, dummy = 0;                     // the step's first query
+  int qt = kv0;                                // the step's first query
   int buf = 0;
   // step t: the first kind takes tile t, the second tile t - 1, and tile t + 1
   // is loaded; three buffers go round
   for (int t = 0; t <= steps; ++t) {
-    if (t + 1 < steps) next(lh, lq);
+    if (t + 1 < steps) advance();
     load();
     const int mine = first ? buf : (buf == 0 ? 2 : buf - 1);
     const char* qi = lds + mine * BUF;
@@ -716,7 +765,8 @@ void packed_dkdv_kernel(const PackedArgs a) {
       f32x16 s = zero16();
       #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        s = mfma(row_frag<DP>(ri, 0, lane, ks), kvf[ks], s);
+        s = mfma(rows.get(ri, ks), kvf[ks], s);
+      reads_ahead<KS, 1>();
       float p[16];
       if (first) {
         #pragma unroll
@@ -753,12 +803,12 @@ void packed_dkdv_kernel(const PackedArgs a) {
         const bf16x8 pf = pack_frag(&p[8 * st]);
         #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
-          acc[dt] = mfma(col_frag<DP>(ci, 16 * st, lane, dt), pf, acc[dt]);
+          acc[dt] = mfma(cols.get(ci, 16 * st, dt), pf, acc[dt]);
       }
     }
     buf = buf == 2 ? 0 : buf + 1;
     store(lds + buf * BUF);
-    if (live) next(dummy, qt);
+    if (live) qt = qt + BQT > last ? kv0 : qt + BQT;
     __syncthreads();
   }
   if (ki < w.len) {
