@@ -1096,16 +1096,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
   auto dv = at::empty({T, HKV, D}, q.options());
   if (T == 0) return {dq, dk, dv};
   auto delta = at::empty({H, T}, lse.options());
-  // dK / dV: a workgroup goes over at most T queries of its heads, and the causal
-  // half of all (query, key, head) pairs is spread over 256 units. Where the
-  // longest one alone takes more than such a share (T * HKV below 2 * 128 * 256
-  // pairs' worth), the group's heads are split, at the price of fp32 results
-  // that are written and read once more.
+  // dK / dV: a workgroup goes over the queries of its 128 keys for all heads of
+  // the group. The causal half of all (query, key, head) pairs is spread over 256
+  // units, and the longest workgroup alone takes more than its share while
+  // T * HKV < 65536; twice that levels the rest. Below it the group's heads are
+  // split, at the price of fp32 results that are written and read once more.
+  // 8192 tokens: 8 kv heads x 4 x 128, 1 / 2 / 4 parts: 625 / 574 / 661 us;
+  // 4 kv heads x 3 x 159, 1 / 3 parts: 343 / 257 us.
   const int64_t G = H / HKV;
   int64_t splits = 1;
-  while (splits < G && (G % splits != 0 || splits * HKV * T < 65536)) ++splits;
+  while (splits < G && (G % splits != 0 || splits * HKV * T < 131072)) ++splits;
   at::Tensor part;
-  if (splits > 1) part = at::empty({2, splits, T, HKV, D}, lse.options());
+  if (splits > 1) part = at::empty({2, splits, T, HKV, (D + 3) / 4 * 4}, lse.options());
   const int64_t strides[8] = {q.stride(0), q.stride(1), k.stride(0),
                               k.stride(1), v.stride(0), v.stride(1),
                               go.stride(0), go.stride(1)};

@@ -50,7 +50,7 @@ struct PackedArgs {
   uint16_t* dq;                // [T, H, D]
   uint16_t* dk;                // [T, HKV, D]
   uint16_t* dv;
-  float* part;                 // [2 (dk, dv), splits, T, HKV, D]
+  float* part;                 // [2 (dk, dv), splits, T, HKV, D up to 4]
   float* lse;                  // [H, T], log2 units; +inf where nothing summed
   float* delta;                // [H, T]
   const int* cu;               // [B + 1]
@@ -341,23 +341,33 @@ DEV_INLINE void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
 }
 
-// A column of a transposed result: this lane's row of memory takes channels
-// 8 g + 4 hi + {0..3}, g = 0 .. 4 DT - 1.
+// A column of a transposed result: this lane's row of memory has channels
+// 8 g + 4 hi + {0..3}, g = 0 .. 4 DT - 1, in this lane and the rest in the lane
+// 32 away. They swap halves, and each stores 8 channels at once.
 template <int DT>
 DEV_INLINE void store_col(uint16_t* row, const f32x16* acc, float f, int hi,
-                          int D) {
+                          int D, bool live) {
   #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
     #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * dt + 8 * g + 4 * hi;
-      const uintx2 u = {pack2(acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f),
-                        pack2(acc[dt][4 * g + 2] * f, acc[dt][4 * g + 3] * f)};
-      if (d + 4 <= D) {
-        __builtin_memcpy(row + d, &u, 8);
+    for (int g = 0; g < 4; g += 2) {
+      uint32_t u[4];
+      #pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = 4 * g + 2 * j;
+        const auto x = __builtin_amdgcn_permlane32_swap(
+            pack2(acc[dt][r] * f, acc[dt][r + 1] * f),
+            pack2(acc[dt][r + 4] * f, acc[dt][r + 5] * f), false, false);
+        u[j] = x[0];
+        u[2 + j] = x[1];
+      }
+      const int d = 32 * dt + 8 * g + 8 * hi;
+      if (!live) continue;
+      if (d + 8 <= D) {
+        *reinterpret_cast<uintx4_any*>(row + d) = uintx4{u[0], u[1], u[2], u[3]};
       } else {
         #pragma unroll
-        for (int j = 0; j < 3; ++j)
+        for (int j = 0; j < 7; ++j)
           if (d + j < D) row[d + j] = (uint16_t)(u[j >> 1] >> (16 * (j & 1)));
       }
     }
@@ -499,14 +509,12 @@ void packed_fwd_kernel(const PackedArgs a) {
     __syncthreads();
   }
   l += __shfl_xor(l, 32, 64);
-  if (qi < w.len) {
-    const int64_t tok = w.start + qi;
-    store_col<DT>(a.out + (tok * a.H + h) * a.D, o, l == 0.f ? 0.f : 1.f / l,
-                  hi, a.D);
-    if (a.lse && hi == 0)
-      a.lse[(int64_t)h * a.T + tok] =
-          l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
-  }
+  const int64_t tok = w.start + qi;
+  store_col<DT>(a.out + (tok * a.H + h) * a.D, o, l == 0.f ? 0.f : 1.f / l, hi,
+                a.D, qi < w.len);
+  if (a.lse && hi == 0 && qi < w.len)
+    a.lse[(int64_t)h * a.T + tok] =
+        l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 // ===========================================================================
@@ -629,8 +637,8 @@ void packed_dq_kernel(const PackedArgs a) {
     sv.store(next + IMG, a.D);
     __syncthreads();
   }
-  if (qi < w.len)
-    store_col<DT>(a.dq + (tok * a.H + h) * a.D, dq, a.scale, hi, a.D);
+  store_col<DT>(a.dq + (tok * a.H + h) * a.D, dq, a.scale, hi, a.D,
+                qi < w.len);
 }
 
 // ===========================================================================
@@ -811,53 +819,53 @@ void packed_dkdv_kernel(const PackedArgs a) {
     if (live) qt = qt + BQT > last ? kv0 : qt + BQT;
     __syncthreads();
   }
-  if (ki < w.len) {
-    const float f = first ? 1.f : a.scale;
-    if (a.splits == 1) {
-      store_col<DT>((first ? a.dv : a.dk) + (tok * a.HKV + hk) * a.D, acc, f,
-                    hi, a.D);
-    } else {
-      float* row = a.part + ((((int64_t)(first ? 1 : 0) * a.splits + split)
-                              * a.T + tok) * a.HKV + hk) * a.D;
+  const float f = first ? 1.f : a.scale;
+  if (a.splits == 1) {
+    store_col<DT>((first ? a.dv : a.dk) + (tok * a.HKV + hk) * a.D, acc, f, hi,
+                  a.D, ki < w.len);
+  } else if (ki < w.len) {
+    const int pw = (a.D + 3) & ~3;
+    float* row = a.part + ((((int64_t)(first ? 1 : 0) * a.splits + split) * a.T
+                            + tok) * a.HKV + hk) * pw;
+    #pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
       #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int d = 32 * dt + 8 * (r >> 2) + 4 * hi + (r & 3);
-          if (d < a.D) row[d] = acc[dt][r] * f;
-        }
-    }
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * dt + 8 * g + 4 * hi;
+        if (d < pw)
+          *reinterpret_cast<floatx4*>(row + d) =
+              floatx4{acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f,
+                      acc[dt][4 * g + 2] * f, acc[dt][4 * g + 3] * f};
+      }
   }
 }
 
-// Adds the splits' results in order, for the rows of the sequences.
+// Adds the splits' results in order, for the rows of the sequences. A thread
+// takes four channels of a row.
 __global__ __launch_bounds__(256)
 void packed_join_kernel(const PackedArgs a) {
   int end = a.B > 0 ? a.cu[a.B] : 0;
   end = end < 0 ? 0 : (end > a.T ? a.T : end);
-  const int64_t n = (int64_t)a.T * a.HKV * a.D;
-  const int64_t live = (int64_t)end * a.HKV * a.D;
+  const int pw = (a.D + 3) & ~3, q = pw / 4;
+  const int64_t n = (int64_t)a.T * a.HKV * pw;
+  const int64_t live = (int64_t)end * a.HKV * q;
   const float* part = a.part + blockIdx.y * a.splits * n;
   uint16_t* out = blockIdx.y ? a.dv : a.dk;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < live;
-       i += (int64_t)gridDim.x * 1024) {
-    const int m = live - i < 4 ? (int)(live - i) : 4;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-      if (m == 4) {
-        floatx4 y;
-        __builtin_memcpy(&y, part + s * n + i, 16);
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] += y[j];
-      } else {
-        for (int j = 0; j < m; ++j) x[j] += part[s * n + i + j];
-      }
-    }
-    if (m == 4) {
-      const uintx2 u = {pack2(x[0], x[1]), pack2(x[2], x[3])};
-      __builtin_memcpy(out + i, &u, 8);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < live;
+       i += (int64_t)gridDim.x * 256) {
+    floatx4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s)
+      x += *reinterpret_cast<const floatx4*>(part + s * n + 4 * i);
+    const int64_t row = i / q;
+    const int d = 4 * (int)(i - row * q);
+    uint16_t* p = out + row * a.D + d;
+    const uintx2 u = {pack2(x[0], x[1]), pack2(x[2], x[3])};
+    if (d + 4 <= a.D) {
+      __builtin_memcpy(p, &u, 8);
     } else {
-      for (int j = 0; j < m; ++j) out[i + j] = f32_to_bf16(x[j]);
+      #pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (d + j < a.D) p[j] = (uint16_t)(u[j >> 1] >> (16 * (j & 1)));
     }
   }
 }
@@ -889,8 +897,8 @@ static hipError_t run_bwd(const PackedArgs& a, hipStream_t stream) {
                                 stream>>>(a);
   HIP_CHECK_LAST();
   if (a.splits > 1) {
-    const int64_t each = (int64_t)a.T * a.HKV * a.D;
-    packed_join_kernel<<<dim3(elementwise_grid(each, 256, 4), 2), dim3(256), 0,
+    const int64_t each = (int64_t)a.T * a.HKV * ((a.D + 3) / 4);
+    packed_join_kernel<<<dim3(elementwise_grid(each, 256, 2), 2), dim3(256), 0,
                          stream>>>(a);
     HIP_CHECK_LAST();
   }
