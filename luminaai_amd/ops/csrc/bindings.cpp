@@ -75,8 +75,9 @@ hipError_t lumina_moe_dispatch_bwd(const void*, const int64_t*, void*, int64_t, 
 hipError_t lumina_moe_combine_fwd(const void*, const float*, const int64_t*, void*, int64_t, int, int, int64_t, int, hipStream_t);
 hipError_t lumina_moe_combine_bwd_y(const void*, const float*, const int64_t*, const int64_t*, const bool*, void*, int64_t, int64_t, int, int, hipStream_t);
 hipError_t lumina_moe_combine_bwd_w(const void*, const void*, const int64_t*, float*, int64_t, int, int, int64_t, int, hipStream_t);
-hipError_t lumina_packed_attn_fwd(const void*, const void*, const void*, void*, float*, const int*, const int64_t*, int, int, int, int, int, float, hipStream_t);
-hipError_t lumina_packed_attn_bwd(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, float*, int, const int*, const int64_t*, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_packed_attn_fwd(const void*, const void*, const void*, void*, float*, const int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_packed_attn_bwd(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, float*, int, const int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_pack_rows(const void* const*, void* const*, const int64_t*, const int*, int, int64_t, int, hipStream_t);
 hipError_t lumina_paged_attn(const void*, const void*, const void*, void*, const int*, const int*, float*, float*, const int64_t*, int64_t, int, int, int, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_paged_append(const void*, const void*, void*, void*, const int*, const int*, const int*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int, int, hipStream_t);
 hipError_t lumina_copy_pages(void* const*, int, const int64_t*, const int64_t*, int, int64_t, const int*, const int*, int64_t, hipStream_t);
@@ -1006,28 +1007,56 @@ at::Tensor logprob_bwd(const at::Tensor& x, const at::Tensor& tok,
 
 // ---- packed attention ------------------------------------------------------
 namespace {
-// Channels beside each other; heads and tokens may lie anywhere, the tokens not
+// Rows as the kernels take them: whole aligned 16-byte pieces, and tokens no
 // further apart than a tile's 32-bit offsets reach.
-at::Tensor dense_channels(const at::Tensor& t) {
-  const bool fine = (t.stride(2) == 1 || t.size(2) == 1) &&
-                    t.stride(0) >= 0 && t.stride(0) <= (1 << 23);
-  return fine ? t : t.contiguous();
+bool aligned_rows(const at::Tensor& t) {
+  return t.size(2) % 8 == 0 && t.stride(2) == 1 && t.stride(0) % 8 == 0 &&
+         t.stride(1) % 8 == 0 && t.stride(0) >= 0 &&
+         t.stride(0) <= (1 << 23) && (uintptr_t)t.data_ptr() % 16 == 0;
+}
+
+// Those that are not become copies of head_dim rounded up to 8, zero past it;
+// all of them if one has to change its width.
+std::vector<at::Tensor> align_rows(std::vector<at::Tensor> ts) {
+  const int64_t T = ts[0].size(0), D = ts[0].size(2), W = (D + 7) / 8 * 8;
+  const void* src[3];
+  void* dst[3];
+  int64_t strides[6];
+  int heads[3], n = 0;
+  std::vector<at::Tensor> keep;
+  for (auto& t : ts) {
+    if (T == 0 || aligned_rows(t)) continue;
+    const at::Tensor s = t.stride(2) == 1 || D == 1 ? t : t.contiguous();
+    keep.push_back(s);
+    t = at::empty({T, s.size(1), W}, s.options());
+    src[n] = s.data_ptr();
+    dst[n] = t.data_ptr();
+    strides[2 * n] = s.stride(0);
+    strides[2 * n + 1] = s.stride(1);
+    heads[n++] = (int)s.size(1);
+  }
+  if (n > 0)
+    check_hip(lumina_pack_rows(src, dst, strides, heads, n, T, (int)D,
+                               cur_stream()), "flash_attention_packed");
+  return ts;
 }
 }  // namespace
 
-// -> (o, lse2); lse2 is empty where want_lse is false
-std::tuple<at::Tensor, at::Tensor> packed_attn_fwd(
-    const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
-    const at::Tensor& cu, double scale, bool want_lse) {
+// -> (o, lse2, q, k, v): lse2 is empty where want_lse is false; q, k and v as the
+// kernels read them, which is what packed_attn_bwd takes
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+packed_attn_fwd(const at::Tensor& q_, const at::Tensor& k_,
+                const at::Tensor& v_, const at::Tensor& cu, double scale,
+                bool want_lse) {
   TORCH_CHECK_VALUE(q_.dim() == 3 && k_.dim() == 3 && v_.sizes() == k_.sizes(),
                     "q must be [tokens, heads, head_dim], k and v [tokens, "
                     "kv_heads, head_dim]");
   TORCH_CHECK_TYPE(is_bf16(q_), "flash_attention_packed on the GPU takes bf16, "
                    "got ", q_.scalar_type());
-  for (const auto& t : {k_, v_}) {
-    check_same_device(t, q_, "k or v");
-    TORCH_CHECK_TYPE(t.scalar_type() == q_.scalar_type(), "k or v is ",
-                     t.scalar_type(), ", not ", q_.scalar_type());
+  for (const auto* t : {&k_, &v_}) {
+    check_same_device(*t, q_, "k or v");
+    TORCH_CHECK_TYPE(t->scalar_type() == q_.scalar_type(), "k or v is ",
+                     t->scalar_type(), ", not ", q_.scalar_type());
   }
   const int64_t T = q_.size(0), H = q_.size(1), D = q_.size(2);
   const int64_t HKV = k_.size(1);
@@ -1043,19 +1072,11 @@ std::tuple<at::Tensor, at::Tensor> packed_attn_fwd(
   TORCH_CHECK_VALUE(scale > 0 && scale < INFINITY, "scale must be positive, got ",
                     scale);
   const c10::DeviceGuard guard(q_.device());
-  if (D < 8) {
-    // the kernels take 8 channels at least: zeros change no score
-    const auto r = packed_attn_fwd(at::constant_pad_nd(q_, {0, 8 - D}),
-                                   at::constant_pad_nd(k_, {0, 8 - D}),
-                                   at::constant_pad_nd(v_, {0, 8 - D}), cu,
-                                   scale, want_lse);
-    return {std::get<0>(r).narrow(2, 0, D).contiguous(), std::get<1>(r)};
-  }
-  const auto q = dense_channels(q_), k = dense_channels(k_),
-             v = dense_channels(v_);
+  const auto in = align_rows({q_, k_, v_});
+  const auto &q = in[0], &k = in[1], &v = in[2];
   auto o = at::empty({T, H, D}, q.options());
   auto lse = at::empty({want_lse ? H : 0, T}, q.options().dtype(at::kFloat));
-  if (T == 0) return {o, lse};
+  if (T == 0) return {o, lse, q, k, v};
   const int64_t strides[8] = {q.stride(0), q.stride(1), k.stride(0),
                               k.stride(1), v.stride(0), v.stride(1), 0, 0};
   check_hip(lumina_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(),
@@ -1063,38 +1084,27 @@ std::tuple<at::Tensor, at::Tensor> packed_attn_fwd(
                                    want_lse ? lse.data_ptr<float>() : nullptr,
                                    cu.data_ptr<int>(), strides, (int)T,
                                    (int)cu.size(0) - 1, (int)H, (int)HKV,
-                                   (int)D, (float)scale, cur_stream()),
+                                   (int)q.size(2), (int)D, (float)scale,
+                                   cur_stream()),
             "flash_attention_packed");
-  return {o, lse};
+  return {o, lse, q, k, v};
 }
 
-// Takes what packed_attn_fwd took and gave.
+// Takes the gradient of o, and what packed_attn_fwd returned.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
-    const at::Tensor& go_, const at::Tensor& q_, const at::Tensor& k_,
-    const at::Tensor& v_, const at::Tensor& o, const at::Tensor& lse,
+    const at::Tensor& go_, const at::Tensor& o, const at::Tensor& lse,
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& cu, double scale) {
-  TORCH_CHECK_VALUE(go_.sizes() == q_.sizes() && go_.device() == q_.device(),
-                    "the gradient must be of q's shape and device");
+  TORCH_CHECK_VALUE(go_.sizes() == o.sizes() && go_.device() == o.device(),
+                    "the gradient must be of the result's shape and device");
   TORCH_CHECK_TYPE(is_bf16(go_), "the gradient must be bf16");
-  const c10::DeviceGuard guard(q_.device());
-  const int64_t T = q_.size(0), H = q_.size(1), D = q_.size(2);
-  const int64_t HKV = k_.size(1);
-  if (D < 8) {
-    auto wide = [D](const at::Tensor& t) {
-      return at::constant_pad_nd(t, {0, 8 - D});
-    };
-    const auto r = packed_attn_bwd(wide(go_), wide(q_), wide(k_), wide(v_),
-                                   wide(o), lse, cu, scale);
-    return {std::get<0>(r).narrow(2, 0, D).contiguous(),
-            std::get<1>(r).narrow(2, 0, D).contiguous(),
-            std::get<2>(r).narrow(2, 0, D).contiguous()};
-  }
-  const auto q = dense_channels(q_), k = dense_channels(k_),
-             v = dense_channels(v_), go = dense_channels(go_);
+  const c10::DeviceGuard guard(q.device());
+  const int64_t T = o.size(0), H = o.size(1), D = o.size(2), HKV = k.size(1);
   auto dq = at::empty({T, H, D}, q.options());
   auto dk = at::empty({T, HKV, D}, q.options());
   auto dv = at::empty({T, HKV, D}, q.options());
   if (T == 0) return {dq, dk, dv};
+  const auto go = align_rows({go_})[0];
   auto delta = at::empty({H, T}, lse.options());
   // dK / dV: a workgroup goes over the queries of its 128 keys for all heads of
   // the group. The causal half of all (query, key, head) pairs is spread over 256
@@ -1120,7 +1130,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
                                               : nullptr, (int)splits,
                                    cu.data_ptr<int>(), strides, (int)T,
                                    (int)cu.size(0) - 1, (int)H, (int)HKV,
-                                   (int)D, (float)scale, cur_stream()),
+                                   (int)q.size(2), (int)D, (float)scale,
+                                   cur_stream()),
             "flash_attention_packed gradient");
   return {dq, dk, dv};
 }

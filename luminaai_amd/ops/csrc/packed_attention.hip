@@ -55,7 +55,7 @@ struct PackedArgs {
   float* delta;                // [H, T]
   const int* cu;               // [B + 1]
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, go_st, go_sh;
-  int T, B, H, HKV, D;
+  int T, B, H, HKV, W, D;
   int splits;                  // parts of a group's heads in dK / dV
   float scale;
 };
@@ -167,32 +167,27 @@ template <int DP> struct Img {
   }
 };
 
-// 8 channels from 8 c on of a row of D >= 8: zero past D. Rows may start at any
-// element. A row's last, partial piece is read as the last 8 channels and
-// moved down.
-DEV_INLINE uintx4 load_piece(const uint16_t* row, int c, int D) {
+// 8 channels from 8 c on of a row, zero past its end
+DEV_INLINE uintx4 load_piece(const uint16_t* row, int c, int W) {
+  if (8 * c >= W) return uintx4{0, 0, 0, 0};
+  return *reinterpret_cast<const uintx4*>(row + 8 * c);
+}
+// the same for a row of any alignment and length
+DEV_INLINE uintx4 load_ragged(const uint16_t* row, int c, int D) {
+  const int n = D - 8 * c;
+  if (n >= 8) return *reinterpret_cast<const uintx4_any*>(row + 8 * c);
   uintx4 v = {0, 0, 0, 0};
-  const int off = 8 * c;
-  if (off < D) {
-    const int o = off < D - 8 ? off : D - 8;
-    v = *reinterpret_cast<const uintx4_any*>(row + o);
-    const int e = off - o;
-    if (e & 1) {
-      #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        v[j] = __builtin_amdgcn_alignbit(j < 3 ? v[j + 1] : 0, v[j], 16);
-    }
-    if (e & 2) v = uintx4{v[1], v[2], v[3], 0};
-    if (e & 4) v = uintx4{v[2], v[3], 0, 0};
-  }
+  #pragma unroll
+  for (int j = 0; j < 7; ++j)
+    if (j < n) v[j >> 1] |= (uint32_t)row[8 * c + j] << (16 * (j & 1));
   return v;
 }
 
 // A tile of ROWS rows on its way from memory to LDS, in the registers of NT
-// threads. Channels past D are not cleared: they meet zeros in the other
+// threads. Channels past W are not cleared: they meet zeros in the other
 // operand's fragment (load_piece), or columns that are not stored. They repeat
 // the row's own channels, never what lies behind it.
-template <int DP, int ROWS, int NT, bool ODD>   // ODD: D % 8 != 0
+template <int DP, int ROWS, int NT>
 struct Stage {
   static constexpr int PIECES = ROWS * DP / 8;
   static constexpr int N = (PIECES + NT - 1) / NT;
@@ -204,12 +199,12 @@ struct Stage {
     const int p = threadIdx.x + i * NT;
     return PIECES % NT == 0 || p < PIECES ? p : PIECES - 1;
   }
-  DEV_INLINE void init(int64_t st, int D) {
+  DEV_INLINE void init(int64_t st, int W) {
     #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int row = piece(i) / (DP / 8), c = piece(i) - row * (DP / 8);
       roff[i] = 2 * (uint32_t)(row * (int)st);
-      coff[i] = 2 * (8 * c < D - 8 ? 8 * c : D - 8);
+      coff[i] = 2 * (8 * c < W - 8 ? 8 * c : W - 8);
     }
   }
   // base: the tile's first row; rows past `lim` repeat that one, so that
@@ -220,45 +215,14 @@ struct Stage {
     const uint32_t most = 2 * (uint32_t)((lim < ROWS ? lim : ROWS) * (int)st);
     #pragma unroll
     for (int i = 0; i < N; ++i)
-      v[i] = *reinterpret_cast<const uintx4_any*>(
+      v[i] = *reinterpret_cast<const uintx4*>(
           b + ((roff[i] < most ? roff[i] : most) + coff[i]));
   }
-  DEV_INLINE void store(char* img, int D) const {
-    uintx4 x[N];
-    #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = v[i];
-    if (ODD) {
-      // a row's last, partial piece was read as its last 8 channels: move it
-      // down by so many, the same everywhere
-      const int e = 8 - (D & 7);
-      bool part[N];
-      #pragma unroll
-      for (int i = 0; i < N; ++i) part[i] = piece(i) % (DP / 8) == D / 8;
-      if (e & 1) {
-        #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint32_t w[5] = {x[i][0], x[i][1], x[i][2], x[i][3], 0};
-          #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            x[i][j] = part[i] ? __builtin_amdgcn_alignbit(w[j + 1], w[j], 16)
-                              : w[j];
-        }
-      }
-      if (e & 2) {
-        #pragma unroll
-        for (int i = 0; i < N; ++i)
-          x[i] = part[i] ? uintx4{x[i][1], x[i][2], x[i][3], 0} : x[i];
-      }
-      if (e & 4) {
-        #pragma unroll
-        for (int i = 0; i < N; ++i)
-          x[i] = part[i] ? uintx4{x[i][2], x[i][3], 0, 0} : x[i];
-      }
-    }
+  DEV_INLINE void store(char* img) const {
     #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int row = piece(i) / (DP / 8), c = piece(i) - row * (DP / 8);
-      *reinterpret_cast<uintx4*>(img + Img<DP>::at(row, c)) = x[i];
+      *reinterpret_cast<uintx4*>(img + Img<DP>::at(row, c)) = v[i];
     }
   }
 };
@@ -390,7 +354,7 @@ DEV_INLINE void zero_rows(uint16_t* out, int heads, int head, int D, int from,
 #define FQ (32 * FW)           // query rows of a workgroup
 #define FK 64                  // keys of a step
 
-template <int DP, bool ODD>
+template <int DP>
 __global__ __launch_bounds__(64 * FW, 2)
 void packed_fwd_kernel(const PackedArgs a) {
   constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * FW;
@@ -421,7 +385,7 @@ void packed_fwd_kernel(const PackedArgs a) {
                          * a.q_st + h * a.q_sh;
     #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
-      qf[ks] = __builtin_bit_cast(bf16x8, load_piece(qr, 2 * ks + hi, a.D));
+      qf[ks] = __builtin_bit_cast(bf16x8, load_piece(qr, 2 * ks + hi, a.W));
   }
   f32x16 o[DT];
   #pragma unroll
@@ -432,13 +396,13 @@ void packed_fwd_kernel(const PackedArgs a) {
   // keys up to the last query of the workgroup, or of the sequence
   const int kend = q0 + FQ < w.len ? q0 + FQ : w.len;
   const int steps = (kend + FK - 1) / FK;
-  Stage<DP, FK, NT, ODD> sk, sv;
-  sk.init(a.k_st, a.D);
-  sv.init(a.v_st, a.D);
+  Stage<DP, FK, NT> sk, sv;
+  sk.init(a.k_st, a.W);
+  sv.init(a.v_st, a.W);
   sk.load(kb, a.k_st, last);
   sv.load(vb, a.v_st, last);
-  sk.store(lds, a.D);
-  sv.store(lds + IMG, a.D);
+  sk.store(lds);
+  sv.store(lds + IMG);
   __syncthreads();
   for (int t = 0; t < steps; ++t) {
     const char* ki = lds + (t & 1) * 2 * IMG;
@@ -504,8 +468,8 @@ void packed_fwd_kernel(const PackedArgs a) {
       }
     }
     char* next = lds + ((t + 1) & 1) * 2 * IMG;
-    sk.store(next, a.D);
-    sv.store(next + IMG, a.D);
+    sk.store(next);
+    sv.store(next + IMG);
     __syncthreads();
   }
   l += __shfl_xor(l, 32, 64);
@@ -525,7 +489,7 @@ void packed_fwd_kernel(const PackedArgs a) {
 #define BQ (32 * BW)
 #define BK 32                  // keys of a step
 
-template <int DP, bool ODD>
+template <int DP>
 __global__ __launch_bounds__(64 * BW, DP <= 160 ? 2 : 1)
 void packed_dq_kernel(const PackedArgs a) {
   constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * BW;
@@ -565,16 +529,16 @@ void packed_dq_kernel(const PackedArgs a) {
     const uint16_t* orow = a.o + (tok * a.H + h) * a.D;
     #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      qf[ks] = __builtin_bit_cast(bf16x8, load_piece(qr, 2 * ks + hi, a.D));
+      qf[ks] = __builtin_bit_cast(bf16x8, load_piece(qr, 2 * ks + hi, a.W));
       const bf16x8 gk = __builtin_bit_cast(bf16x8,
-                                           load_piece(gr, 2 * ks + hi, a.D));
+                                           load_piece(gr, 2 * ks + hi, a.W));
       if (GO_LDS)
         *reinterpret_cast<bf16x8*>(own + Img<DP>::at(lane & 31, 2 * ks + hi)) =
             gk;
       else
         gf[ks] = gk;
       const bf16x8 of = __builtin_bit_cast(
-          bf16x8, load_piece(orow, 2 * ks + hi, a.D));
+          bf16x8, load_ragged(orow, 2 * ks + hi, a.D));
       #pragma unroll
       for (int j = 0; j < 8; ++j)
         delta = __builtin_fmaf((float)gk[j], (float)of[j], delta);
@@ -590,13 +554,13 @@ void packed_dq_kernel(const PackedArgs a) {
 
   const int kend = q0 + BQ < w.len ? q0 + BQ : w.len;
   const int steps = (kend + BK - 1) / BK;
-  Stage<DP, BK, NT, ODD> sk, sv;
-  sk.init(a.k_st, a.D);
-  sv.init(a.v_st, a.D);
+  Stage<DP, BK, NT> sk, sv;
+  sk.init(a.k_st, a.W);
+  sv.init(a.v_st, a.W);
   sk.load(kb, a.k_st, last);
   sv.load(vb, a.v_st, last);
-  sk.store(lds, a.D);
-  sv.store(lds + IMG, a.D);
+  sk.store(lds);
+  sv.store(lds + IMG);
   __syncthreads();
   for (int t = 0; t < steps; ++t) {
     const char* ki = lds + (t & 1) * 2 * IMG;
@@ -633,8 +597,8 @@ void packed_dq_kernel(const PackedArgs a) {
       }
     }
     char* next = lds + ((t + 1) & 1) * 2 * IMG;
-    sk.store(next, a.D);
-    sv.store(next + IMG, a.D);
+    sk.store(next);
+    sv.store(next + IMG);
     __syncthreads();
   }
   store_col<DT>(a.dq + (tok * a.H + h) * a.D, dq, a.scale, hi, a.D,
@@ -663,7 +627,7 @@ void packed_dq_kernel(const PackedArgs a) {
 #define BQT 32                 // queries of a step
 #define BKW 8                  // waves: 4 of each kind
 
-template <int DP, bool ODD>
+template <int DP>
 __global__ __launch_bounds__(64 * BKW, 2)
 void packed_dkdv_kernel(const PackedArgs a) {
   constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * BKW;
@@ -706,7 +670,7 @@ void packed_dkdv_kernel(const PackedArgs a) {
                               : a.v + tok * a.v_st + hk * a.v_sh;
     #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
-      kvf[ks] = __builtin_bit_cast(bf16x8, load_piece(r, 2 * ks + hi, a.D));
+      kvf[ks] = __builtin_bit_cast(bf16x8, load_piece(r, 2 * ks + hi, a.W));
   }
   f32x16 acc[DT];                              // dV^T or dK^T
   #pragma unroll
@@ -715,7 +679,7 @@ void packed_dkdv_kernel(const PackedArgs a) {
 
   const int per = (w.len - kv0 + BQT - 1) / BQT;   // steps of one head
   const int steps = per * heads;
-  Stage<DP, BQT, NT, ODD> sq, sg;
+  Stage<DP, BQT, NT> sq, sg;
   float slab = 0.f;
   // the tile to load: its first query and where its rows lie
   int lq = kv0;
@@ -743,13 +707,13 @@ void packed_dkdv_kernel(const PackedArgs a) {
     sp += wrap ? a.T : 0;
   };
   auto store = [&](char* buf) {
-    sq.store(buf, a.D);
-    sg.store(buf + IMG, a.D);
+    sq.store(buf);
+    sg.store(buf + IMG);
     if (threadIdx.x < 2 * BQT)
       reinterpret_cast<float*>(buf + 2 * IMG)[threadIdx.x] = slab;
   };
-  sq.init(a.q_st, a.D);
-  sg.init(a.go_st, a.D);
+  sq.init(a.q_st, a.W);
+  sg.init(a.go_st, a.W);
   load();
   store(lds);
   __syncthreads();
@@ -876,24 +840,24 @@ static int64_t max_blocks(const PackedArgs& a, int rows) {
   return a.T / rows + a.B + 1;
 }
 
-template <int DP, bool ODD>
+template <int DP>
 static hipError_t run_fwd(const PackedArgs& a, hipStream_t stream) {
   const int64_t n = max_blocks(a, FQ) * a.H;
   if (n > 0x7fffffff) return hipErrorInvalidValue;
-  packed_fwd_kernel<DP, ODD><<<dim3((uint32_t)n), dim3(64 * FW), 0, stream>>>(a);
+  packed_fwd_kernel<DP><<<dim3((uint32_t)n), dim3(64 * FW), 0, stream>>>(a);
   HIP_CHECK_LAST();
   return hipSuccess;
 }
 
-template <int DP, bool ODD>
+template <int DP>
 static hipError_t run_bwd(const PackedArgs& a, hipStream_t stream) {
   const int64_t n = max_blocks(a, BQ) * a.H;
   if (n > 0x7fffffff) return hipErrorInvalidValue;
-  packed_dq_kernel<DP, ODD><<<dim3((uint32_t)n), dim3(64 * BW), 0, stream>>>(a);
+  packed_dq_kernel<DP><<<dim3((uint32_t)n), dim3(64 * BW), 0, stream>>>(a);
   HIP_CHECK_LAST();
   const int64_t m = max_blocks(a, BKV) * a.HKV * a.splits;
   if (m > 0x7fffffff) return hipErrorInvalidValue;
-  packed_dkdv_kernel<DP, ODD><<<dim3((uint32_t)m), dim3(64 * BKW), 0,
+  packed_dkdv_kernel<DP><<<dim3((uint32_t)m), dim3(64 * BKW), 0,
                                 stream>>>(a);
   HIP_CHECK_LAST();
   if (a.splits > 1) {
@@ -906,51 +870,97 @@ static hipError_t run_bwd(const PackedArgs& a, hipStream_t stream) {
 }
 
 static void fill(PackedArgs& a, const int64_t* st, const int* cu, int T, int B,
-                 int H, int HKV, int D, float scale) {
+                 int H, int HKV, int W, int D, float scale) {
   a.q_st = st[0]; a.q_sh = st[1]; a.k_st = st[2]; a.k_sh = st[3];
   a.v_st = st[4]; a.v_sh = st[5]; a.go_st = st[6]; a.go_sh = st[7];
-  a.cu = cu; a.T = T; a.B = B; a.H = H; a.HKV = HKV; a.D = D; a.scale = scale;
+  a.cu = cu; a.T = T; a.B = B; a.H = H; a.HKV = HKV; a.W = W; a.D = D;
+  a.scale = scale;
 }
 
-#define DISPATCH_DP(D, FN)                                                   \
-  if ((D) < 8) return hipErrorInvalidValue;                                  \
-  if ((D) & 7) {                                                             \
-    if ((D) <= 64) return FN<64, true>(a, stream);                           \
-    if ((D) <= 96) return FN<96, true>(a, stream);                           \
-    if ((D) <= 128) return FN<128, true>(a, stream);                         \
-    if ((D) <= 160) return FN<160, true>(a, stream);                         \
-    if ((D) <= 192) return FN<192, true>(a, stream);                         \
-    return hipErrorInvalidValue;                                             \
-  }                                                                          \
-  if ((D) <= 64) return FN<64, false>(a, stream);                            \
-  if ((D) <= 96) return FN<96, false>(a, stream);                            \
-  if ((D) <= 128) return FN<128, false>(a, stream);                          \
-  if ((D) <= 160) return FN<160, false>(a, stream);                          \
-  if ((D) <= 192) return FN<192, false>(a, stream);                          \
+#define DISPATCH_DP(W, FN)                                                   \
+  if ((W) <= 64) return FN<64>(a, stream);                                   \
+  if ((W) <= 96) return FN<96>(a, stream);                                   \
+  if ((W) <= 128) return FN<128>(a, stream);                                 \
+  if ((W) <= 160) return FN<160>(a, stream);                                 \
+  if ((W) <= 192) return FN<192>(a, stream);                                 \
   return hipErrorInvalidValue;
 
 extern "C" hipError_t lumina_packed_attn_fwd(
     const void* q, const void* k, const void* v, void* out, float* lse,
-    const int* cu, const int64_t* strides, int T, int B, int H, int HKV, int D,
-    float scale, hipStream_t stream) {
+    const int* cu, const int64_t* strides, int T, int B, int H, int HKV, int W,
+    int D, float scale, hipStream_t stream) {
   PackedArgs a = {};
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
   a.out = (uint16_t*)out; a.lse = lse;
-  fill(a, strides, cu, T, B, H, HKV, D, scale);
-  DISPATCH_DP(D, run_fwd)
+  fill(a, strides, cu, T, B, H, HKV, W, D, scale);
+  DISPATCH_DP(W, run_fwd)
 }
 
 extern "C" hipError_t lumina_packed_attn_bwd(
     const void* q, const void* k, const void* v, const void* o, const void* go,
     const float* lse, float* delta, void* dq, void* dk, void* dv, float* part,
     int splits, const int* cu, const int64_t* strides, int T, int B, int H,
-    int HKV, int D, float scale, hipStream_t stream) {
+    int HKV, int W, int D, float scale, hipStream_t stream) {
   PackedArgs a = {};
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
   a.o = (const uint16_t*)o; a.go = (const uint16_t*)go;
   a.lse = const_cast<float*>(lse); a.delta = delta;
   a.part = part; a.splits = splits;
   a.dq = (uint16_t*)dq; a.dk = (uint16_t*)dk; a.dv = (uint16_t*)dv;
-  fill(a, strides, cu, T, B, H, HKV, D, scale);
-  DISPATCH_DP(D, run_bwd)
+  fill(a, strides, cu, T, B, H, HKV, W, D, scale);
+  DISPATCH_DP(W, run_bwd)
+}
+
+// ===========================================================================
+// Rows of D channels anywhere -> rows of W, zero past D, for up to three tensors
+// [T, heads, .] at once; a thread moves 8 channels. Rows that start between 16
+// bytes cost the kernels above more than this copy: at D = 159 they took 563 us
+// together for 8192 tokens of 12:4 heads, and 430 at D = 160, while q, k, v and
+// dO are copied in 40.
+// ===========================================================================
+struct PackRowsArgs {
+  const uint16_t* src[3];
+  uint16_t* dst[3];
+  int64_t st[3], sh[3];        // strides of tokens and heads
+  int64_t total[3];            // threads
+  int heads[3];
+  int D, pieces;
+};
+
+__global__ __launch_bounds__(256)
+void pack_rows_kernel(const PackRowsArgs a) {
+  const int w = blockIdx.y;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.total[w]) return;
+  const int64_t row = i / a.pieces;
+  const int c = (int)(i - row * a.pieces);
+  const int64_t t = row / a.heads[w];
+  const int h = (int)(row - t * a.heads[w]);
+  const uint16_t* src = a.src[w] + t * a.st[w] + h * a.sh[w];
+  *reinterpret_cast<uintx4*>(a.dst[w] + 8 * i) = load_ragged(src, c, a.D);
+}
+
+extern "C" hipError_t lumina_pack_rows(const void* const* src, void* const* dst,
+                                       const int64_t* strides,
+                                       const int* heads, int n, int64_t T,
+                                       int D, hipStream_t stream) {
+  PackRowsArgs a = {};
+  if (n < 1 || n > 3) return hipErrorInvalidValue;
+  a.D = D;
+  a.pieces = (D + 7) / 8;
+  int64_t most = 0;
+  for (int i = 0; i < n; ++i) {
+    a.src[i] = (const uint16_t*)src[i];
+    a.dst[i] = (uint16_t*)dst[i];
+    a.st[i] = strides[2 * i];
+    a.sh[i] = strides[2 * i + 1];
+    a.heads[i] = heads[i];
+    a.total[i] = T * heads[i] * a.pieces;
+    most = a.total[i] > most ? a.total[i] : most;
+  }
+  const int64_t blocks = (most + 255) / 256;
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  pack_rows_kernel<<<dim3((uint32_t)blocks, n), dim3(256), 0, stream>>>(a);
+  HIP_CHECK_LAST();
+  return hipSuccess;
 }
