@@ -32,6 +32,39 @@ DEV_INLINE uint16_t f32_to_bf16(float f) {
   return (uint16_t)(v.i >> 16);
 }
 
+// ---- rows of 16-bit channels at any address -------------------------------
+// 16 bytes at any element: one load, gfx950 takes any alignment there
+typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t uintx4_any;
+
+// Channels 8 c .. 8 c + 7 of a row of D, zero past its end. Nothing outside the
+// row is read: its last, partial piece is read as its last 8 channels and moved
+// down, without a branch that lanes could take apart (a piece of one in twenty
+// lanes, loaded channel by channel, made a copy of rows of 159 three times as
+// long).
+DEV_INLINE uintx4 load8_ragged(const uint16_t* row, int c, int D) {
+  if (D >= 8) {                               // uniform, and below
+    const int o = 8 * c < D - 8 ? 8 * c : D - 8;
+    uintx4 v = *reinterpret_cast<const uintx4_any*>(row + o);
+    const int e = (8 - (D & 7)) & 7;
+    const bool part = 8 * c > D - 8;
+    if (e & 1) {
+      const uint32_t by = part ? 16 : 0;
+      #pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = __builtin_amdgcn_alignbit(j < 3 ? v[j + 1] : (part ? 0 : v[3]),
+                                         v[j], by);
+    }
+    if (e & 2) v = part ? uintx4{v[1], v[2], v[3], 0} : v;
+    if (e & 4) v = part ? uintx4{v[2], v[3], 0, 0} : v;
+    return 8 * c < D ? v : uintx4{0, 0, 0, 0};
+  }
+  uintx4 v = {0, 0, 0, 0};
+  #pragma unroll
+  for (int j = 0; j < 7; ++j)
+    if (8 * c + j < D) v[j >> 1] |= (uint32_t)row[8 * c + j] << (16 * (j & 1));
+  return v;
+}
+
 // generic element accessors so kernels template over T in {float, bf16-as-u16}
 struct F32Elem {
   using storage = float;

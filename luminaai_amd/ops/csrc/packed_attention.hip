@@ -34,8 +34,6 @@ typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(2))) float floatx2;
 typedef __attribute__((ext_vector_type(2))) uint32_t uintx2;
-// 16 bytes at any element: one load, gfx950 takes any alignment there
-typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t uintx4_any;
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 #define LOG2E 1.4426950408889634f
@@ -172,17 +170,6 @@ DEV_INLINE uintx4 load_piece(const uint16_t* row, int c, int W) {
   if (8 * c >= W) return uintx4{0, 0, 0, 0};
   return *reinterpret_cast<const uintx4*>(row + 8 * c);
 }
-// the same for a row of any alignment and length
-DEV_INLINE uintx4 load_ragged(const uint16_t* row, int c, int D) {
-  const int n = D - 8 * c;
-  if (n >= 8) return *reinterpret_cast<const uintx4_any*>(row + 8 * c);
-  uintx4 v = {0, 0, 0, 0};
-  #pragma unroll
-  for (int j = 0; j < 7; ++j)
-    if (j < n) v[j >> 1] |= (uint32_t)row[8 * c + j] << (16 * (j & 1));
-  return v;
-}
-
 // A tile of ROWS rows on its way from memory to LDS, in the registers of NT
 // threads. Channels past W are not cleared: they meet zeros in the other
 // operand's fragment (load_piece), or columns that are not stored. They repeat
@@ -538,7 +525,7 @@ void packed_dq_kernel(const PackedArgs a) {
       else
         gf[ks] = gk;
       const bf16x8 of = __builtin_bit_cast(
-          bf16x8, load_ragged(orow, 2 * ks + hi, a.D));
+          bf16x8, load8_ragged(orow, 2 * ks + hi, a.D));
       #pragma unroll
       for (int j = 0; j < 8; ++j)
         delta = __builtin_fmaf((float)gk[j], (float)of[j], delta);
@@ -922,22 +909,29 @@ struct PackRowsArgs {
   const uint16_t* src[3];
   uint16_t* dst[3];
   int64_t st[3], sh[3];        // strides of tokens and heads
-  int64_t total[3];            // threads
+  int64_t T;
   int heads[3];
-  int D, pieces;
+  int D, pieces, per;          // per: tokens of a workgroup
 };
 
+// A workgroup's pieces are counted in 32 bits: two 64-bit divisions a piece took
+// longer than its bytes.
 __global__ __launch_bounds__(256)
 void pack_rows_kernel(const PackRowsArgs a) {
   const int w = blockIdx.y;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.total[w]) return;
-  const int64_t row = i / a.pieces;
-  const int c = (int)(i - row * a.pieces);
-  const int64_t t = row / a.heads[w];
-  const int h = (int)(row - t * a.heads[w]);
-  const uint16_t* src = a.src[w] + t * a.st[w] + h * a.sh[w];
-  *reinterpret_cast<uintx4*>(a.dst[w] + 8 * i) = load_ragged(src, c, a.D);
+  const int64_t t0 = (int64_t)blockIdx.x * a.per;
+  const int64_t left = a.T - t0;
+  const uint32_t heads = a.heads[w], pieces = a.pieces;
+  const uint32_t n = (uint32_t)(left < a.per ? left : a.per) * heads * pieces;
+  const uint16_t* src = a.src[w] + t0 * a.st[w];
+  uint16_t* dst = a.dst[w] + t0 * heads * pieces * 8;
+  #pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < n; i += 256) {
+    const uint32_t row = i / pieces, c = i - row * pieces;
+    const uint32_t t = row / heads, h = row - t * heads;
+    *reinterpret_cast<uintx4*>(dst + 8 * (int64_t)i) =
+        load8_ragged(src + t * a.st[w] + h * a.sh[w], c, a.D);
+  }
 }
 
 extern "C" hipError_t lumina_pack_rows(const void* const* src, void* const* dst,
@@ -946,19 +940,19 @@ extern "C" hipError_t lumina_pack_rows(const void* const* src, void* const* dst,
                                        int D, hipStream_t stream) {
   PackRowsArgs a = {};
   if (n < 1 || n > 3) return hipErrorInvalidValue;
+  a.T = T;
   a.D = D;
   a.pieces = (D + 7) / 8;
-  int64_t most = 0;
+  // few tokens: a workgroup each, so that the call has enough of them
+  a.per = T >= 4096 ? 8 : 1;
   for (int i = 0; i < n; ++i) {
     a.src[i] = (const uint16_t*)src[i];
     a.dst[i] = (uint16_t*)dst[i];
     a.st[i] = strides[2 * i];
     a.sh[i] = strides[2 * i + 1];
     a.heads[i] = heads[i];
-    a.total[i] = T * heads[i] * a.pieces;
-    most = a.total[i] > most ? a.total[i] : most;
   }
-  const int64_t blocks = (most + 255) / 256;
+  const int64_t blocks = (T + a.per - 1) / a.per;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   pack_rows_kernel<<<dim3((uint32_t)blocks, n), dim3(256), 0, stream>>>(a);
   HIP_CHECK_LAST();

@@ -13,21 +13,6 @@ typedef __attribute__((ext_vector_type(2))) float  floatx2;
 
 #define LOG2E 1.4426950408889634f
 
-// Eight elements from an address that is only element-aligned; elements at
-// and after n are zero. The full load is one 16-byte global load: gfx950 takes
-// any alignment there.
-DEV_INLINE ushortx8 load8_guarded(const uint16_t* p, int n) {
-  ushortx8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (n >= 8) {
-    __builtin_memcpy(&v, p, 16);
-  } else {
-    #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) v[j] = p[j];
-  }
-  return v;
-}
-
 DEV_INLINE uint32_t pack_bf16(float lo, float hi) {
   floatx2 f = {lo, hi};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
@@ -116,10 +101,9 @@ void paged_attn_kernel(const PagedAttnArgs a) {
     const uint16_t* qp = a.q + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh;
     #pragma unroll
     for (int ks = 0; ks < NDW; ++ks) {
-      const int d0 = 32 * ks + 8 * g;
-      qf[ks] = __builtin_bit_cast(
-          bf16x8, load8_guarded(qp + (d0 < a.D ? d0 : 0),
-                                head_ok ? a.D - d0 : 0));
+      const uintx4 x = load8_ragged(qp, 4 * ks + g, a.D);
+      qf[ks] = __builtin_bit_cast(bf16x8,
+                                  head_ok ? x : uintx4{0u, 0u, 0u, 0u});
     }
   }
   // channels past head_dim in K's last 8 may hold anything: cut them
@@ -386,43 +370,46 @@ struct PagedAppendArgs {
   int64_t s_t[2], s_h[2];      // source strides in elements
   int64_t d_p[2], d_h[2], d_t[2];
   int64_t table_sb;
-  int64_t P, total;            // total: threads of one of the two tensors
-  int B, HKV, D, chunks, page_shift, M;
+  int64_t P, T;
+  int B, HKV, D, chunks, page_shift, M, per;   // per: tokens of a workgroup
 };
 
-template <typename T>
+template <typename E>
 __global__ __launch_bounds__(256)
 void paged_append_kernel(const PagedAppendArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.total) return;
   const int which = blockIdx.y;
-  const int64_t row = i / a.chunks;
-  const int c = (int)(i - row * a.chunks);
-  const int64_t t = row / a.HKV;
-  const int h = (int)(row - t * a.HKV);
-  const int seq = a.ids ? a.ids[t] : (int)t;
-  const int pos = a.pos[t];
-  // tokens without a place (negative position, past the table, a page number
-  // outside the pool) are not written
-  if (seq < 0 || seq >= a.B || pos < 0) return;
-  const int pi = pos >> a.page_shift;
-  if (pi >= a.M) return;
-  const int pg = a.table[seq * a.table_sb + pi];
-  if (pg < 0 || pg >= a.P) return;
-  const T* src = reinterpret_cast<const T*>(a.src[which]) + t * a.s_t[which]
-                 + h * a.s_h[which] + 8 * c;
-  T* dst = reinterpret_cast<T*>(a.dst[which]) + pg * a.d_p[which]
-           + h * a.d_h[which]
-           + (pos & ((1 << a.page_shift) - 1)) * a.d_t[which] + 8 * c;
-  T v[8];
-  const int n = a.D - 8 * c;
-  if (n >= 8) {
-    __builtin_memcpy(v, src, sizeof(v));
-  } else {
-    #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? src[j] : (T)0;
+  const int64_t t0 = (int64_t)blockIdx.x * a.per;
+  const int64_t left = a.T - t0;
+  // 32 bits count a workgroup's pieces: 64-bit divisions cost more than the bytes
+  const uint32_t heads = a.HKV, chunks = a.chunks;
+  const uint32_t n = (uint32_t)(left < a.per ? left : a.per) * heads * chunks;
+  #pragma unroll 2
+  for (uint32_t i = threadIdx.x; i < n; i += 256) {
+    const uint32_t row = i / chunks, c = i - row * chunks;
+    const uint32_t tr = row / heads, h = row - tr * heads;
+    const int64_t t = t0 + tr;
+    const int seq = a.ids ? a.ids[t] : (int)t;
+    const int pos = a.pos[t];
+    // tokens without a place (negative position, past the table, a page number
+    // outside the pool) are not written
+    if (seq < 0 || seq >= a.B || pos < 0) continue;
+    const int pi = pos >> a.page_shift;
+    if (pi >= a.M) continue;
+    const int pg = a.table[seq * a.table_sb + pi];
+    if (pg < 0 || pg >= a.P) continue;
+    const E* src = reinterpret_cast<const E*>(a.src[which]) + t * a.s_t[which]
+                   + h * a.s_h[which];
+    E* dst = reinterpret_cast<E*>(a.dst[which]) + pg * a.d_p[which]
+             + h * a.d_h[which]
+             + (pos & ((1 << a.page_shift) - 1)) * a.d_t[which] + 8 * c;
+    if constexpr (sizeof(E) == 2) {
+      *reinterpret_cast<uintx4*>(dst) = load8_ragged(src, c, a.D);
+    } else {
+      #pragma unroll
+      for (int j = 0; j < 8; ++j)
+        dst[j] = 8 * (int)c + j < a.D ? src[8 * c + j] : (E)0;
+    }
   }
-  __builtin_memcpy(__builtin_assume_aligned(dst, 16), v, sizeof(v));
 }
 
 extern "C" hipError_t lumina_paged_append(
@@ -442,8 +429,10 @@ extern "C" hipError_t lumina_paged_append(
   a.table_sb = strides[10];
   a.P = P; a.B = B; a.HKV = HKV; a.D = D; a.chunks = W / 8;
   a.page_shift = page_shift; a.M = M;
-  a.total = T * HKV * a.chunks;
-  const int64_t blocks = (a.total + 255) / 256;
+  a.T = T;
+  // few tokens: a workgroup each, so that the call has enough of them
+  a.per = T >= 4096 ? 8 : 1;
+  const int64_t blocks = (T + a.per - 1) / a.per;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   const dim3 grid((uint32_t)blocks, 2), block(256);
   if (elem_size == 2)
