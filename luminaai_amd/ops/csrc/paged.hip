@@ -277,10 +277,14 @@ void paged_attn_kernel(const PagedAttnArgs a) {
   }
 }
 
-// Joins the chunks of one (sequence, head), always in the same order.
+// Joins the chunks of one (sequence, head), always in the same order: wave w
+// takes chunks w, w + 4, .., four at a time, so that their loads are under way
+// together; what a small call waits for here is one trip to memory, not one for
+// the maxima and one for the rest.
 __global__ __launch_bounds__(256)
 void paged_attn_join_kernel(const PagedAttnArgs a) {
-  __shared__ float so[4][192], sl[4];
+  __shared__ float so[4][192], sm[4], sl[4];
+  constexpr int U = 4;
   const int64_t bh = blockIdx.x;
   const int b = (int)(bh / a.H);
   const int len = clampi(a.lens[b], 0, a.M << a.page_shift);
@@ -289,28 +293,59 @@ void paged_attn_join_kernel(const PagedAttnArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float* ml = a.ml + bh * a.S * 2;
   const float* part = a.part + bh * a.S * a.D;
-  float m = -1e30f;
-  for (int s = lane; s < n; s += 64) m = fmaxf(m, ml[2 * s]);
-  #pragma unroll
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  float l = 0.f, acc[3] = {0.f, 0.f, 0.f};
-  for (int s = wave; s < n; s += 4) {
-    const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m);
-    l += f * ml[2 * s + 1];
+  float m = -1e30f, l = 0.f, acc[3] = {0.f, 0.f, 0.f};
+  for (int s0 = wave; s0 < n; s0 += 4 * U) {
+    float cm[U], cl[U], x[U][3];
     #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const int d = lane + 64 * i;
-      if (d < a.D) acc[i] += f * part[(int64_t)s * a.D + d];
+    for (int u = 0; u < U; ++u) {
+      // past the end the last one again, with weight 0
+      const bool ok = s0 + 4 * u < n;
+      const int s = ok ? s0 + 4 * u : n - 1;
+      cm[u] = ml[2 * s];
+      cl[u] = ml[2 * s + 1];
+      #pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const int d = lane + 64 * i;
+        x[u][i] = d < a.D ? part[(int64_t)s * a.D + d] : 0.f;
+      }
+      if (!ok) cm[u] = -INFINITY;
+    }
+    float mn = m;
+    #pragma unroll
+    for (int u = 0; u < U; ++u) mn = fmaxf(mn, cm[u]);
+    const float f = __builtin_amdgcn_exp2f(m - mn);
+    l *= f;
+    #pragma unroll
+    for (int i = 0; i < 3; ++i) acc[i] *= f;
+    m = mn;
+    #pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float g = __builtin_amdgcn_exp2f(cm[u] - mn);
+      l += g * cl[u];
+      #pragma unroll
+      for (int i = 0; i < 3; ++i) acc[i] += g * x[u][i];
     }
   }
   #pragma unroll
   for (int i = 0; i < 3; ++i)
     if (lane + 64 * i < a.D) so[wave][lane + 64 * i] = acc[i];
-  if (lane == 0) sl[wave] = l;
+  if (lane == 0) {
+    sm[wave] = m;
+    sl[wave] = l;
+  }
   __syncthreads();
-  const float ls = ((sl[0] + sl[1]) + sl[2]) + sl[3];
-  for (int d = threadIdx.x; d < a.D; d += 256) {
-    const float os = ((so[0][d] + so[1][d]) + so[2][d]) + so[3][d];
+  const float mm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  float g[4], ls = 0.f;
+  #pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    g[w] = __builtin_amdgcn_exp2f(sm[w] - mm);
+    ls += g[w] * sl[w];
+  }
+  const int d = threadIdx.x;
+  if (d < a.D) {
+    float os = 0.f;
+    #pragma unroll
+    for (int w = 0; w < 4; ++w) os += g[w] * so[w][d];
     a.o[bh * a.D + d] = f32_to_bf16(ls == 0.f ? 0.f : os / ls);
   }
 }
