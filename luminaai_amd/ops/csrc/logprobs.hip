@@ -11,9 +11,9 @@
 // logits, with the exponentials close behind.
 //
 // Alternatives: the k-th largest of 64 group maxima is a lower bound of
-// the k-th largest logit, so only threads whose own maximum reaches it look at
-// their elements again (from L2) and put the candidates into LDS, where each is
-// ranked by counting. Ties go to the lowest index: value and index make one
+// the k-th largest logit, so only the elements of threads whose own maximum
+// reaches it are looked at again (from L2); the candidates go to LDS, where each
+// is ranked by counting. Ties go to the lowest index: value and index make one
 // 64-bit key. Rows with more candidates than fit (many equal logits) take
 // k rounds of a maximum over the row.
 #include "common.h"
@@ -54,6 +54,13 @@ DEV_INLINE Vec8<S> load8(const S* p) {
   Vec8<S> r;
   __builtin_memcpy(&r, p, sizeof(r));
   return r;
+}
+
+// The maximum, NaN if one of them is: an instruction for two of them
+// (v_maximum3_f32). fmaxf of loaded numbers takes three, since it has to quiet
+// NaNs, and made the forward kernel bound by arithmetic.
+DEV_INLINE float max_nan(float a, float b) {
+  return __builtin_elementwise_maximum(a, b);
 }
 
 // orders floats as unsigned numbers; NaN above all, the two zeros equal
@@ -121,8 +128,8 @@ void logprob_fwd_kernel(const LogprobArgs a) {
   auto take = [&](const float* f, int n) {
     float cm = f[0];
     #pragma unroll
-    for (int j = 1; j < n; ++j) cm = fmaxf(cm, f[j]);
-    if (cm > mx) {
+    for (int j = 1; j < n; ++j) cm = max_nan(cm, f[j]);
+    if (!(cm <= mx)) {
       // the reference is 0 while all is -inf (inf - inf otherwise): s is 0
       if (mx > -INFINITY) {
         const float d = (mx - cm) * LOG2E, sc = __builtin_amdgcn_exp2f(d);
@@ -176,7 +183,7 @@ void logprob_fwd_kernel(const LogprobArgs a) {
   if (lane == 0) {
     red[wave][0] = st.m; red[wave][1] = st.s; red[wave][2] = st.t;
   }
-  if (TOP) gmax[wave][lane] = mx;
+  if (TOP) gmax[wave][lane] = mx == mx ? mx : -INFINITY;   // NaN: not known
   if (threadIdx.x == 0) n_cand = 0;
   __syncthreads();
   RowState r = {red[0][0], red[0][1], red[0][2]};
@@ -206,34 +213,35 @@ void logprob_fwd_kernel(const LogprobArgs a) {
     #pragma unroll
     for (int w = 1; w < NW; ++w) g = fmaxf(g, gmax[w][lane]);
     int rank = 0;
+    #pragma unroll
     for (int j = 0; j < 64; ++j) {
-      const float o = __shfl(g, j, 64);
+      const float o = __builtin_bit_cast(
+          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, g), j));
       rank += (o > g || (o == g && j < lane)) ? 1 : 0;
     }
     if (rank == a.k - 1) thr = g;
   }
   __syncthreads();
   const float T = thr;
-  if (mx >= T || s != s) {
-    for (int q = threadIdx.x; q < nvec; q += BLOCK) {
+  auto offer = [&](float f, int idx) {
+    if (!(f < T)) {
+      const int at = atomicAdd(&n_cand, 1);
+      if (at < LP_CAP) cand[at] = pair_key(f, idx);
+    }
+  };
+  // A thread whose maximum reaches T (or that met a NaN) has its vectors looked
+  // through by its whole wave: one trip to L2 each, not one for every vector.
+  unsigned long long hits = __ballot(mx >= T || s != s);
+  while (hits) {
+    const int owner = wave * 64 + __builtin_ctzll(hits);
+    hits &= hits - 1;
+    for (int q = owner + lane * BLOCK; q < nvec; q += 64 * BLOCK) {
       const Vec8<S> v = load8(x + 8 * (int64_t)q);
       #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float f = E::get(v.v[j]);
-        if (!(f < T)) {
-          const int at = atomicAdd(&n_cand, 1);
-          if (at < LP_CAP) cand[at] = pair_key(f, 8 * q + j);
-        }
-      }
-    }
-    if (tail < a.V) {
-      const float f = E::get(x[tail]);
-      if (!(f < T)) {
-        const int at = atomicAdd(&n_cand, 1);
-        if (at < LP_CAP) cand[at] = pair_key(f, tail);
-      }
+      for (int j = 0; j < 8; ++j) offer(E::get(v.v[j]), 8 * q + j);
     }
   }
+  if (tail < a.V && threadIdx.x < 8) offer(E::get(x[tail]), tail);
   __syncthreads();
   auto put = [&](int rank, uint64_t key) {
     const int idx = (int)~(uint32_t)key;
