@@ -11,7 +11,7 @@
 // logits, with the exponentials close behind.
 //
 // Alternatives: the k-th largest of 64 group maxima is a lower bound of
-// the k-th largest logit, so only the elements of threads whose own maximum
+// the k-th largest logit (a little less will do), so only the elements of threads whose own maximum
 // reaches it are looked at again (from L2); the candidates go to LDS, where each
 // is ranked by counting. Ties go to the lowest index: value and index make one
 // 64-bit key. Rows with more candidates than fit (many equal logits) take
@@ -69,6 +69,9 @@ DEV_INLINE uint32_t order_key(float f) {
   const uint32_t u = __builtin_bit_cast(uint32_t, f + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+DEV_INLINE float from_order_key(uint32_t k) {
+  return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
 DEV_INLINE uint64_t pair_key(float f, int idx) {
   return ((uint64_t)order_key(f) << 32) | (uint32_t)~idx;
 }
@@ -123,6 +126,10 @@ void logprob_fwd_kernel(const LogprobArgs a) {
   const S* x = reinterpret_cast<const S*>(a.x) + row * a.row_stride;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int nvec = a.V >> 3;
+  // asked for now, so that nothing waits for it at the end
+  const int64_t tk = token_of(a.tok, a.tok64, row);
+  const bool inside = tk >= 0 && tk < a.V;
+  const float xt = E::get(x[inside ? tk : 0]);
 
   float mx = -INFINITY, ref = 0.f, s = 0.f, t = 0.f;
   auto take = [&](const float* f, int n) {
@@ -194,11 +201,9 @@ void logprob_fwd_kernel(const LogprobArgs a) {
   if (r.s == 0.f) r.s = __builtin_nanf("");
   const float ls = __builtin_log2f(r.s);
   if (threadIdx.x == 0) {
-    const int64_t tk = token_of(a.tok, a.tok64, row);
     float lp = __builtin_nanf("");         // a token outside the vocabulary
     if (tk == a.ignore) lp = 0.f;
-    else if (tk >= 0 && tk < a.V)
-      lp = E::get(x[tk]) - r.m - LN2 * ls;
+    else if (inside) lp = xt - r.m - LN2 * ls;
     a.lp[row] = lp;
     a.ent[row] = LN2 * (ls - r.t / r.s);
     if (a.stat) {
@@ -212,50 +217,72 @@ void logprob_fwd_kernel(const LogprobArgs a) {
     float g = gmax[0][lane];
     #pragma unroll
     for (int w = 1; w < NW; ++w) g = fmaxf(g, gmax[w][lane]);
-    int rank = 0;
+    // T: the upper half of the order key of the k-th largest maximum, by
+    // bisection over its bits; at least k of them are T or more
+    const uint32_t key = order_key(g);
+    uint32_t lo = 0;
     #pragma unroll
-    for (int j = 0; j < 64; ++j) {
-      const float o = __builtin_bit_cast(
-          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, g), j));
-      rank += (o > g || (o == g && j < lane)) ? 1 : 0;
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t mid = lo | (1u << bit);
+      if (__builtin_popcountll(__ballot(key >= mid)) >= a.k) lo = mid;
     }
-    if (rank == a.k - 1) thr = g;
+    if (lane == 0)                         // keys below -inf's are no numbers
+      thr = lo < 0x007fffffu ? -INFINITY : from_order_key(lo);
   }
   __syncthreads();
   const float T = thr;
-  auto offer = [&](float f, int idx) {
-    if (!(f < T)) {
-      const int at = atomicAdd(&n_cand, 1);
-      if (at < LP_CAP) cand[at] = pair_key(f, idx);
-    }
-  };
-  // A thread whose maximum reaches T (or that met a NaN) has its vectors looked
-  // through by its whole wave: one trip to L2 each, not one for every vector.
+  // Threads whose maximum reaches T (or that met a NaN) have their vectors looked
+  // through by their wave, 16 lanes for each of up to four of them: one trip to
+  // L2, not one for every vector.
   unsigned long long hits = __ballot(mx >= T || s != s);
   while (hits) {
-    const int owner = wave * 64 + __builtin_ctzll(hits);
-    hits &= hits - 1;
-    for (int q = owner + lane * BLOCK; q < nvec; q += 64 * BLOCK) {
+    int owner = -1;
+    #pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (hits && lane >> 4 == u) owner = wave * 64 + __builtin_ctzll(hits);
+      hits &= hits - 1;                      // 0 & -1 stays 0
+    }
+    if (owner < 0) continue;
+    for (int q = owner + (lane & 15) * BLOCK; q < nvec; q += 16 * BLOCK) {
       const Vec8<S> v = load8(x + 8 * (int64_t)q);
+      int n = 0;
       #pragma unroll
-      for (int j = 0; j < 8; ++j) offer(E::get(v.v[j]), 8 * q + j);
+      for (int j = 0; j < 8; ++j) n += E::get(v.v[j]) < T ? 0 : 1;
+      if (n == 0) continue;
+      int at = atomicAdd(&n_cand, n);
+      #pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float f = E::get(v.v[j]);
+        if (!(f < T)) {
+          if (at < LP_CAP) cand[at] = pair_key(f, 8 * q + j);
+          ++at;
+        }
+      }
     }
   }
-  if (tail < a.V && threadIdx.x < 8) offer(E::get(x[tail]), tail);
+  if (tail < a.V && threadIdx.x < 8) {
+    const float f = E::get(x[tail]);
+    if (!(f < T)) {
+      const int at = atomicAdd(&n_cand, 1);
+      if (at < LP_CAP) cand[at] = pair_key(f, tail);
+    }
+  }
   __syncthreads();
   auto put = [&](int rank, uint64_t key) {
-    const int idx = (int)~(uint32_t)key;
-    a.top_id[row * a.k + rank] = idx;
+    a.top_id[row * a.k + rank] = (int)~(uint32_t)key;
     a.top_lp[row * a.k + rank] =
-        E::get(x[idx]) - r.m - LN2 * ls;
+        from_order_key((uint32_t)(key >> 32)) - r.m - LN2 * ls;
   };
   const int n = n_cand;
   if (n <= LP_CAP) {
-    for (int c = threadIdx.x; c < n; c += BLOCK) {
+    // a wave ranks a candidate: 64 comparisons at once
+    for (int c = wave; c < n; c += NW) {
       const uint64_t key = cand[c];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += cand[j] > key ? 1 : 0;
-      if (rank < a.k) put(rank, key);
+      for (int j = lane; j - lane < n; j += 64)
+        rank += __builtin_popcountll(__ballot(j < n && cand[j < n ? j : 0]
+                                              > key));
+      if (lane == 0 && rank < a.k) put(rank, key);
     }
     return;
   }
