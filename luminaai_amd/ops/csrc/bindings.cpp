@@ -75,8 +75,8 @@ hipError_t lumina_moe_dispatch_bwd(const void*, const int64_t*, void*, int64_t, 
 hipError_t lumina_moe_combine_fwd(const void*, const float*, const int64_t*, void*, int64_t, int, int, int64_t, int, hipStream_t);
 hipError_t lumina_moe_combine_bwd_y(const void*, const float*, const int64_t*, const int64_t*, const bool*, void*, int64_t, int64_t, int, int, hipStream_t);
 hipError_t lumina_moe_combine_bwd_w(const void*, const void*, const int64_t*, float*, int64_t, int, int, int64_t, int, hipStream_t);
-hipError_t lumina_packed_attn_fwd(const void*, const void*, const void*, void*, float*, const int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
-hipError_t lumina_packed_attn_bwd(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, float*, int, const int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_packed_attn_fwd(const void*, const void*, const void*, void*, void*, float*, const int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_packed_attn_bwd(const void*, const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, float*, int, const int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_pack_rows(const void* const*, void* const*, const int64_t*, const int*, int, int64_t, int, hipStream_t);
 hipError_t lumina_paged_attn(const void*, const void*, const void*, void*, const int*, const int*, float*, float*, const int64_t*, int64_t, int, int, int, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_paged_append(const void*, const void*, void*, void*, const int*, const int*, const int*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int, int, hipStream_t);
@@ -1042,9 +1042,11 @@ std::vector<at::Tensor> align_rows(std::vector<at::Tensor> ts) {
 }
 }  // namespace
 
-// -> (o, lse2, q, k, v): lse2 is empty where want_lse is false; q, k and v as the
-// kernels read them, which is what packed_attn_bwd takes
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+// -> (o, rest, lse2, q, k, v) for packed_attn_bwd: rest is what rounding o left
+// over, q, k and v are as the kernels read them. rest and lse2 are empty where
+// want_lse is false.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
+           at::Tensor>
 packed_attn_fwd(const at::Tensor& q_, const at::Tensor& k_,
                 const at::Tensor& v_, const at::Tensor& cu, double scale,
                 bool want_lse) {
@@ -1076,24 +1078,26 @@ packed_attn_fwd(const at::Tensor& q_, const at::Tensor& k_,
   const auto &q = in[0], &k = in[1], &v = in[2];
   auto o = at::empty({T, H, D}, q.options());
   auto lse = at::empty({want_lse ? H : 0, T}, q.options().dtype(at::kFloat));
-  if (T == 0) return {o, lse, q, k, v};
+  auto rest = at::empty({want_lse ? T : 0, H, q.size(2)}, q.options());
+  if (T == 0) return {o, rest, lse, q, k, v};
   const int64_t strides[8] = {q.stride(0), q.stride(1), k.stride(0),
                               k.stride(1), v.stride(0), v.stride(1), 0, 0};
   check_hip(lumina_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                    o.data_ptr(),
+                                   want_lse ? rest.data_ptr() : nullptr,
                                    want_lse ? lse.data_ptr<float>() : nullptr,
                                    cu.data_ptr<int>(), strides, (int)T,
                                    (int)cu.size(0) - 1, (int)H, (int)HKV,
                                    (int)q.size(2), (int)D, (float)scale,
                                    cur_stream()),
             "flash_attention_packed");
-  return {o, lse, q, k, v};
+  return {o, rest, lse, q, k, v};
 }
 
 // Takes the gradient of o, and what packed_attn_fwd returned.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
-    const at::Tensor& go_, const at::Tensor& o, const at::Tensor& lse,
-    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    const at::Tensor& go_, const at::Tensor& o, const at::Tensor& rest,
+    const at::Tensor& lse, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const at::Tensor& cu, double scale) {
   TORCH_CHECK_VALUE(go_.sizes() == o.sizes() && go_.device() == o.device(),
                     "the gradient must be of the result's shape and device");
@@ -1122,7 +1126,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
                               k.stride(1), v.stride(0), v.stride(1),
                               go.stride(0), go.stride(1)};
   check_hip(lumina_packed_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                   o.data_ptr(), go.data_ptr(),
+                                   o.data_ptr(), rest.data_ptr(),
+                                   go.data_ptr(),
                                    lse.data_ptr<float>(),
                                    delta.data_ptr<float>(), dq.data_ptr(),
                                    dk.data_ptr(), dv.data_ptr(),

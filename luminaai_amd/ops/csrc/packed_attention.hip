@@ -43,6 +43,7 @@ struct PackedArgs {
   const uint16_t* k;
   const uint16_t* v;
   const uint16_t* o;           // backward: forward's result [T, H, D]
+  uint16_t* rest;              // [T, H, W] what rounding o left over, or null
   const uint16_t* go;          // backward: its gradient
   uint16_t* out;               // forward: [T, H, D]
   uint16_t* dq;                // [T, H, D]
@@ -294,33 +295,47 @@ DEV_INLINE void reads_ahead() {
 
 // A column of a transposed result: this lane's row of memory has channels
 // 8 g + 4 hi + {0..3}, g = 0 .. 4 DT - 1, in this lane and the rest in the lane
-// 32 away. They swap halves, and each stores 8 channels at once.
+// 32 away. They swap halves, and each stores 8 channels at once. `rest`, if not
+// null, takes what the rounding left over.
+DEV_INLINE void store8(uint16_t* row, uint32_t a0, uint32_t a1, uint32_t b0,
+                       uint32_t b1, int d, int D, bool live) {
+  const auto x = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+  const auto y = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+  if (!live) return;
+  const uint32_t u[4] = {x[0], y[0], x[1], y[1]};
+  if (d + 8 <= D) {
+    *reinterpret_cast<uintx4_any*>(row + d) = uintx4{u[0], u[1], u[2], u[3]};
+  } else {
+    #pragma unroll
+    for (int j = 0; j < 7; ++j)
+      if (d + j < D) row[d + j] = (uint16_t)(u[j >> 1] >> (16 * (j & 1)));
+  }
+}
+
+DEV_INLINE uint32_t left_over(float lo, float hi, uint32_t u) {
+  return pack2(lo - __builtin_bit_cast(float, u << 16),
+               hi - __builtin_bit_cast(float, u & 0xffff0000u));
+}
+
 template <int DT>
-DEV_INLINE void store_col(uint16_t* row, const f32x16* acc, float f, int hi,
-                          int D, bool live) {
+DEV_INLINE void store_col(uint16_t* row, uint16_t* rest, const f32x16* acc,
+                          float f, int hi, int D, int W, bool live) {
   #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
     #pragma unroll
     for (int g = 0; g < 4; g += 2) {
+      float x[8];
       uint32_t u[4];
       #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r = 4 * g + 2 * j;
-        const auto x = __builtin_amdgcn_permlane32_swap(
-            pack2(acc[dt][r] * f, acc[dt][r + 1] * f),
-            pack2(acc[dt][r + 4] * f, acc[dt][r + 5] * f), false, false);
-        u[j] = x[0];
-        u[2 + j] = x[1];
-      }
+      for (int j = 0; j < 8; ++j) x[j] = acc[dt][4 * g + j] * f;
+      #pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = pack2(x[2 * j], x[2 * j + 1]);
       const int d = 32 * dt + 8 * g + 8 * hi;
-      if (!live) continue;
-      if (d + 8 <= D) {
-        *reinterpret_cast<uintx4_any*>(row + d) = uintx4{u[0], u[1], u[2], u[3]};
-      } else {
-        #pragma unroll
-        for (int j = 0; j < 7; ++j)
-          if (d + j < D) row[d + j] = (uint16_t)(u[j >> 1] >> (16 * (j & 1)));
-      }
+      store8(row, u[0], u[1], u[2], u[3], d, D, live);
+      if (rest)
+        store8(rest, left_over(x[0], x[1], u[0]), left_over(x[2], x[3], u[1]),
+               left_over(x[4], x[5], u[2]), left_over(x[6], x[7], u[3]), d, W,
+               live);
     }
 }
 
@@ -461,8 +476,9 @@ void packed_fwd_kernel(const PackedArgs a) {
   }
   l += __shfl_xor(l, 32, 64);
   const int64_t tok = w.start + qi;
-  store_col<DT>(a.out + (tok * a.H + h) * a.D, o, l == 0.f ? 0.f : 1.f / l, hi,
-                a.D, qi < w.len);
+  const int64_t at = tok * a.H + h;
+  store_col<DT>(a.out + at * a.D, a.rest ? a.rest + at * a.W : nullptr, o,
+                l == 0.f ? 0.f : 1.f / l, hi, a.D, a.W, qi < w.len);
   if (a.lse && hi == 0 && qi < w.len)
     a.lse[(int64_t)h * a.T + tok] =
         l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
@@ -513,7 +529,10 @@ void packed_dq_kernel(const PackedArgs a) {
   {
     const uint16_t* qr = a.q + tok * a.q_st + h * a.q_sh;
     const uint16_t* gr = a.go + tok * a.go_st + h * a.go_sh;
+    // delta from o with what its rounding left over: the rounding alone would
+    // add a third to the error of dQ and dK (2.5e-3 for 2.4e-3 in all)
     const uint16_t* orow = a.o + (tok * a.H + h) * a.D;
+    const uint16_t* rrow = a.rest + (tok * a.H + h) * a.W;
     #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qf[ks] = __builtin_bit_cast(bf16x8, load_piece(qr, 2 * ks + hi, a.W));
@@ -526,9 +545,12 @@ void packed_dq_kernel(const PackedArgs a) {
         gf[ks] = gk;
       const bf16x8 of = __builtin_bit_cast(
           bf16x8, load8_ragged(orow, 2 * ks + hi, a.D));
+      const bf16x8 rf = __builtin_bit_cast(
+          bf16x8, load_piece(rrow, 2 * ks + hi, a.W));
       #pragma unroll
       for (int j = 0; j < 8; ++j)
-        delta = __builtin_fmaf((float)gk[j], (float)of[j], delta);
+        delta = __builtin_fmaf((float)gk[j], (float)of[j] + (float)rf[j],
+                               delta);
     }
     delta += __shfl_xor(delta, 32, 64);
   }
@@ -588,8 +610,8 @@ void packed_dq_kernel(const PackedArgs a) {
     sv.store(next + IMG);
     __syncthreads();
   }
-  store_col<DT>(a.dq + (tok * a.H + h) * a.D, dq, a.scale, hi, a.D,
-                qi < w.len);
+  store_col<DT>(a.dq + (tok * a.H + h) * a.D, nullptr, dq, a.scale, hi, a.D,
+                0, qi < w.len);
 }
 
 // ===========================================================================
@@ -772,8 +794,8 @@ void packed_dkdv_kernel(const PackedArgs a) {
   }
   const float f = first ? 1.f : a.scale;
   if (a.splits == 1) {
-    store_col<DT>((first ? a.dv : a.dk) + (tok * a.HKV + hk) * a.D, acc, f, hi,
-                  a.D, ki < w.len);
+    store_col<DT>((first ? a.dv : a.dk) + (tok * a.HKV + hk) * a.D, nullptr,
+                  acc, f, hi, a.D, 0, ki < w.len);
   } else if (ki < w.len) {
     const int pw = (a.D + 3) & ~3;
     float* row = a.part + ((((int64_t)(first ? 1 : 0) * a.splits + split) * a.T
@@ -873,24 +895,25 @@ static void fill(PackedArgs& a, const int64_t* st, const int* cu, int T, int B,
   return hipErrorInvalidValue;
 
 extern "C" hipError_t lumina_packed_attn_fwd(
-    const void* q, const void* k, const void* v, void* out, float* lse,
-    const int* cu, const int64_t* strides, int T, int B, int H, int HKV, int W,
+    const void* q, const void* k, const void* v, void* out, void* rest,
+    float* lse, const int* cu, const int64_t* strides, int T, int B, int H, int HKV, int W,
     int D, float scale, hipStream_t stream) {
   PackedArgs a = {};
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
-  a.out = (uint16_t*)out; a.lse = lse;
+  a.out = (uint16_t*)out; a.rest = (uint16_t*)rest; a.lse = lse;
   fill(a, strides, cu, T, B, H, HKV, W, D, scale);
   DISPATCH_DP(W, run_fwd)
 }
 
 extern "C" hipError_t lumina_packed_attn_bwd(
-    const void* q, const void* k, const void* v, const void* o, const void* go,
-    const float* lse, float* delta, void* dq, void* dk, void* dv, float* part,
+    const void* q, const void* k, const void* v, const void* o,
+    const void* rest, const void* go, const float* lse, float* delta, void* dq, void* dk, void* dv, float* part,
     int splits, const int* cu, const int64_t* strides, int T, int B, int H,
     int HKV, int W, int D, float scale, hipStream_t stream) {
   PackedArgs a = {};
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
   a.o = (const uint16_t*)o; a.go = (const uint16_t*)go;
+  a.rest = (uint16_t*)const_cast<void*>(rest);
   a.lse = const_cast<float*>(lse); a.delta = delta;
   a.part = part; a.splits = splits;
   a.dq = (uint16_t*)dq; a.dk = (uint16_t*)dk; a.dv = (uint16_t*)dv;

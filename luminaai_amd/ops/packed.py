@@ -21,18 +21,18 @@ class _PackedAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, scale):
         # rows that start between 16 bytes were copied: the copies are kept
-        o, lse, q, k, v = get_ext().packed_attn_fwd(q, k, v, cu_seqlens, scale,
-                                                    True)
-        ctx.save_for_backward(q, k, v, o, lse, cu_seqlens)
+        o, rest, lse, q, k, v = get_ext().packed_attn_fwd(
+            q, k, v, cu_seqlens, scale, True)
+        ctx.save_for_backward(q, k, v, o, rest, lse, cu_seqlens)
         ctx.scale = scale
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, go):
-        q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
-        dq, dk, dv = get_ext().packed_attn_bwd(go, o, lse, q, k, v, cu_seqlens,
-                                               ctx.scale)
+        q, k, v, o, rest, lse, cu_seqlens = ctx.saved_tensors
+        dq, dk, dv = get_ext().packed_attn_bwd(go, o, rest, lse, q, k, v,
+                                               cu_seqlens, ctx.scale)
         return dq, dk, dv, None, None
 
 
