@@ -69,6 +69,9 @@ class Config:
     streaming_threshold_gb: float = 10.0
     prefetch_factor: int = 4
     pin_memory: bool = True
+    # a micro-batch is one row of sequences without padding (attention inside
+    # each of them); dense and MoE models, not with MoD, SP or pipelines
+    pack_sequences: bool = False
 
     # Generation parameters
     max_new_tokens: int = 512

@@ -7,11 +7,12 @@ from .dataset import (
     StreamingBaseTrainingDataset,
     SyntheticDataset,
     create_dataloader,
+    pack_collate,
     setup_datasets,
 )
 
 __all__ = [
     "BaseTrainingDataset", "ConversationDataset", "ConversationTokenizer",
     "HybridDatasetManager", "InterleavedDataset", "StreamingBaseTrainingDataset",
-    "SyntheticDataset", "create_dataloader", "setup_datasets",
+    "SyntheticDataset", "create_dataloader", "pack_collate", "setup_datasets",
 ]

@@ -222,6 +222,24 @@ class HybridDatasetManager:
 
 
 # ----------------------------------------------------------------------
+def pack_collate(samples: List[Dict[str, torch.Tensor]]
+                 ) -> Dict[str, torch.Tensor]:
+    """One row of sequences instead of a padded batch: input_ids, labels and
+    loss_weights [1, T] and their borders cu_seqlens (int32 [n + 1]), as
+    DeepSeekTransformer.forward takes them. A sample's end without labels (its
+    padding) is cut off: nothing later attends to it and it has no loss."""
+    parts, cu = {}, [0]
+    for s in samples:
+        valid = (s["labels"] != -100).nonzero()
+        n = int(valid[-1]) + 1 if len(valid) else 1
+        for k, v in s.items():
+            parts.setdefault(k, []).append(v[:n])
+        cu.append(cu[-1] + n)
+    out = {k: torch.cat(v)[None] for k, v in parts.items()}
+    out["cu_seqlens"] = torch.tensor(cu, dtype=torch.int32)
+    return out
+
+
 def create_dataloader(dataset: Dataset, config, shuffle: bool = True) -> DataLoader:
     """Tuned DataLoader (reference create_fast_dataloader, dataset.py:807-845).
 
@@ -237,6 +255,8 @@ def create_dataloader(dataset: Dataset, config, shuffle: bool = True) -> DataLoa
         pin_memory=config.pin_memory and torch.cuda.is_available(),
         drop_last=True,
     )
+    if getattr(config, "pack_sequences", False):
+        kwargs["collate_fn"] = pack_collate
     if not is_iterable and dist.is_available() and dist.is_initialized() \
             and dist.get_world_size() > 1:
         from ..parallel.mesh import get_mesh

@@ -34,6 +34,9 @@ class GenerationConfig:
     rep_window: int = 50
     stop_token_ids: List[int] = field(default_factory=list)
     max_context: int = 2048
+    # log probabilities of the answer's tokens with so many alternatives
+    # (paged serving); None: none
+    logprobs: Optional[int] = None
 
     @classmethod
     def from_mode(cls, mode: str, **overrides) -> "GenerationConfig":
@@ -390,6 +393,45 @@ class GenerationEngine:
         self.stats["tokens_generated"] += sum(len(o) for o in outs)
         self.stats["time_in_generate"] += time.perf_counter() - t0
         return outs
+
+    @torch.no_grad()
+    def score(self, sequences: List[List[int]], top_k: int = 0) -> List[Dict]:
+        """Log probability of every token of each sequence after its first, the
+        entropy of the distribution that it was drawn from, and the top_k
+        alternatives there (ops.token_logprobs). The sequences go through the
+        model packed, in one row without padding; one by one where the model
+        does not take them so (mixture-of-depths layers; on the GPU, other
+        types than bf16)."""
+        from .. import ops
+        self.model.eval()
+        p = next(self.model.parameters())
+        packed = not any(l.use_mod for l in self.model.layers) and \
+            (self.device.type != "cuda" or p.dtype == torch.bfloat16)
+        out: List[Dict] = []
+        for group in ([sequences] if packed else [[s] for s in sequences]):
+            flat = [t for s in group for t in s]
+            if not flat:
+                out += [{"logprobs": [], "entropy": [], "top_ids": [],
+                         "top_logprobs": []} for _ in group]
+                continue
+            target: List[int] = []
+            cu = [0]
+            for s in group:
+                target += list(s[1:]) + [-100] * bool(s)
+                cu.append(cu[-1] + len(s))
+            x = torch.tensor([flat], dtype=torch.long, device=self.device)
+            kw = {"cu_seqlens": torch.tensor(cu, dtype=torch.int32,
+                                             device=self.device)} \
+                if packed else {}
+            logits, _, _ = self.model(x, **kw)
+            r = ops.token_logprobs(
+                logits[0], torch.tensor(target, device=self.device), top_k)
+            lp, ent, top, ids = (t.tolist() for t in r)
+            for a, b in zip(cu, cu[1:]):
+                e = max(a, b - 1)
+                out.append({"logprobs": lp[a:e], "entropy": ent[a:e],
+                            "top_ids": ids[a:e], "top_logprobs": top[a:e]})
+        return out
 
     def generate_text(self, prompt: str, config: Optional[GenerationConfig] = None,
                       stream: bool = False) -> str:

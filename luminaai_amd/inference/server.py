@@ -41,6 +41,10 @@ def _gen_config(body: Dict) -> GenerationConfig:
         cfg.repetition_penalty = float(body["repetition_penalty"])
     if "stop_token_ids" in body:
         cfg.stop_token_ids = list(body["stop_token_ids"])
+    if body.get("logprobs") is not None and body["logprobs"] is not False:
+        # completions: a number; chat: true with top_logprobs beside it
+        cfg.logprobs = int(body.get("top_logprobs", 0)
+                           if body["logprobs"] is True else body["logprobs"])
     return cfg
 
 
@@ -104,30 +108,48 @@ class _DynamicBatcher:
 class _ContinuousWorker:
     """Serving loop over ContinuousBatchingEngine: requests (streaming or
     not) join the running decode batch at token granularity; a lone
-    request pays batch-1 compute (active-row compaction)."""
+    request pays batch-1 compute (active-row compaction). paged: over
+    PagedBatchingEngine instead, where a request may ask for several answers
+    (forks of its prompt) and for log probabilities."""
 
     def __init__(self, model, tokenizer, max_batch: int = 8,
-                 max_len: int = 2048):
+                 max_len: int = 2048, paged: bool = False):
         from .continuous import ContinuousBatchingEngine
-        self.eng = ContinuousBatchingEngine(model, tokenizer,
-                                            max_batch=max_batch,
-                                            max_len=max_len)
+        from .paged import PagedBatchingEngine
+        self.paged = paged
+        self.eng = (PagedBatchingEngine if paged else
+                    ContinuousBatchingEngine)(model, tokenizer,
+                                              max_batch=max_batch,
+                                              max_len=max_len)
         self.q: "queue.Queue" = queue.Queue()
         self._thread = threading.Thread(target=self._loop, daemon=True)
         self._thread.start()
 
     def submit(self, prompt_ids: List[int], cfg: GenerationConfig,
                cb=None) -> List[int]:
+        return self.submit_n(prompt_ids, cfg, 1, cb)[0][0]
+
+    def submit_n(self, prompt_ids: List[int], cfg: GenerationConfig,
+                 n: int = 1, cb=None) -> List:
+        """n answers: (tokens, log probabilities or None) of each."""
         evt = threading.Event()
-        item = {"ids": prompt_ids, "cfg": cfg, "cb": cb, "evt": evt}
+        item = {"ids": prompt_ids, "cfg": cfg, "cb": cb, "evt": evt, "n": n,
+                "out": [None] * n}
         self.q.put(item)
         evt.wait()
         if "err" in item:
             raise item["err"]
         return item["out"]
 
+    def _admit(self, item: Dict, tracked: Dict):
+        b = self.eng.admit(item["ids"], item["cfg"], item.get("cb"))
+        tracked[b] = (item, 0)
+        for i in range(1, item["n"]):
+            tracked[self.eng.fork(b)] = (item, i)
+
     def _loop(self):
-        tracked: Dict[int, Dict] = {}
+        # slot -> (request, which of its answers)
+        tracked: Dict[int, tuple] = {}
         pending: List[Dict] = []
         while True:
             # drain arrivals; block only when completely idle
@@ -146,7 +168,9 @@ class _ContinuousWorker:
                 except queue.Empty:
                     break
             for item in list(pending):
-                if not self.eng.can_admit(len(item["ids"])):
+                fits = self.eng.can_admit(len(item["ids"]), item["n"]) \
+                    if self.paged else self.eng.can_admit(len(item["ids"]))
+                if not fits:
                     if self.eng.n_active() == 0:
                         item["err"] = RuntimeError(
                             "prompt exceeds the serving context window")
@@ -154,9 +178,7 @@ class _ContinuousWorker:
                         pending.remove(item)
                     continue
                 try:
-                    b = self.eng.admit(item["ids"], item["cfg"],
-                                       item.get("cb"))
-                    tracked[b] = item
+                    self._admit(item, tracked)
                 except Exception as e:  # noqa: BLE001
                     item["err"] = e
                     item["evt"].set()
@@ -165,23 +187,25 @@ class _ContinuousWorker:
                 try:
                     self.eng.step()
                 except Exception as e:  # noqa: BLE001
-                    for item in tracked.values():
+                    for item, _ in tracked.values():
                         item["err"] = e
                         item["evt"].set()
                     tracked.clear()
-            for b, item in list(tracked.items()):
+            for b, (item, i) in list(tracked.items()):
                 s = self.eng.slots[b]
                 if not s.active and s.result is not None:
-                    item["out"] = s.result
-                    item["evt"].set()
+                    item["out"][i] = (s.result, getattr(s, "logprobs", None))
                     del tracked[b]
+                    if None not in item["out"]:
+                        item["evt"].set()
 
 
 def create_app(model, tokenizer, model_name: str = "luminaai-amd",
                max_batch: int = 8, serving: str = "continuous",
                max_len: int = 2048):
     """Build the ASGI app around an already-loaded model. serving:
-    "continuous" (token-level joins, default) or "dynamic" (request-level
+    "continuous" (token-level joins, default), "paged" (the same over a paged
+    cache, with `n` answers and `logprobs`) or "dynamic" (request-level
     batching with the hipGraph single-stream path for streaming)."""
     from fastapi import FastAPI
     from fastapi.responses import JSONResponse, StreamingResponse
@@ -190,9 +214,9 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
     device = next(model.parameters()).device
     engine = GenerationEngine(model, tokenizer, device)
     lock = threading.Lock()
-    if serving == "continuous":
+    if serving in ("continuous", "paged"):
         worker = _ContinuousWorker(model, tokenizer, max_batch=max_batch,
-                                   max_len=max_len)
+                                   max_len=max_len, paged=serving == "paged")
         batcher = None
     else:
         batcher = _DynamicBatcher(engine, max_batch=max_batch, lock=lock)
@@ -226,6 +250,30 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
                 out = engine.generate(prompt_ids, cfg, stream_callback=cb)
         _account(endpoint, len(out), t0)
         return out
+
+    def _answers(prompt_ids: List[int], cfg: GenerationConfig, body: Dict,
+                 endpoint: str = "completions") -> List:
+        """The request's `n` answers: (tokens, log probabilities or None)."""
+        n = int(body.get("n", 1))
+        if serving != "paged":
+            return [(_decode(prompt_ids, cfg, endpoint=endpoint), None)]
+        t0 = time.perf_counter()
+        outs = worker.submit_n(prompt_ids, cfg, n)
+        _account(endpoint, sum(len(t) for t, _ in outs), t0)
+        return [(t, lp if cfg.logprobs is not None else None)
+                for t, lp in outs]
+
+    def _refusal(body: Dict, cfg: GenerationConfig):
+        n = int(body.get("n", 1))
+        if (n != 1 or cfg.logprobs is not None) and serving != "paged":
+            return "n and logprobs need serving=\"paged\""
+        if not 1 <= n <= max_batch:
+            return f"n must be 1 to {max_batch}"
+        if cfg.logprobs is not None and not 0 <= cfg.logprobs <= 64:
+            return "logprobs must be 0 to 64"
+        if body.get("stream") and (n != 1 or cfg.logprobs is not None):
+            return "a stream takes neither n nor logprobs"
+        return None
 
     def _sse_stream(prompt_ids: List[int], cfg: GenerationConfig,
                     wrap, endpoint: str = "completions") -> StreamingResponse:
@@ -280,26 +328,44 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
     def completions(body: Dict):
         prompt = body.get("prompt", "")
         cfg = _gen_config(body)
+        bad = _refusal(body, cfg)
+        if bad:
+            return JSONResponse({"error": bad}, status_code=400)
         ids = tokenizer.encode(prompt)
         if body.get("stream"):
             return _sse_stream(ids, cfg, lambda piece: {
                 "object": "text_completion.chunk",
                 "choices": [{"text": piece, "index": 0}]})
-        toks = _decode(ids, cfg)
+        outs = _answers(ids, cfg, body)
+        n_out = sum(len(t) for t, _ in outs)
+        choices = []
+        for i, (toks, lps) in enumerate(outs):
+            c = {"text": tokenizer.decode(toks), "index": i,
+                 "finish_reason": "stop"}
+            if lps is not None:
+                c["logprobs"] = {
+                    "tokens": [tokenizer.decode([e["token"]]) for e in lps],
+                    "token_logprobs": [e["logprob"] for e in lps],
+                    "top_logprobs": [
+                        {tokenizer.decode([t]): p for t, p in e["top"]}
+                        for e in lps]}
+            choices.append(c)
         return JSONResponse({
             "object": "text_completion",
             "model": model_name,
-            "choices": [{"text": tokenizer.decode(toks), "index": 0,
-                         "finish_reason": "stop"}],
+            "choices": choices,
             "usage": {"prompt_tokens": len(ids),
-                      "completion_tokens": len(toks),
-                      "total_tokens": len(ids) + len(toks)},
+                      "completion_tokens": n_out,
+                      "total_tokens": len(ids) + n_out},
         })
 
     @app.post("/v1/chat/completions")
     def chat_completions(body: Dict):
         messages = body.get("messages", [])
         cfg = _gen_config(body)
+        bad = _refusal(body, cfg)
+        if bad:
+            return JSONResponse({"error": bad}, status_code=400)
         ids: List[int] = []
         for m in messages:
             ids.extend(tokenizer.encode_message(m.get("role", "user"),
@@ -311,16 +377,28 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
                 "object": "chat.completion.chunk",
                 "choices": [{"delta": {"content": piece}, "index": 0}]},
                 endpoint="chat")
-        toks = _decode(ids, cfg, endpoint="chat")
+        outs = _answers(ids, cfg, body, endpoint="chat")
+        n_out = sum(len(t) for t, _ in outs)
+        choices = []
+        for i, (toks, lps) in enumerate(outs):
+            c = {"message": {"role": "assistant",
+                             "content": tokenizer.decode(toks)},
+                 "index": i, "finish_reason": "stop"}
+            if lps is not None:
+                c["logprobs"] = {"content": [
+                    {"token": tokenizer.decode([e["token"]]),
+                     "logprob": e["logprob"],
+                     "top_logprobs": [{"token": tokenizer.decode([t]),
+                                       "logprob": p} for t, p in e["top"]]}
+                    for e in lps]}
+            choices.append(c)
         return JSONResponse({
             "object": "chat.completion",
             "model": model_name,
-            "choices": [{"message": {"role": "assistant",
-                                     "content": tokenizer.decode(toks)},
-                         "index": 0, "finish_reason": "stop"}],
+            "choices": choices,
             "usage": {"prompt_tokens": len(ids),
-                      "completion_tokens": len(toks),
-                      "total_tokens": len(ids) + len(toks)},
+                      "completion_tokens": n_out,
+                      "total_tokens": len(ids) + n_out},
         })
 
     return app
@@ -346,7 +424,7 @@ def main(argv=None):
     ap.add_argument("--max-len", type=int, default=2048,
                     help="serving context window (KV cache columns)")
     ap.add_argument("--serving", default="continuous",
-                    choices=["continuous", "dynamic"])
+                    choices=["continuous", "paged", "dynamic"])
     args = ap.parse_args(argv)
 
     device = torch.device(args.device) if args.device else (

@@ -362,7 +362,8 @@ class GroupedQueryAttention(nn.Module):
 
     def forward(self, x, rope_cs, pos: Optional[torch.Tensor] = None,
                 pos_offset: int = 0, kv_cache: Optional[KVCache] = None,
-                attn_mask: Optional[torch.Tensor] = None):
+                attn_mask: Optional[torch.Tensor] = None,
+                cu_seqlens: Optional[torch.Tensor] = None):
         B, S, _ = x.shape
         if self.tp_group is not None:
             from ..parallel.tensor_parallel import tp_copy
@@ -377,6 +378,14 @@ class GroupedQueryAttention(nn.Module):
         # RoPE first, on local tokens with their GLOBAL positions — the
         # Ulysses exchange below then needs no position bookkeeping.
         q, k = ops.rope(q, k, cos, sin, pos, pos_offset)
+
+        if cu_seqlens is not None or getattr(kv_cache, "paged", False):
+            out = self._ragged(q, k, v, kv_cache, cu_seqlens)
+            out = _linear(self.o_proj, out.reshape(B, S, self.q_size))
+            if self.tp_group is not None:
+                from ..parallel.tensor_parallel import tp_reduce
+                out = tp_reduce(out, self.tp_group)
+            return out
 
         if kv_cache is not None:
             k, v = kv_cache.append(k, v)
@@ -458,6 +467,23 @@ class GroupedQueryAttention(nn.Module):
             from ..parallel.tensor_parallel import tp_reduce
             out = tp_reduce(out, self.tp_group)
         return out
+
+
+    def _ragged(self, q, k, v, kv_cache, cu_seqlens):
+        """Attention of sequences of different lengths without padding: packed
+        prompts or documents ([1, T], cu_seqlens), or one new token for each
+        row over a paged cache ([B, 1])."""
+        if self.dropout > 0 and self.training:
+            raise ValueError("packed sequences do not support attention "
+                             "dropout")
+        if kv_cache is not None:
+            kv_cache.append(k.flatten(0, 1), v.flatten(0, 1))
+            if cu_seqlens is None:
+                return kv_cache.attend(q.flatten(0, 1),
+                                       self.head_dim ** -0.5)
+        self._flash_calls = getattr(self, "_flash_calls", 0) + 1
+        return ops.flash_attention_packed(q[0], k[0], v[0], cu_seqlens,
+                                          self.head_dim ** -0.5)
 
 
 class SwiGLUExpert(nn.Module):
@@ -821,10 +847,11 @@ class TransformerBlock(nn.Module):
                                         config.mod_routing_temperature)
         self._mod_skip_frac = 0.0
 
-    def _inner(self, x, rope_cs, pos, pos_offset, kv_cache, attn_mask):
+    def _inner(self, x, rope_cs, pos, pos_offset, kv_cache, attn_mask,
+               cu_seqlens=None):
         """attention + FFN with residuals; returns (out, aux_loss)."""
         h = self.attention(self.input_norm(x), rope_cs, pos, pos_offset,
-                           kv_cache, attn_mask)
+                           kv_cache, attn_mask, cu_seqlens)
         x = x + h
         if self.is_moe:
             f, aux = self.ffn(self.post_attn_norm(x))
@@ -835,12 +862,17 @@ class TransformerBlock(nn.Module):
 
     def forward(self, x, rope_cs, pos: Optional[torch.Tensor] = None,
                 pos_offset: int = 0, kv_cache: Optional[KVCache] = None,
-                attn_mask: Optional[torch.Tensor] = None):
+                attn_mask: Optional[torch.Tensor] = None,
+                cu_seqlens: Optional[torch.Tensor] = None):
         B, S, H = x.shape
         run_mod = (self.use_mod and kv_cache is None and S > 1
                    and int(S * self.mod_capacity) < S)
         if not run_mod:
-            return self._inner(x, rope_cs, pos, pos_offset, kv_cache, attn_mask)
+            return self._inner(x, rope_cs, pos, pos_offset, kv_cache,
+                               attn_mask, cu_seqlens)
+        if cu_seqlens is not None:
+            raise ValueError("mixture-of-depths layers choose tokens of a whole "
+                             "row: packed sequences are not supported")
 
         top, scores = self.mod_router(x)                 # [B, K], [B, S]
         K = top.shape[1]
@@ -936,12 +968,35 @@ class DeepSeekTransformer(nn.Module):
                 kv_caches: Optional[List[KVCache]] = None,
                 pos_offset: int = 0,
                 return_hidden_states: bool = False,
-                return_aux_loss: bool = True):
-        """Returns (logits, total_aux_loss, aux_losses dict)."""
+                return_aux_loss: bool = True,
+                cu_seqlens: Optional[torch.Tensor] = None):
+        """Returns (logits, total_aux_loss, aux_losses dict).
+
+        cu_seqlens (int32 [n + 1], rising from 0): input_ids [1, T] holds n
+        sequences one after the other, each with positions from 0 and
+        attention inside itself (ops.flash_attention_packed). Not together
+        with an attention_mask, unpaged caches, sequence parallelism or
+        mixture-of-depths layers in training."""
         B, S = input_ids.shape
+        paged = kv_caches is not None and getattr(kv_caches[0], "paged", False)
+        if cu_seqlens is not None:
+            if B != 1:
+                raise ValueError("packed sequences are one row: input_ids must "
+                                 f"be [1, tokens], got {tuple(input_ids.shape)}")
+            if attention_mask is not None or (kv_caches is not None
+                                              and not paged):
+                raise ValueError("packed sequences take no attention_mask and "
+                                 "no cache but a paged one")
+        elif paged and S != 1:
+            raise ValueError("a paged cache takes packed prompts (cu_seqlens) "
+                             "or one token for each row")
         x = self.embed_tokens(input_ids) * self.embed_scale
         pos = None
-        if kv_caches is not None and kv_caches[0].seq_len > 0:
+        if paged:
+            pos = kv_caches[0].positions.view(B, S)
+        elif cu_seqlens is not None:
+            pos = ops.packed_positions(cu_seqlens, S)
+        elif kv_caches is not None and kv_caches[0].seq_len > 0:
             pos_offset = kv_caches[0].seq_len
         if kv_caches is not None and S == 1 \
                 and getattr(kv_caches[0], "graph_mode", False) \
@@ -954,8 +1009,12 @@ class DeepSeekTransformer(nn.Module):
         from ..parallel.mesh import get_mesh
         mesh = get_mesh()
         if mesh is not None and mesh.sp_size > 1 and kv_caches is None and S > 1:
+            if cu_seqlens is not None:
+                raise ValueError("packed sequences do not support sequence "
+                                 "parallelism")
             pos_offset = pos_offset + mesh.sp_rank * S
-        rope_cs = self.rotary.get(pos_offset + S, x.device)
+        rope_cs = self.rotary.get(kv_caches[0].max_len if paged
+                                  else pos_offset + S, x.device)
 
         attn_mask = None
         if attention_mask is not None and attention_mask.dim() == 2 \
@@ -982,9 +1041,10 @@ class DeepSeekTransformer(nn.Module):
             if self.gradient_checkpointing and self.training and cache is None:
                 x, aux = torch.utils.checkpoint.checkpoint(
                     layer, x, rope_cs, pos, pos_offset, None, attn_mask,
-                    use_reentrant=False)
+                    cu_seqlens, use_reentrant=False)
             else:
-                x, aux = layer(x, rope_cs, pos, pos_offset, cache, attn_mask)
+                x, aux = layer(x, rope_cs, pos, pos_offset, cache, attn_mask,
+                               cu_seqlens)
             if layer.is_moe:
                 total_aux = total_aux + aux
                 aux_losses[f"layer_{i}_moe"] = aux.detach()

@@ -66,4 +66,5 @@ def packed_positions(cu_seqlens: torch.Tensor, total: int) -> torch.Tensor:
     tok = torch.arange(total, dtype=torch.int32, device=cu_seqlens.device)
     seq = torch.searchsorted(cu_seqlens[1:].contiguous(), tok, right=True)
     start = cu_seqlens[seq.clamp(max=cu_seqlens.shape[0] - 1)]
-    return (tok - start).view(1, total)
+    # wrong borders must not index outside a rope table
+    return (tok - start).clamp(0, total - 1).view(1, total)

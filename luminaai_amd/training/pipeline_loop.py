@@ -99,6 +99,9 @@ def run_pipeline_training(model, cfg, train_ds, logger, pp: int = 0,
     """Train `model` over a pp (x tp) (x dp) world. Returns summary stats."""
     from torch.utils.data import DataLoader, Subset
 
+    if getattr(cfg, "pack_sequences", False):
+        raise ValueError("pipeline training does not support packed batches: "
+                         "set pack_sequences = False")
     world = comm.get_world_size()
     rank = comm.get_rank()
     pp = pp or (world // max(tp, 1))

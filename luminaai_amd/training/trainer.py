@@ -155,7 +155,14 @@ class Trainer:
         weights = batch.get("loss_weights")
         if weights is not None:
             weights = weights.to(self.device, non_blocking=True)
+        # a packed batch (data/dataset.py pack_collate): one row of sequences
+        cu_seqlens = batch.get("cu_seqlens")
+        if cu_seqlens is not None:
+            cu_seqlens = cu_seqlens.to(self.device, non_blocking=True)
         if self.mesh is not None and self.mesh.sp_size > 1:
+            if cu_seqlens is not None:
+                raise ValueError("packed batches do not support sequence "
+                                 "parallelism: set pack_sequences = False")
             if input_ids.shape[1] % self.mesh.sp_size != 0:
                 # A silent skip here would leave every rank training on the
                 # FULL sequence while the model still applies sp_rank-shifted
@@ -176,7 +183,8 @@ class Trainer:
                 weights = shard_sequence(weights, self.mesh.sp_rank,
                                          self.mesh.sp_size)
 
-        logits, aux, _ = self.model(input_ids)
+        kw = {} if cu_seqlens is None else {"cu_seqlens": cu_seqlens}
+        logits, aux, _ = self.model(input_ids, **kw)
         out = self.compute_loss(logits, labels, weights, aux)
         # grads are SUMMED over micro-batches; normalisation happens once in
         # the fused optimizer kernel via grad_scale = 1/(accum*world).
@@ -324,7 +332,9 @@ class Trainer:
             w = batch.get("loss_weights")
             if w is not None:
                 w = w.to(self.device)
-            logits, aux, _ = self.model(input_ids)
+            kw = {"cu_seqlens": batch["cu_seqlens"].to(self.device)} \
+                if "cu_seqlens" in batch else {}
+            logits, aux, _ = self.model(input_ids, **kw)
             out = self.compute_loss(logits, labels, w, None)
             tot_loss += float(out["ce_loss"])
             tot_acc += float(out["accuracy"])
@@ -997,8 +1007,10 @@ class Trainer:
             _sync(); t0 = _time.perf_counter()
             ids = batch["input_ids"].to(self.device, non_blocking=False)
             labels = batch["labels"].to(self.device, non_blocking=False)
+            kw = {"cu_seqlens": batch["cu_seqlens"].to(self.device)} \
+                if "cu_seqlens" in batch else {}
             _sync(); t1 = _time.perf_counter()
-            logits, aux, _ = self.model(ids)
+            logits, aux, _ = self.model(ids, **kw)
             out = self.compute_loss(logits, labels, None, aux)
             _sync(); t2 = _time.perf_counter()
             out["loss"].backward()

@@ -1,0 +1,455 @@
+"""Paged cache bookkeeping, paged serving, packed forwards and scoring (CPU), and
+the same runs on the kernels."""
+
+import math
+
+import pytest
+import torch
+
+from luminaai_amd import ops
+from luminaai_amd.inference import (ContinuousBatchingEngine,
+                                    GenerationConfig, GenerationEngine,
+                                    PagedBatchingEngine, PagedKVCache)
+
+
+def _cfg(n=6, **kw):
+    return GenerationConfig(max_new_tokens=n, temperature=0.0,
+                            stop_token_ids=[-1], **kw)
+
+
+def _engine(model, tokenizer, **kw):
+    kw = {"max_batch": 4, "max_len": 64, "page_size": 16, **kw}
+    return PagedBatchingEngine(model, tokenizer, **kw)
+
+
+# ------------------------------------------------------------ bookkeeping
+def _cache(pages=8, **kw):
+    return PagedKVCache(2, 1, 8, pages, 16, max_seqs=4, max_len=80,
+                        dtype=torch.float32, **kw)
+
+
+def _check(c):
+    """Reference counts are what the tables say, and the free pages the rest."""
+    used = [p for t in c.tables for p in t]
+    assert c._refs == [used.count(p) for p in range(c.pages)]
+    assert sorted(c._free) == [p for p in range(c.pages) if not c._refs[p]]
+    for slot, t in enumerate(c.tables):
+        assert c._table[slot, :len(t)].tolist() == t
+        assert len(t) == c.pages_for(c.lens[slot])
+
+
+def _write(c, slot, value):
+    """One token of `value` into every layer."""
+    layers = c.decode([slot])
+    for i, layer in enumerate(layers):
+        kv = torch.full((1, 1, 8), value + i)
+        layer.append(kv, -kv)
+
+
+def _read(c, slot):
+    pages = torch.tensor(c.tables[slot])
+    return [c.k[i][pages].transpose(1, 2).reshape(-1, 8)[:c.lens[slot], 0]
+            .tolist() for i in range(2)]
+
+
+def test_cache_grow_fork_free_compact_resize():
+    c = _cache()
+    c.prefill([1], [20])
+    _check(c)
+    for t in range(15):
+        _write(c, 0, 100.0 + t)
+    _write(c, 1, 7.0)
+    _check(c)
+    c.fork(0, 2)
+    c.fork(0, 3)
+    _check(c)
+    assert c.tables[2] == c.tables[0] and c.free_pages == 8 - 3
+    # the first two writers copy the shared page, the last one keeps it
+    assert c.pages_needed([0, 2, 3], [1, 1, 1]) == 2
+    for slot, v in ((0, 1.0), (2, 2.0), (3, 3.0)):
+        _write(c, slot, v)
+        _check(c)
+    assert len({c.tables[s][0] for s in (0, 2, 3)}) == 3
+    base = [100.0 + t for t in range(15)]
+    for slot, v in ((0, 1.0), (2, 2.0), (3, 3.0)):
+        assert _read(c, slot) == [base + [v], [x + 1 for x in base] + [v + 1]]
+    one = _read(c, 1)
+    c.free(0)
+    c.free(2)
+    _check(c)
+    assert c.compact() == 0         # the live pages are the first already
+    _write(c, 0, 5.0)
+    assert _read(c, 1) == one
+    c.free(1)
+    assert c.compact() == 2
+    _check(c)
+    assert sorted(p for t in c.tables for p in t) == [0, 1]
+    assert _read(c, 3)[0] == base + [3.0] and _read(c, 0) == [[5.0], [6.0]]
+    c.resize(2)
+    _check(c)
+    assert _read(c, 3)[0] == base + [3.0] and c.free_pages == 0
+    with pytest.raises(ValueError, match="in use"):
+        c.resize(1)
+    c.resize(9)
+    _check(c)
+    _write(c, 3, 4.0)
+    assert _read(c, 3)[0] == base + [3.0, 4.0]
+    assert _read(c, 0) == [[5.0], [6.0]]
+
+
+def test_cache_refusals_change_nothing():
+    c = _cache(pages=2)
+    c.prefill([0], [17])
+    for call, err in [(lambda: c.prefill([1], [1]), MemoryError),
+                      (lambda: c.extend([0], [64]), ValueError),
+                      (lambda: c.decode([0, 0]), ValueError),
+                      (lambda: c.prefill([0], [1]), ValueError),
+                      (lambda: c.fork(1, 0), ValueError)]:
+        with pytest.raises(err):
+            call()
+        _check(c)
+        assert c.lens == [17, 0, 0, 0]
+    with pytest.raises(ValueError, match="power of two"):
+        PagedKVCache(1, 1, 8, 4, 24)
+
+
+# ------------------------------------------------------------ packed forward
+def test_packed_forward_equals_each_alone(small_model):
+    m = small_model.eval()
+    g = torch.Generator().manual_seed(0)
+    seqs = [torch.randint(1, 500, (n,), generator=g) for n in (5, 1, 17, 30)]
+    cu = torch.tensor([0, 5, 6, 23, 53], dtype=torch.int32)
+    with torch.no_grad():
+        out, _, _ = m(torch.cat(seqs)[None], cu_seqlens=cu)
+        for i, s in enumerate(seqs):
+            alone, _, _ = m(s[None])
+            assert torch.allclose(out[0, cu[i]:cu[i + 1]], alone[0],
+                                  atol=1e-5)
+
+
+@pytest.mark.parametrize("checkpointing", [False, True])
+def test_packed_training_equals_padded(small_model, tiny_config,
+                                       checkpointing):
+    """Loss and gradients of a packed batch are those of the padded one."""
+    from luminaai_amd.data import pack_collate
+    from luminaai_amd.ops import fused_cross_entropy
+    m = small_model.train()
+    m.gradient_checkpointing = checkpointing
+    g = torch.Generator().manual_seed(1)
+    samples = []
+    for n in (3, 11, 20):
+        ids = torch.zeros(21, dtype=torch.long)
+        ids[:n + 1] = torch.randint(1, 500, (n + 1,), generator=g)
+        labels = ids[1:].clone()
+        labels[n:] = -100
+        samples.append({"input_ids": ids[:-1], "labels": labels,
+                        "loss_weights": torch.rand(20, generator=g)})
+    grads = []
+    for batch in (torch.utils.data.default_collate(samples),
+                  pack_collate(samples)):
+        kw = {k: v for k, v in batch.items() if k == "cu_seqlens"}
+        logits, _, _ = m(batch["input_ids"], **kw)
+        loss, _, n = fused_cross_entropy(logits, batch["labels"],
+                                         batch["loss_weights"])
+        grads.append((loss, torch.autograd.grad(loss, list(m.parameters())),
+                      int(n)))
+    assert grads[0][2] == grads[1][2] == 34
+    assert torch.allclose(grads[0][0], grads[1][0], atol=1e-6)
+    for a, b in zip(grads[0][1], grads[1][1]):
+        assert torch.allclose(a, b, atol=1e-6)
+
+
+def test_trainer_takes_packed_batches(tiny_config, sample_conversations,
+                                      tokenizer):
+    from luminaai_amd.data import ConversationDataset, create_dataloader
+    from luminaai_amd.models import (DeepSeekTransformer,
+                                     config_to_deepseek_config)
+    from luminaai_amd.training import Trainer
+    tiny_config.pack_sequences = True
+    torch.manual_seed(0)
+    m = DeepSeekTransformer(config_to_deepseek_config(tiny_config))
+    ds = ConversationDataset(sample_conversations, tokenizer, 64)
+    loader = create_dataloader(ds, tiny_config, shuffle=False)
+    batch = next(iter(loader))
+    assert batch["input_ids"].shape[0] == 1
+    assert batch["cu_seqlens"].tolist()[-1] == batch["input_ids"].shape[1]
+    t = Trainer(m, tokenizer, tiny_config)
+    t._setup_scheduler(4)
+    out = t.train_step(batch)
+    t.optimizer_step()
+    assert math.isfinite(float(out["ce_loss"]))
+    res = t.evaluate(loader)
+    assert math.isfinite(res["loss"])
+
+
+@pytest.mark.parametrize("cu", [[0, 3, 8], [5, 6, 8], [0, 9, 2, 5], [0, 99],
+                                [-40, 2, 8], [8, 8], [0]])
+def test_positions_index_inside_the_row(cu):
+    """Whatever the borders hold, positions stay below the row's length."""
+    pos = ops.packed_positions(torch.tensor(cu, dtype=torch.int32), 8)
+    assert pos.shape == (1, 8) and pos.dtype == torch.int32
+    assert 0 <= int(pos.min()) and int(pos.max()) < 8
+    if cu == [0, 3, 8]:
+        assert pos[0].tolist() == [0, 1, 2, 0, 1, 2, 3, 4]
+
+
+def test_packed_forward_refusals(small_model, tiny_config):
+    from luminaai_amd.models import (DeepSeekTransformer,
+                                     config_to_deepseek_config)
+    ids = torch.ones(1, 6, dtype=torch.long)
+    cu = torch.tensor([0, 2, 6], dtype=torch.int32)
+    m = small_model.eval()
+    with pytest.raises(ValueError, match="one row"):
+        m(ids.expand(2, 6), cu_seqlens=cu)
+    with pytest.raises(ValueError, match="no attention_mask"):
+        m(ids, attention_mask=torch.ones(1, 6), cu_seqlens=cu)
+    with pytest.raises(ValueError, match="no attention_mask"):
+        m(ids, kv_caches=m.make_kv_caches(8), cu_seqlens=cu)
+    c = PagedKVCache(2, 2, 16, 4, 16, dtype=torch.float32)
+    layers, _ = c.prefill([0], [6])
+    with pytest.raises(ValueError, match="packed prompts"):
+        m(ids, kv_caches=layers)
+    tiny_config.use_mod = True
+    mod = DeepSeekTransformer(config_to_deepseek_config(tiny_config))
+    with pytest.raises(ValueError, match="mixture-of-depths"):
+        mod(ids, cu_seqlens=cu)
+    tiny_config.use_mod = False
+    tiny_config.dropout = 0.1
+    drop = DeepSeekTransformer(config_to_deepseek_config(tiny_config)).train()
+    with pytest.raises(ValueError, match="dropout"):
+        drop(ids, cu_seqlens=cu)
+
+
+# ------------------------------------------------------------ serving
+def test_paged_matches_solo_staggered(small_model, tokenizer):
+    solo = GenerationEngine(small_model.eval(), tokenizer)
+    prompts = [tokenizer.encode(p) for p in
+               ("the first and longest prompt here", "second one", "third",
+                "a", "and one that comes when a slot is free again")]
+    refs = [solo.generate(p, _cfg()) for p in prompts]
+    eng = _engine(small_model, tokenizer, max_batch=3)
+    outs = eng.run_to_completion(prompts, _cfg(),
+                                 admit_schedule=[0, 2, 0, 9, 1])
+    assert outs == refs
+    assert eng.stats["admitted"] == eng.stats["finished"] == 5
+    assert eng.cache.free_pages == eng.cache.pages
+    _check(eng.cache)
+
+
+def test_long_prompt_joins_at_once(small_model, tokenizer):
+    """No admission waits for the others' length."""
+    eng = _engine(small_model, tokenizer)
+    a = eng.admit(tokenizer.encode("ab"), _cfg(8))
+    eng.step()
+    long = tokenizer.encode("a much longer prompt than two tokens")
+    assert eng.can_admit(len(long))
+    b = eng.admit(long, _cfg(3))
+    while eng.n_active():
+        eng.step()
+    solo = GenerationEngine(small_model.eval(), tokenizer)
+    assert eng.slots[b].result == solo.generate(long, _cfg(3))
+    assert eng.slots[a].result == solo.generate(tokenizer.encode("ab"),
+                                                _cfg(8))
+
+
+def test_forks_continue_on_shared_pages(small_model, tokenizer):
+    """Forks that decode greedily agree with solo; then one of them is led
+    elsewhere and the others do not notice."""
+    prompt = tokenizer.encode("a prompt that is forked in the middle of a page")
+    solo = GenerationEngine(small_model.eval(), tokenizer)
+    ref = solo.generate(prompt, _cfg(6))
+    eng = _engine(small_model, tokenizer)
+    a = eng.admit(prompt, _cfg(6))
+    used = eng.cache.pages - eng.cache.free_pages
+    b, c = eng.fork(a), eng.fork(a)
+    assert eng.cache.pages - eng.cache.free_pages == used
+    eng.last_logits[c] = 0
+    eng.last_logits[c, ref[0] + 1] = 9.0
+    while eng.n_active():
+        eng.step()
+    assert eng.slots[a].result == eng.slots[b].result == ref
+    other = solo.generate(prompt + [ref[0] + 1], _cfg(5))
+    assert eng.slots[c].result == [ref[0] + 1] + other
+    _check(eng.cache)
+
+
+def test_full_pool_ends_a_sequence(small_model, tokenizer):
+    eng = _engine(small_model, tokenizer, pages=2)
+    a = eng.admit([5] * 10, _cfg(60))
+    b = eng.admit([6] * 12, _cfg(60))
+    assert not eng.can_admit(1)
+    while eng.n_active():
+        eng.step()
+    got = sorted(len(eng.slots[s].result) for s in (a, b))
+    assert got[0] < got[1] and _check(eng.cache) is None
+    with pytest.raises(RuntimeError, match="does not hold"):
+        eng.run_to_completion([[5] * 40], _cfg(2))
+
+
+def test_continuous_and_paged_agree(small_model, tokenizer):
+    prompts = [tokenizer.encode(f"prompt number {i}") for i in range(4)]
+    a = ContinuousBatchingEngine(small_model.eval(), tokenizer, max_batch=2,
+                                 max_len=64)
+    b = _engine(small_model, tokenizer, max_batch=2)
+    assert a.run_to_completion(prompts, _cfg(4)) == \
+        b.run_to_completion(prompts, _cfg(4))
+
+
+def test_logprobs_of_answers_equal_scores(small_model, tokenizer):
+    """What the engine reports while it decodes is what scoring the finished
+    text says."""
+    prompts = [tokenizer.encode("some prompt"), tokenizer.encode("x")]
+    eng = _engine(small_model, tokenizer)
+    slots = eng.admit_many(prompts, [_cfg(5, logprobs=3), _cfg(4)])
+    while eng.n_active():
+        eng.step()
+    s = eng.slots[slots[0]]
+    assert eng.slots[slots[1]].logprobs == []
+    assert [e["token"] for e in s.logprobs] == s.result
+    solo = GenerationEngine(small_model.eval(), tokenizer)
+    full = prompts[0] + s.result
+    score, empty, one = solo.score([full, [], [3]], top_k=3)
+    assert empty["logprobs"] == [] and one["logprobs"] == []
+    assert len(score["logprobs"]) == len(full) - 1
+    for i, e in enumerate(s.logprobs):
+        at = len(prompts[0]) - 1 + i
+        assert abs(e["logprob"] - score["logprobs"][at]) < 1e-4
+        assert [t for t, _ in e["top"]] == score["top_ids"][at]
+        assert e["top"][0][0] == e["token"]         # greedy
+    with pytest.raises(ValueError, match="logprobs"):
+        eng.admit([1, 2], _cfg(2, logprobs=65))
+
+
+def test_scores_one_by_one_for_mixture_of_depths(tiny_config, tokenizer):
+    from luminaai_amd.models import (DeepSeekTransformer,
+                                     config_to_deepseek_config)
+    tiny_config.use_mod = True
+    torch.manual_seed(0)
+    m = DeepSeekTransformer(config_to_deepseek_config(tiny_config)).eval()
+    out = GenerationEngine(m, tokenizer).score([[1, 2, 3], [4, 5]])
+    assert [len(o["logprobs"]) for o in out] == [2, 1]
+    with torch.no_grad():
+        lp = m(torch.tensor([[1, 2, 3]]))[0][0].float().log_softmax(-1)
+    assert abs(out[0]["logprobs"][1] - float(lp[1, 3])) < 1e-5
+
+
+def test_server_paged(small_model, tokenizer):
+    pytest.importorskip("fastapi")
+    from fastapi.testclient import TestClient
+    from luminaai_amd.inference.server import create_app
+    client = TestClient(create_app(small_model.eval(), tokenizer,
+                                   serving="paged", max_len=64, max_batch=4))
+    body = {"prompt": "hello", "max_tokens": 4, "temperature": 0.0}
+    one = client.post("/v1/completions", json=body).json()
+    r = client.post("/v1/completions", json={**body, "n": 3, "logprobs": 2})
+    got = r.json()
+    assert r.status_code == 200 and len(got["choices"]) == 3
+    for c in got["choices"]:
+        assert c["text"] == one["choices"][0]["text"]
+        assert len(c["logprobs"]["token_logprobs"]) == \
+            one["usage"]["completion_tokens"]
+    assert "logprobs" not in one["choices"][0]
+    chat = client.post("/v1/chat/completions", json={
+        "messages": [{"role": "user", "content": "hi"}], "max_tokens": 3,
+        "temperature": 0.0, "logprobs": True, "top_logprobs": 1}).json()
+    assert all(len(e["top_logprobs"]) == 1
+               for e in chat["choices"][0]["logprobs"]["content"])
+    for bad in ({"n": 9}, {"n": 0}, {"logprobs": 65},
+                {"n": 2, "stream": True}):
+        assert client.post("/v1/completions",
+                           json={**body, **bad}).status_code == 400
+    plain = TestClient(create_app(small_model.eval(), tokenizer, max_len=64))
+    assert plain.post("/v1/completions",
+                      json={**body, "n": 2}).status_code == 400
+
+
+# ------------------------------------------------------------ on the GPU
+@pytest.fixture
+def gpu_model(tiny_config):
+    from luminaai_amd.models import (DeepSeekTransformer,
+                                     config_to_deepseek_config)
+    tiny_config.hidden_size, tiny_config.num_heads = 318, 6    # heads of 53
+    tiny_config.num_kv_heads = 2
+    torch.manual_seed(0)
+    m = DeepSeekTransformer(config_to_deepseek_config(tiny_config))
+    return m.to("cuda", torch.bfloat16).eval()
+
+
+@pytest.mark.gpu
+def test_gpu_paged_forward_matches_dense(gpu_model):
+    """Prefill and decode over pages against dense forwards of the same weights
+    in fp32 on the CPU. A value passes about 24 roundings of at most 2^-8 on
+    its way to the logits; added up as a random walk they make 5, and the
+    bound is three times that."""
+    import copy
+    ref_model = copy.deepcopy(gpu_model).cpu().float()
+    g = torch.Generator().manual_seed(0)
+    seqs = [torch.randint(1, 500, (n,), generator=g).cuda()
+            for n in (5, 40, 17, 33)]
+    at = gpu_model.layers[0].attention
+    c = PagedKVCache(2, at.num_kv_heads, at.head_dim, 30, 16, max_seqs=4,
+                     max_len=64, device=torch.device("cuda"))
+    with torch.no_grad():
+        layers, cu = c.prefill([2, 0, 3, 1], [len(s) - 2 for s in seqs])
+        out, _, _ = gpu_model(torch.cat([s[:-2] for s in seqs])[None],
+                              kv_caches=layers, cu_seqlens=cu)
+        got = [[out[0, cu[i]:cu[i + 1]]] for i in range(4)]
+        for t in (-2, -1):
+            x = torch.stack([s[t] for s in seqs])[:, None]
+            out, _, _ = gpu_model(x, kv_caches=c.decode([2, 0, 3, 1]))
+            for i in range(4):
+                got[i].append(out[i])
+        for i, s in enumerate(seqs):
+            ref, _, _ = ref_model(s[None].cpu())
+            x, y = torch.cat(got[i]).float().cpu(), ref[0]
+            assert (x - y).norm() <= 16 * 2 ** -8 * y.norm()
+
+
+@pytest.mark.gpu
+def test_gpu_engine_answers_and_forks(gpu_model, tokenizer):
+    prompts = [tokenizer.encode("a first prompt for the engine"),
+               tokenizer.encode("b"), tokenizer.encode("the third of them")]
+    eng = _engine(gpu_model, tokenizer)
+    slots = eng.admit_many(prompts, [_cfg(8, logprobs=2)] * 3)
+    fork = eng.fork(slots[0])
+    while eng.n_active():
+        eng.step()
+    assert eng.slots[fork].result == eng.slots[slots[0]].result
+    solo = GenerationEngine(gpu_model, tokenizer)
+    for p, b in zip(prompts, slots):
+        s = eng.slots[b]
+        assert len(s.result) == 8
+        # greedy: each token is the likeliest at its place, up to what two bf16
+        # forwards of different kernels differ by
+        score = solo.score([p + s.result], top_k=1)[0]
+        for i, e in enumerate(s.logprobs):
+            at = len(p) - 1 + i
+            assert e["top"][0][0] == e["token"]
+            assert score["logprobs"][at] >= \
+                score["top_logprobs"][at][0] - 0.25
+    _check(eng.cache)
+    with pytest.raises(TypeError, match="bf16"):
+        _engine(gpu_model.float(), tokenizer)
+
+
+@pytest.mark.gpu
+def test_gpu_packed_training_step(gpu_model):
+    """Gradients of a packed batch against those of each sequence alone in fp32
+    on the CPU: twice the roundings of a forward (about 50 of 2^-8, 7 as a
+    random walk), and three times that as the bound."""
+    import copy
+    g = torch.Generator().manual_seed(3)
+    seqs = [torch.randint(1, 500, (n,), generator=g) for n in (40, 7, 64)]
+    w = torch.randn(111, 512, generator=g)
+    cu = torch.tensor([0, 40, 47, 111], dtype=torch.int32)
+
+    def grads(m, logits):
+        loss = (logits.float() * w.to(logits.device)).sum()
+        return torch.autograd.grad(loss, list(m.parameters()))
+
+    ref_model = copy.deepcopy(gpu_model).cpu().float().train()
+    b = grads(ref_model, torch.cat([ref_model(s[None])[0][0] for s in seqs]))
+    m = gpu_model.train()
+    out, _, _ = m(torch.cat(seqs)[None].cuda(), cu_seqlens=cu.cuda())
+    for x, y in zip(grads(m, out[0][:, :512]), b):
+        assert (x.float().cpu() - y).norm() <= 21 * 2 ** -8 * y.norm()
