@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <optional>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 namespace {
@@ -725,6 +726,21 @@ void check_same_device(const at::Tensor& t, const at::Tensor& first,
                     ", not on ", first.device());
 }
 
+// Whether two elements of t may share memory (an expanded tensor, or strides
+// that step over less than they span): what is written there is not defined.
+bool overlaps(const at::Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> dims;     // stride, size
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+  std::sort(dims.begin(), dims.end());
+  int64_t extent = 1;
+  for (const auto& [stride, size] : dims) {
+    if (stride < extent) return t.numel() > 0;
+    extent += stride * (size - 1);
+  }
+  return false;
+}
+
 // Pages [P, HKV, page, W]; returns log2(page).
 int check_pages(const at::Tensor& t, const at::Tensor& like, const char* name,
                 int64_t heads, int64_t dim) {
@@ -757,7 +773,7 @@ void check_int32(const at::Tensor& t, const at::Tensor& like, int64_t dims,
   TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " must be int32, got ",
                    t.scalar_type());
   TORCH_CHECK_VALUE(t.dim() == dims && (t.numel() == 0 ||
-                    t.stride(dims - 1) == 1), name, " must be a ", dims,
+                    t.size(dims - 1) == 1 || t.stride(dims - 1) == 1), name, " must be a ", dims,
                     "-dimensional tensor with contiguous rows");
 }
 
@@ -769,7 +785,9 @@ at::Tensor paged_attn(const at::Tensor& q_, const at::Tensor& kp,
   TORCH_CHECK_VALUE(q_.dim() == 3, "q must be [batch, heads, head_dim]");
   TORCH_CHECK_TYPE(is_bf16(q_), "paged_attention on the GPU takes bf16, got ",
                    q_.scalar_type());
-  TORCH_CHECK(!(at::GradMode::is_enabled() && q_.requires_grad()),
+  TORCH_CHECK(!(at::GradMode::is_enabled() &&
+                (q_.requires_grad() || kp.requires_grad() ||
+                 vp.requires_grad())),
               "paged_attention has no gradient: call it under torch.no_grad()");
   const c10::DeviceGuard guard(q_.device());
   const at::Tensor q = q_.stride(2) == 1 || q_.size(2) == 1
@@ -782,6 +800,8 @@ at::Tensor paged_attn(const at::Tensor& q_, const at::Tensor& kp,
   TORCH_CHECK_VALUE(D >= 1 && D <= 192, "head_dim must be 1 to 192, got ", D);
   TORCH_CHECK_VALUE(HKV > 0 && H > 0 && H % HKV == 0, "heads (", H,
                     ") must be a multiple of kv_heads (", HKV, ")");
+  TORCH_CHECK_VALUE(scale > -1e30 && scale < 1e30, "scale must be between -1e30 "
+                    "and 1e30, got ", scale);
   const int shift = check_pages(kp, q, "k_pages", HKV, D);
   check_pages(vp, q, "v_pages", HKV, D);
   check_int32(table, q, 2, "block_table");
@@ -845,6 +865,9 @@ void paged_append(const at::Tensor& k_, const at::Tensor& v_,
                     "k_pages and v_pages must be of one shape");
   const int shift = check_pages(kp, k, "k_pages", HKV, D);
   check_pages(vp, k, "v_pages", HKV, D);
+  TORCH_CHECK_VALUE(!overlaps(kp) && !overlaps(vp) &&
+                    (kp.numel() == 0 || kp.data_ptr() != vp.data_ptr()),
+                    "the pages' memory overlaps");
   check_int32(table, k, 2, "block_table");
   check_int32(pos, k, 1, "positions");
   TORCH_CHECK_VALUE(pos.size(0) == T, "positions has ", pos.size(0),
@@ -896,6 +919,7 @@ void copy_pages(const std::vector<at::Tensor>& pools,
                       "a pool is empty");
     TORCH_CHECK_VALUE(t[0][0].is_contiguous(), "a pool's pages must be "
                       "contiguous");
+    TORCH_CHECK_VALUE(!overlaps(t), "a pool's memory overlaps");
     TORCH_CHECK_VALUE(t.size(1) <= INT32_MAX, "a pool has too many pages");
     if (!d.empty())
       TORCH_CHECK_VALUE(s.front() >= 0 && d.front() >= 0 &&
@@ -957,7 +981,7 @@ logprob_fwd(const at::Tensor& x, const at::Tensor& tok, int64_t k,
   const int64_t N = x.size(0), V = x.size(1);
   TORCH_CHECK_VALUE(tok.dim() == 1 && tok.size(0) == N && tok.is_contiguous(),
                     "tokens must hold one token for each of the ", N, " rows");
-  TORCH_CHECK_VALUE(V <= INT32_MAX - 8 && N <= INT32_MAX,
+  TORCH_CHECK_VALUE(V <= (1 << 30) && N <= INT32_MAX,
                     "logits of ", N, " x ", V, " are not supported");
   TORCH_CHECK_VALUE(k >= 0 && k <= 64 && k <= V, "top_k must be 0 to 64 and at "
                     "most the vocabulary's ", V, ", got ", k);
@@ -1069,10 +1093,13 @@ packed_attn_fwd(const at::Tensor& q_, const at::Tensor& k_,
                     ") must be a multiple of kv_heads (", HKV, ")");
   TORCH_CHECK_VALUE(T <= (1 << 30), "at most 2^30 tokens, got ", T);
   check_int32(cu, q_, 1, "cu_seqlens");
-  TORCH_CHECK_VALUE(cu.size(0) >= 1 && cu.size(0) <= (1 << 24),
-                    "cu_seqlens needs one entry more than there are sequences");
-  TORCH_CHECK_VALUE(scale > 0 && scale < INFINITY, "scale must be positive, got ",
-                    scale);
+  TORCH_CHECK_VALUE(cu.size(0) >= 1, "cu_seqlens needs one entry more than "
+                    "there are sequences");
+  // every workgroup looks for its rows in cu_seqlens
+  TORCH_CHECK_VALUE(cu.size(0) <= 65537, "at most 65536 sequences, got ",
+                    cu.size(0) - 1);
+  TORCH_CHECK_VALUE(scale > 1e-30 && scale < 1e30, "scale must be positive "
+                    "(1e-30 to 1e30), got ", scale);
   const c10::DeviceGuard guard(q_.device());
   const auto in = align_rows({q_, k_, v_});
   const auto &q = in[0], &k = in[1], &v = in[2];

@@ -28,6 +28,8 @@
 //   branch skipped the loads, their registers would be waited for at its end.
 #include "common.h"
 
+#include <cfloat>
+
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
@@ -392,7 +394,7 @@ void packed_fwd_kernel(const PackedArgs a) {
   f32x16 o[DT];
   #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = zero16();
-  float m = -1e30f, l = 0.f;
+  float m = -FLT_MAX, l = 0.f;               // below every score
   const float c2 = a.scale * LOG2E;
 
   // keys up to the last query of the workgroup, or of the sequence

@@ -7,6 +7,8 @@
 // of a pool over all layers works as it is.
 #include "common.h"
 
+#include <cfloat>
+
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(2))) float  floatx2;
@@ -121,7 +123,7 @@ void paged_attn_kernel(const PagedAttnArgs a) {
   floatx4 oacc[2 * NDW];
   #pragma unroll
   for (int i = 0; i < 2 * NDW; ++i) oacc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-  float m = -1e30f, l = 0.f;
+  float m = -FLT_MAX, l = 0.f;             // below every score
   const int* tb = a.table + (int64_t)b * a.table_sb;
   const int pmask = (1 << a.page_shift) - 1;
   const uint16_t* kh = a.k + hkv * a.k_sh;
@@ -249,7 +251,7 @@ void paged_attn_kernel(const PagedAttnArgs a) {
   __syncthreads();
   for (int i = threadIdx.x; i < nh * a.D; i += 256) {
     const int hh = i / a.D, d = i - hh * a.D;
-    float mw[4], mm = -1e30f;
+    float mw[4], mm = -FLT_MAX;
     #pragma unroll
     for (int w = 0; w < 4; ++w) {
       mw[w] = lds[(w * nh + hh) * rowf];
@@ -293,7 +295,7 @@ void paged_attn_join_kernel(const PagedAttnArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float* ml = a.ml + bh * a.S * 2;
   const float* part = a.part + bh * a.S * a.D;
-  float m = -1e30f, l = 0.f, acc[3] = {0.f, 0.f, 0.f};
+  float m = -FLT_MAX, l = 0.f, acc[3] = {0.f, 0.f, 0.f};
   for (int s0 = wave; s0 < n; s0 += 4 * U) {
     float cm[U], cl[U], x[U][3];
     #pragma unroll

@@ -42,8 +42,8 @@ def flash_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """Causal GQA attention inside each packed sequence.
 
     q [T, H, D], k and v [T, kv_heads, D] (bf16 on the GPU, D <= 192, any
-    strides), H a multiple of kv_heads. Returns [T, H, D]. `scale` (positive)
-    defaults to D ** -0.5. Rows behind the last sequence give zeros and get zero
+    strides), H a multiple of kv_heads, and at most 65536
+    sequences. Returns [T, H, D]. `scale` (positive) defaults to D ** -0.5. Rows behind the last sequence give zeros and get zero
     gradients. The gradient is once differentiable and has one order of
     summation, so it is the same each time. The CPU refuses borders that fall or
     pass T; the GPU, which does not read them, cuts them to T and computes

@@ -219,12 +219,24 @@ def _check_pages(k_pages, v_pages, heads, dim, like):
                          f"8 wide (head_dim {dim}, got {width})")
 
 
+def _overlaps(t):
+    """Whether two elements of t may share memory (expanded tensors)."""
+    extent = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape)
+                               if n > 1):
+        if stride < extent:
+            return t.numel() > 0
+        extent += stride * (size - 1)
+    return False
+
+
 def _check_int32(t, like, dims, name):
     if t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, not on {like.device}")
     if t.dtype != torch.int32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if t.dim() != dims or (t.numel() and t.stride(-1) != 1):
+    if t.dim() != dims or (t.numel() and t.shape[-1] != 1
+                           and t.stride(-1) != 1):
         raise ValueError(f"{name} must be a {dims}-dimensional tensor with "
                          "contiguous rows")
 
@@ -233,7 +245,8 @@ def paged_attention(q, k_pages, v_pages, block_table, seq_lens, scale):
     """Sequence by sequence over gathered pages, fp32 (fp64 for fp64 input)."""
     if q.dim() != 3:
         raise ValueError("q must be [batch, heads, head_dim]")
-    if torch.is_grad_enabled() and q.requires_grad:
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad
+                                    or v_pages.requires_grad):
         raise RuntimeError("paged_attention has no gradient: call it under "
                            "torch.no_grad()")
     B, H, D = q.shape
@@ -243,6 +256,8 @@ def paged_attention(q, k_pages, v_pages, block_table, seq_lens, scale):
     P, HKV, page, _ = k_pages.shape
     if HKV == 0 or H == 0 or H % HKV:
         raise ValueError(f"heads ({H}) must be a multiple of kv_heads ({HKV})")
+    if not -1e30 < scale < 1e30:
+        raise ValueError(f"scale must be between -1e30 and 1e30, got {scale}")
     _check_int32(block_table, q, 2, "block_table")
     _check_int32(seq_lens, q, 1, "seq_lens")
     if block_table.shape[0] != B or seq_lens.shape[0] != B:
@@ -275,6 +290,9 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, positions, seq_ids):
     if not HKV or not D:
         raise ValueError("k has no heads or no channels")
     _check_pages(k_pages, v_pages, HKV, D, k)
+    if _overlaps(k_pages) or _overlaps(v_pages) or (
+            k_pages.numel() and k_pages.data_ptr() == v_pages.data_ptr()):
+        raise ValueError("the pages' memory overlaps")
     _check_int32(block_table, k, 2, "block_table")
     _check_int32(positions, k, 1, "positions")
     if positions.shape[0] != T:
@@ -325,6 +343,8 @@ def copy_pages(pools, src, dst):
             raise ValueError("a pool is empty")
         if not t[0, 0].is_contiguous():
             raise ValueError("a pool's pages must be contiguous")
+        if _overlaps(t):
+            raise ValueError("a pool's memory overlaps")
         if any(not 0 <= p < t.shape[1] for p in (*src, *dst)):
             raise ValueError(f"page numbers must be in 0 to {t.shape[1] - 1}")
     if not len(src):
@@ -400,8 +420,12 @@ def flash_attention_packed(q, k, v, cu_seqlens, scale):
     if cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens needs one entry more than there are "
                          "sequences")
-    if not 0 < scale < float("inf"):
-        raise ValueError(f"scale must be positive, got {scale}")
+    if cu_seqlens.shape[0] > 65537:
+        raise ValueError("at most 65536 sequences, got "
+                         f"{cu_seqlens.shape[0] - 1}")
+    if not 1e-30 < scale < 1e30:
+        raise ValueError("scale must be positive (1e-30 to 1e30), got "
+                         f"{scale}")
     cu = cu_seqlens.tolist()
     if cu[0] != 0 or cu[-1] > T or any(b < a for a, b in zip(cu, cu[1:])):
         raise ValueError("cu_seqlens must rise from 0 to at most the "

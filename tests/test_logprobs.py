@@ -287,3 +287,10 @@ def test_offsets_past_32_bits():
     want = ops.token_logprobs(x[-2:].clone(), tok[-2:], 2)
     for a, b in zip(r, want):
         assert torch.equal(a[-2:], b)
+
+
+@pytest.mark.gpu
+def test_gpu_refuses_rows_past_its_indexes():
+    x = torch.empty(1, 2 ** 30 + 1, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="not supported"):
+        ops.token_logprobs(x, torch.zeros(1, dtype=torch.long, device="cuda"))

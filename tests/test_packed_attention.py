@@ -258,9 +258,37 @@ def test_refusals(dev):
             (ValueError, "1-dimensional", (q, k, v, cu[None])),
             (ValueError, "one entry more", (q, k, v, cu[:0])),
             (ValueError, "scale must be positive", (q, k, v, cu, 0.0)),
-            (ValueError, "scale must be positive", (q, k, v, cu, math.nan))]:
+            (ValueError, "scale must be positive", (q, k, v, cu, math.nan)),
+            (ValueError, "scale must be positive", (q, k, v, cu, 1e-50)),
+            (ValueError, "scale must be positive", (q, k, v, cu, 1e50)),
+            (ValueError, "65536 sequences", (q, k, v, cu.new_zeros(65538)))]:
         with pytest.raises(err, match=match):
             f(*args)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_huge_scores(dev):
+    """Scores near the end of the range on either side, all of one sign: the
+    mean of the values, not zeros."""
+    q, k, v, _ = _inputs([70, 300], 0, 4, 2, 64, dev)
+    for sign in (-1, 1):
+        o = ops.flash_attention_packed(
+            torch.full_like(q, 2.0 ** 60), torch.full_like(k, sign * 2.0 ** 60),
+            torch.full_like(v, 1.5), _cu([70, 300], dev))
+        assert torch.equal(o, torch.full_like(o, 1.5))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_as_many_sequences_as_are_taken(dev):
+    """65536 sequences, all but a few of them empty."""
+    lens = [0] * 65536
+    for b, n in ((0, 3), (63, 1), (64, 40), (40000, 7), (65535, 300)):
+        lens[b] = n
+    q, k, v, go = _inputs([351], 5, 4, 2, 64, dev)
+    qkv = [t.requires_grad_(True) for t in (q, k, v)]
+    o = ops.flash_attention_packed(*qkv, _cu(lens, dev))
+    got = (o, *torch.autograd.grad(o, qkv, go))
+    _check(got, *_oracle(q, k, v, go, [n for n in lens if n], 64 ** -0.5))
 
 
 def test_border_refusals_on_the_cpu():

@@ -296,6 +296,39 @@ def test_refusals(dev):
     refuse(ValueError, "no pool", cp, ([], [0], [1]))
     refuse(ValueError, "layers, pages", cp, ([pool[0, 0, 0]], [0], [1]))
     refuse(ValueError, "contiguous", cp, ([pool.transpose(2, 3)], [0], [1]))
+    # memory that several pages share
+    same = k[:1].expand(k.shape)
+    refuse(ValueError, "overlaps", cp, ([same[None]], [0], [1]))
+    refuse(ValueError, "overlaps", cp, ([pool.expand(2, *k.shape)], [0], [1]))
+    refuse(ValueError, "overlaps", app, (kn, kn, same, v, table, P))
+    refuse(ValueError, "overlaps", app, (kn, kn, k, k, table, P))
+    refuse(RuntimeError, "no gradient",
+           args=swap(1, k.clone().requires_grad_(True)))
+    for scale in (math.inf, math.nan, 1e31):
+        refuse(ValueError, "scale", args=(*A, scale))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_huge_scores(dev):
+    """Scores near the end of the range on either side, all of one sign: the
+    mean of the values, not zeros."""
+    q, k, v, table, n, _ = _scene([20, 300], 4, 2, 64, 16, dev)
+    for sign in (-1, 1):
+        q.fill_(2.0 ** 60)
+        k.fill_(sign * 2.0 ** 60)
+        v.fill_(1.5)
+        o = ops.paged_attention(q, k, v, table, n)
+        assert torch.equal(o, torch.full_like(o, 1.5))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_columns_of_one(dev):
+    """A table or lengths of one entry have no order that could be wrong."""
+    q, k, v, table, n, _ = _scene([9], 4, 2, 64, 16, dev)
+    t = torch.stack([table, table], -1)[:, :1, 0]
+    m = torch.stack([n, n], -1)[:, 0]
+    assert torch.equal(ops.paged_attention(q, k, v, t, m),
+                       ops.paged_attention(q, k, v, table, n))
 
 
 @pytest.mark.gpu
