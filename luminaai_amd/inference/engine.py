@@ -74,6 +74,15 @@ def sample_token(logits: torch.Tensor, cfg: GenerationConfig,
     return int(torch.multinomial(probs, 1))
 
 
+def check_tokens(sequences: List[List[int]], model):
+    """Raises ValueError for a token outside the model's embedding, which a GPU
+    would look up without asking."""
+    n = model.embed_tokens.num_embeddings
+    for s in sequences:
+        if len(s) and not 0 <= min(s) <= max(s) < n:
+            raise ValueError(f"a token is outside the vocabulary of {n}")
+
+
 class GenerationEngine:
     def __init__(self, model, tokenizer, device: Optional[torch.device] = None):
         self.model = model
@@ -407,8 +416,18 @@ class GenerationEngine:
         p = next(self.model.parameters())
         packed = not any(l.use_mod for l in self.model.layers) and \
             (self.device.type != "cuda" or p.dtype == torch.bfloat16)
+        check_tokens(sequences, self.model)
+        groups: List[List[List[int]]] = []
+        room = 0
+        for s in sequences:
+            # a forward over up to 32768 tokens, or one sequence
+            if not packed or len(s) > room:
+                groups.append([])
+                room = 32768
+            groups[-1].append(s)
+            room -= len(s)
         out: List[Dict] = []
-        for group in ([sequences] if packed else [[s] for s in sequences]):
+        for group in groups:
             flat = [t for s in group for t in s]
             if not flat:
                 out += [{"logprobs": [], "entropy": [], "top_ids": [],

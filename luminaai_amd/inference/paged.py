@@ -21,7 +21,7 @@ from typing import Callable, Dict, List, Optional, Sequence, Tuple
 import torch
 
 from .. import ops
-from .engine import GenerationConfig, sample_token
+from .engine import GenerationConfig, check_tokens, sample_token
 
 
 class _Step:
@@ -279,6 +279,8 @@ class PagedBatchingEngine:
         if self.device.type == "cuda" and p.dtype != torch.bfloat16:
             raise TypeError("paged serving on the GPU needs a bf16 model, got "
                             f"{p.dtype}")
+        if model.layers[0].attention.head_dim > 192:
+            raise ValueError("paged serving takes head_dim up to 192")
         self.model = model.eval()
         self.tokenizer = tokenizer
         self.max_batch = max_batch
@@ -335,6 +337,7 @@ class PagedBatchingEngine:
             raise RuntimeError("no free slot — poll can_admit first")
         ids = [p[-min(c.max_context, self.max_len - 1):] or [self._pad]
                for p, c in zip(prompts, cfgs)]
+        check_tokens(ids, self.model)
         caches, cu = self.cache.prefill(slots, [len(x) for x in ids])
         flat = [t for x in ids for t in x]
         try:
@@ -452,7 +455,8 @@ class PagedBatchingEngine:
         rows = [b for b in tok_of if self.slots[b].cfg.logprobs is not None]
         if not rows:
             return
-        k = max(self.slots[b].cfg.logprobs for b in rows)
+        k = min(max(self.slots[b].cfg.logprobs for b in rows),
+                self.last_logits.shape[-1])
         r = ops.token_logprobs(
             self.last_logits.index_select(
                 0, torch.tensor(rows).to(self.device)),

@@ -41,11 +41,24 @@ def _gen_config(body: Dict) -> GenerationConfig:
         cfg.repetition_penalty = float(body["repetition_penalty"])
     if "stop_token_ids" in body:
         cfg.stop_token_ids = list(body["stop_token_ids"])
-    if body.get("logprobs") is not None and body["logprobs"] is not False:
-        # completions: a number; chat: true with top_logprobs beside it
-        cfg.logprobs = int(body.get("top_logprobs", 0)
-                           if body["logprobs"] is True else body["logprobs"])
     return cfg
+
+
+def _paged_options(body: Dict, cfg: GenerationConfig, max_batch: int) -> int:
+    """Reads `n` and `logprobs` of a request to a paged server: sets
+    cfg.logprobs, returns n."""
+    n = 1 if body.get("n") is None else int(body["n"])
+    if not 1 <= n <= max_batch:
+        raise ValueError(f"n must be 1 to {max_batch}")
+    lp = body.get("logprobs")
+    if lp is not None and lp is not False:
+        # completions: a number; chat: true with top_logprobs beside it
+        cfg.logprobs = int(body.get("top_logprobs") or 0 if lp is True else lp)
+        if not 0 <= cfg.logprobs <= 64:
+            raise ValueError("logprobs must be 0 to 64")
+    if body.get("stream") and (n != 1 or cfg.logprobs is not None):
+        raise ValueError("a stream takes neither n nor logprobs")
+    return n
 
 
 class _DynamicBatcher:
@@ -251,10 +264,9 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
         _account(endpoint, len(out), t0)
         return out
 
-    def _answers(prompt_ids: List[int], cfg: GenerationConfig, body: Dict,
+    def _answers(prompt_ids: List[int], cfg: GenerationConfig, n: int,
                  endpoint: str = "completions") -> List:
-        """The request's `n` answers: (tokens, log probabilities or None)."""
-        n = int(body.get("n", 1))
+        """The request's n answers: (tokens, log probabilities or None)."""
         if serving != "paged":
             return [(_decode(prompt_ids, cfg, endpoint=endpoint), None)]
         t0 = time.perf_counter()
@@ -263,17 +275,14 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
         return [(t, lp if cfg.logprobs is not None else None)
                 for t, lp in outs]
 
-    def _refusal(body: Dict, cfg: GenerationConfig):
-        n = int(body.get("n", 1))
-        if (n != 1 or cfg.logprobs is not None) and serving != "paged":
-            return "n and logprobs need serving=\"paged\""
-        if not 1 <= n <= max_batch:
-            return f"n must be 1 to {max_batch}"
-        if cfg.logprobs is not None and not 0 <= cfg.logprobs <= 64:
-            return "logprobs must be 0 to 64"
-        if body.get("stream") and (n != 1 or cfg.logprobs is not None):
-            return "a stream takes neither n nor logprobs"
-        return None
+    def _options(body: Dict, cfg: GenerationConfig):
+        """(n, refusal); other modes take one answer and ignore both fields."""
+        if serving != "paged":
+            return 1, None
+        try:
+            return _paged_options(body, cfg, max_batch), None
+        except (TypeError, ValueError) as e:
+            return 1, JSONResponse({"error": str(e)}, status_code=400)
 
     def _sse_stream(prompt_ids: List[int], cfg: GenerationConfig,
                     wrap, endpoint: str = "completions") -> StreamingResponse:
@@ -328,15 +337,15 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
     def completions(body: Dict):
         prompt = body.get("prompt", "")
         cfg = _gen_config(body)
-        bad = _refusal(body, cfg)
-        if bad:
-            return JSONResponse({"error": bad}, status_code=400)
+        n, refusal = _options(body, cfg)
+        if refusal is not None:
+            return refusal
         ids = tokenizer.encode(prompt)
         if body.get("stream"):
             return _sse_stream(ids, cfg, lambda piece: {
                 "object": "text_completion.chunk",
                 "choices": [{"text": piece, "index": 0}]})
-        outs = _answers(ids, cfg, body)
+        outs = _answers(ids, cfg, n)
         n_out = sum(len(t) for t, _ in outs)
         choices = []
         for i, (toks, lps) in enumerate(outs):
@@ -363,9 +372,9 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
     def chat_completions(body: Dict):
         messages = body.get("messages", [])
         cfg = _gen_config(body)
-        bad = _refusal(body, cfg)
-        if bad:
-            return JSONResponse({"error": bad}, status_code=400)
+        n, refusal = _options(body, cfg)
+        if refusal is not None:
+            return refusal
         ids: List[int] = []
         for m in messages:
             ids.extend(tokenizer.encode_message(m.get("role", "user"),
@@ -377,7 +386,7 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
                 "object": "chat.completion.chunk",
                 "choices": [{"delta": {"content": piece}, "index": 0}]},
                 endpoint="chat")
-        outs = _answers(ids, cfg, body, endpoint="chat")
+        outs = _answers(ids, cfg, n, endpoint="chat")
         n_out = sum(len(t) for t, _ in outs)
         choices = []
         for i, (toks, lps) in enumerate(outs):

@@ -318,6 +318,37 @@ def test_logprobs_of_answers_equal_scores(small_model, tokenizer):
         assert e["top"][0][0] == e["token"]         # greedy
     with pytest.raises(ValueError, match="logprobs"):
         eng.admit([1, 2], _cfg(2, logprobs=65))
+    with pytest.raises(ValueError, match="outside the vocabulary"):
+        eng.admit([1, 512])
+    with pytest.raises(ValueError, match="outside the vocabulary"):
+        solo.score([[1], [-1, 2]])
+
+
+def test_scores_do_not_depend_on_the_batch(small_model, tokenizer):
+    """More than one forward's worth of sequences, and each alone."""
+    g = torch.Generator().manual_seed(0)
+    seqs = [torch.randint(1, 500, (n,), generator=g).tolist()
+            for n in (17, 2, 60)]
+    solo = GenerationEngine(small_model.eval(), tokenizer)
+    alone = [solo.score([s])[0]["logprobs"] for s in seqs]
+    many = solo.score(seqs * 420)                   # 33180 tokens
+    assert len(many) == 1260
+    for i, r in enumerate(many):
+        assert torch.allclose(torch.tensor(r["logprobs"]),
+                              torch.tensor(alone[i % 3]), atol=1e-4)
+
+
+def test_alternatives_of_a_small_vocabulary(tiny_config, tokenizer):
+    from luminaai_amd.models import (DeepSeekTransformer,
+                                     config_to_deepseek_config)
+    tiny_config.vocab_size = 40
+    m = DeepSeekTransformer(config_to_deepseek_config(tiny_config)).eval()
+    eng = _engine(m, tokenizer)
+    eng._pad = 0
+    b = eng.admit([1, 2, 3], _cfg(2, logprobs=64))
+    while eng.n_active():
+        eng.step()
+    assert [len(e["top"]) for e in eng.slots[b].logprobs] == [40, 40]
 
 
 def test_scores_one_by_one_for_mixture_of_depths(tiny_config, tokenizer):
@@ -354,13 +385,17 @@ def test_server_paged(small_model, tokenizer):
         "temperature": 0.0, "logprobs": True, "top_logprobs": 1}).json()
     assert all(len(e["top_logprobs"]) == 1
                for e in chat["choices"][0]["logprobs"]["content"])
-    for bad in ({"n": 9}, {"n": 0}, {"logprobs": 65},
-                {"n": 2, "stream": True}):
+    for bad in ({"n": 9}, {"n": 0}, {"n": "x"}, {"logprobs": 65},
+                {"logprobs": [1]}, {"n": 2, "stream": True}):
         assert client.post("/v1/completions",
                            json={**body, **bad}).status_code == 400
+    lines = client.post("/v1/completions", json={**body, "stream": True}).text
+    assert "text_completion.chunk" in lines
+    # other modes answer once, as they always did
     plain = TestClient(create_app(small_model.eval(), tokenizer, max_len=64))
-    assert plain.post("/v1/completions",
-                      json={**body, "n": 2}).status_code == 400
+    got = plain.post("/v1/completions",
+                     json={**body, "n": 2, "logprobs": 1}).json()
+    assert [c["text"] for c in got["choices"]] == [one["choices"][0]["text"]]
 
 
 # ------------------------------------------------------------ on the GPU
