@@ -496,7 +496,11 @@ void packed_fwd_kernel(const PackedArgs a) {
 
 // ===========================================================================
 // dQ, and delta for the next kernel: the forward's arrangement, with P from the
-// saved lse2. K's image serves S (rows) and dQ (columns).
+// saved lse2. K's image serves S (rows) and dQ (columns). 8192 tokens of 32:8
+// heads x 128: 390 us (770 TFLOP/s), of 12:4 x 159: 148, where the few long
+// blocks that end last cost a third; the keys of a block shared by two sets of
+// four waves in one workgroup took 188 and 467, since all eight then wait for
+// each other at every step.
 // ===========================================================================
 #define BW 4                   // waves
 #define BQ (32 * BW)
@@ -635,8 +639,9 @@ void packed_dq_kernel(const PackedArgs a) {
 // a step behind, with P handed over in LDS (fp32, as it lies in the
 // registers). Each then holds one accumulator and one of K and V, which leaves
 // two waves a SIMD for every head_dim, and one's exponentials run under the
-// other's products. One wave for all of it took 1015 us for 8192 tokens of 32:8
-// heads x 128 (410 registers, one wave a SIMD).
+// other's products: 546 us for 8192 tokens of 32:8 heads x 128 (735 TFLOP/s) and
+// 185 of 12:4 x 159. One wave for all of it took 1015 us for the former (410
+// registers, one wave a SIMD).
 //
 // Where T * HKV / BKV workgroups of uneven length would not fill the chip, a
 // group's heads are split over `splits` workgroups, whose fp32 results
@@ -754,10 +759,15 @@ void packed_dkdv_kernel(const PackedArgs a) {
       const char* ri = first ? qi : gi;        // rows, then columns
       const char* ci = first ? gi : qi;
       f32x16 s = zero16();
+      // products go before the other waves' exponentials (8192 tokens of 12:4 x
+      // 159: 190 -> 185 us, of 32:8 x 128: 556 -> 546; forward and dQ, whose
+      // waves are all of one kind, lose by it)
+      __builtin_amdgcn_s_setprio(1);
       #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
         s = mfma(rows.get(ri, ks), kvf[ks], s);
       reads_ahead<KS, 1>();
+      __builtin_amdgcn_s_setprio(0);
       float p[16];
       if (first) {
         #pragma unroll
@@ -792,9 +802,11 @@ void packed_dkdv_kernel(const PackedArgs a) {
       #pragma unroll
       for (int st = 0; st < 2; ++st) {
         const bf16x8 pf = pack_frag(&p[8 * st]);
+        __builtin_amdgcn_s_setprio(1);
         #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
           acc[dt] = mfma(cols.get(ci, 16 * st, dt), pf, acc[dt]);
+        __builtin_amdgcn_s_setprio(0);
       }
     }
     buf = buf == 2 ? 0 : buf + 1;
@@ -824,7 +836,8 @@ void packed_dkdv_kernel(const PackedArgs a) {
 }
 
 // Adds the splits' results in order, for the rows of the sequences. A thread
-// takes four channels of a row.
+// takes four channels of a row; bound by bytes (two parts of 8192 x 8 x 128 twice
+// over, 168 MB: 25 us, 6.7 TB/s, much of it from the last-level cache).
 __global__ __launch_bounds__(256)
 void packed_join_kernel(const PackedArgs a) {
   int end = a.B > 0 ? a.cu[a.B] : 0;
@@ -937,7 +950,7 @@ extern "C" hipError_t lumina_packed_attn_bwd(
 // [T, heads, .] at once; a thread moves 8 channels. Rows that start between 16
 // bytes cost the kernels above more than this copy: at D = 159 they took 563 us
 // together for 8192 tokens of 12:4 heads, and 430 at D = 160, while q, k, v and
-// dO are copied in 40.
+// dO are copied in 34.
 // ===========================================================================
 struct PackRowsArgs {
   const uint16_t* src[3];
