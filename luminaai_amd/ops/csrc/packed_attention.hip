@@ -990,7 +990,8 @@ extern "C" hipError_t lumina_pack_rows(const void* const* src, void* const* dst,
   a.T = T;
   a.D = D;
   a.pieces = (D + 7) / 8;
-  // few tokens: a workgroup each, so that the call has enough of them
+  // few tokens: a workgroup each, so that the call has enough of them. One / eight
+  // tokens a workgroup: 8192 tokens of 12:4:4 x 159 18.2 / 17.1 us.
   a.per = T >= 4096 ? 8 : 1;
   for (int i = 0; i < n; ++i) {
     a.src[i] = (const uint16_t*)src[i];
