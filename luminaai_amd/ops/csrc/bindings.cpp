@@ -819,7 +819,7 @@ at::Tensor paged_attn(const at::Tensor& q_, const at::Tensor& kp,
   // each of the 256 units, 16 waves) where there is that much, and no fewer
   // than 128 tokens (one step of each of its four waves), for the join's sake no
   // more than 1024. Twice and four times as many workgroups, and limits of 512 and
-  // 2048, measured the same within 2 % from one row of 2041 to 64 of 32690.
+  // 2048, measured alike from one row of 2041 to 64 of 32690.
   const int64_t G = H / HKV, rows = B * HKV * ((G + 15) / 16);
   int64_t chunk = 128;
   while (chunk < 1024 && rows * cap > chunk * 1024) chunk *= 2;

@@ -182,6 +182,36 @@ def test_trainer_takes_packed_batches(tiny_config, sample_conversations,
     assert math.isfinite(res["loss"])
 
 
+def _moe(cfg):
+    from luminaai_amd.models import (DeepSeekTransformer,
+                                     config_to_deepseek_config)
+    torch.manual_seed(0)
+    return DeepSeekTransformer(config_to_deepseek_config(cfg))
+
+
+def test_packed_moe(tiny_moe_config):
+    """Experts see the tokens of all sequences, which attend to themselves."""
+    m = _moe(tiny_moe_config).train()
+    g = torch.Generator().manual_seed(0)
+    ids = torch.randint(1, 500, (1, 30), generator=g)
+    cu = torch.tensor([0, 12, 30], dtype=torch.int32)
+    logits, aux, _ = m(ids, cu_seqlens=cu)
+    grads = torch.autograd.grad(logits.float().square().mean() + aux,
+                                list(m.parameters()), allow_unused=True)
+    assert all(x is None or bool(x.isfinite().all()) for x in grads)
+
+
+def test_paged_engine_with_quantized_moe(tiny_moe_config, tokenizer):
+    from luminaai_amd.ops.quant import quantize_model
+    m = _moe(tiny_moe_config).eval()
+    quantize_model(m, mode="int8", min_dim=32)
+    eng = _engine(m, tokenizer, max_batch=2)
+    outs = eng.run_to_completion([tokenizer.encode("quantized"),
+                                  tokenizer.encode("serving")], _cfg(4))
+    assert all(len(o) == 4 and all(isinstance(t, int) for t in o)
+               for o in outs)
+
+
 @pytest.mark.parametrize("cu", [[0, 3, 8], [5, 6, 8], [0, 9, 2, 5], [0, 99],
                                 [-40, 2, 8], [8, 8], [0]])
 def test_positions_index_inside_the_row(cu):
