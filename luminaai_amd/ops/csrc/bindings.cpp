@@ -76,8 +76,8 @@ hipError_t lumina_moe_dispatch_bwd(const void*, const int64_t*, void*, int64_t, 
 hipError_t lumina_moe_combine_fwd(const void*, const float*, const int64_t*, void*, int64_t, int, int, int64_t, int, hipStream_t);
 hipError_t lumina_moe_combine_bwd_y(const void*, const float*, const int64_t*, const int64_t*, const bool*, void*, int64_t, int64_t, int, int, hipStream_t);
 hipError_t lumina_moe_combine_bwd_w(const void*, const void*, const int64_t*, float*, int64_t, int, int, int64_t, int, hipStream_t);
-hipError_t lumina_packed_attn_fwd(const void*, const void*, const void*, void*, void*, float*, const int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
-hipError_t lumina_packed_attn_bwd(const void*, const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, float*, int, const int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_packed_attn_fwd(const void*, const void*, const void*, void*, void*, float*, const int*, int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_packed_attn_bwd(const void*, const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, float*, int, const int*, int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_pack_rows(const void* const*, void* const*, const int64_t*, const int*, int, int64_t, int, hipStream_t);
 hipError_t lumina_paged_attn(const void*, const void*, const void*, void*, const int*, const int*, float*, float*, const int64_t*, int64_t, int, int, int, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_paged_append(const void*, const void*, void*, void*, const int*, const int*, const int*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int, int, hipStream_t);
@@ -1041,6 +1041,13 @@ bool aligned_rows(const at::Tensor& t) {
          t.stride(0) <= (1 << 23) && (uintptr_t)t.data_ptr() % 16 == 0;
 }
 
+// Room for the blocks of more than 64 sequences (packed_list_kernel).
+at::Tensor block_list(const at::Tensor& cu, int64_t T) {
+  const int64_t B = cu.size(0) - 1;
+  if (B <= 64) return at::Tensor();
+  return at::empty({4 * (T / 128 + B + 2)}, cu.options());
+}
+
 // Those that are not become copies of head_dim rounded up to 8, zero past it;
 // all of them if one has to change its width.
 std::vector<at::Tensor> align_rows(std::vector<at::Tensor> ts) {
@@ -1097,7 +1104,7 @@ packed_attn_fwd(const at::Tensor& q_, const at::Tensor& k_,
   check_int32(cu, q_, 1, "cu_seqlens");
   TORCH_CHECK_VALUE(cu.size(0) >= 1, "cu_seqlens needs one entry more than "
                     "there are sequences");
-  // every workgroup looks for its rows in cu_seqlens
+  // one workgroup lists their blocks
   TORCH_CHECK_VALUE(cu.size(0) <= 65537, "at most 65536 sequences, got ",
                     cu.size(0) - 1);
   TORCH_CHECK_VALUE(scale > 1e-30 && scale < 1e30, "scale must be positive "
@@ -1109,13 +1116,16 @@ packed_attn_fwd(const at::Tensor& q_, const at::Tensor& k_,
   auto lse = at::empty({want_lse ? H : 0, T}, q.options().dtype(at::kFloat));
   auto rest = at::empty({want_lse ? T : 0, H, q.size(2)}, q.options());
   if (T == 0) return {o, rest, lse, q, k, v};
+  const at::Tensor list = block_list(cu, T);
   const int64_t strides[8] = {q.stride(0), q.stride(1), k.stride(0),
                               k.stride(1), v.stride(0), v.stride(1), 0, 0};
   check_hip(lumina_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                    o.data_ptr(),
                                    want_lse ? rest.data_ptr() : nullptr,
                                    want_lse ? lse.data_ptr<float>() : nullptr,
-                                   cu.data_ptr<int>(), strides, (int)T,
+                                   cu.data_ptr<int>(),
+                                   list.defined() ? list.data_ptr<int>()
+                                                  : nullptr, strides, (int)T,
                                    (int)cu.size(0) - 1, (int)H, (int)HKV,
                                    (int)q.size(2), (int)D, (float)scale,
                                    cur_stream()),
@@ -1151,6 +1161,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
   while (splits < G && (G % splits != 0 || splits * HKV * T < 131072)) ++splits;
   at::Tensor part;
   if (splits > 1) part = at::empty({2, splits, T, HKV, (D + 3) / 4 * 4}, lse.options());
+  const at::Tensor list = block_list(cu, T);
   const int64_t strides[8] = {q.stride(0), q.stride(1), k.stride(0),
                               k.stride(1), v.stride(0), v.stride(1),
                               go.stride(0), go.stride(1)};
@@ -1162,7 +1173,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
                                    dk.data_ptr(), dv.data_ptr(),
                                    splits > 1 ? part.data_ptr<float>()
                                               : nullptr, (int)splits,
-                                   cu.data_ptr<int>(), strides, (int)T,
+                                   cu.data_ptr<int>(),
+                                   list.defined() ? list.data_ptr<int>()
+                                                  : nullptr, strides, (int)T,
                                    (int)cu.size(0) - 1, (int)H, (int)HKV,
                                    (int)q.size(2), (int)D, (float)scale,
                                    cur_stream()),

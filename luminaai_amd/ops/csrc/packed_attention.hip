@@ -36,6 +36,7 @@ typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(2))) float floatx2;
 typedef __attribute__((ext_vector_type(2))) uint32_t uintx2;
+typedef __attribute__((ext_vector_type(4))) int intx4;
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 #define LOG2E 1.4426950408889634f
@@ -55,6 +56,7 @@ struct PackedArgs {
   float* lse;                  // [H, T], log2 units; +inf where nothing summed
   float* delta;                // [H, T]
   const int* cu;               // [B + 1]
+  const int* list;             // packed_list_kernel's blocks, or null
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, go_st, go_sh;
   int T, B, H, HKV, W, D;
   int splits;                  // parts of a group's heads in dK / dV
@@ -80,74 +82,154 @@ DEV_INLINE int wave_sum(int x) {
   return __builtin_amdgcn_readlane(x, 63);
 }
 
+// Start and length of sequence b. cu[0] counts as 0 and the rest is cut to [0, T],
+// so that no content of it leads outside the tensors; past the last one, 0.
+DEV_INLINE int sequence(const int* cu, int B, int T, int b, int& s) {
+  s = 0;
+  if (b >= B) return 0;
+  s = b ? cu[b] : 0;
+  s = s < 0 ? 0 : (s > T ? T : s);
+  int e = cu[b + 1];
+  e = e > T ? T : e;
+  return e > s ? e - s : 0;
+}
+
 // Block `id` of all sequences' blocks of `rows` rows, then the blocks of the
-// rows behind the last sequence. cu[0] counts as 0 and the rest is cut to [0, T],
-// so that no content of it leads outside the tensors. Every wave finds its block
-// by itself, from L2.
+// rows behind the last sequence. Every wave finds its block by itself, from L2.
 //
-// Up to 64 sequences: the blocks with the most work first, over all sequences,
-// so that the launch does not end with a few long ones. A sequence of n blocks
-// has one of each level 1 .. n, hence sum max(0, n - x + 1) blocks are of level
-// x or more, and the level is found by bisection. More sequences: one after the
-// other, each from its longest block on.
-DEV_INLINE Work find_work(const int* cu, int B, int T, int id, int rows) {
-  const int lane = threadIdx.x & 63;
+// The blocks with the most work come first, over all sequences, so that the
+// launch does not end with a few long ones. A sequence of n blocks has one of each
+// level 1 .. n, hence sum max(0, n - x + 1) blocks are of level x or more, and the
+// level is found by bisection. That holds for the 64 sequences of a wave; more of
+// them are listed beforehand by packed_list_kernel.
+DEV_INLINE Work find_work(const PackedArgs& a, int id, int rows) {
+  const int lane = threadIdx.x & 63, T = a.T;
   Work w = {0, 0, 0, -1};
-  int before = 0;
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    const int b = b0 + lane;
-    int s = 0, n = 0;
-    if (b < B) {
-      s = b ? cu[b] : 0;
-      s = s < 0 ? 0 : (s > T ? T : s);
-      int e = cu[b + 1];
-      e = e > T ? T : e;
-      n = e > s ? e - s : 0;
-    }
-    const int nb = (n + rows - 1) / rows;
-    const int all = wave_sum(nb);
-    if (id - before < all) {
-      int at = id - before, level, rank = at;
-      if (B <= 64) {
-        int lo = 1, hi = (T + rows - 1) / rows + 1, above = 0;
-        while (hi - lo > 1) {                // blocks of level lo or more: > at
-          const int mid = (lo + hi) >> 1;
-          const int more = wave_sum(nb >= mid ? nb - mid + 1 : 0);
-          if (more > at) {
-            lo = mid;
-          } else {
-            hi = mid;
-            above = more;
-          }
-        }
-        level = lo;
-        rank = at - above;                   // among the sequences that have it
-        unsigned long long has = __ballot(nb >= level);
-        for (int i = 0; i < rank; ++i) has &= has - 1;
-        rank = __builtin_ctzll(has | (1ull << 63));
-      } else {
-        int sum = nb;                        // inclusive prefix sum
-        #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const int x = __shfl_up(sum, o, 64);
-          if (lane >= o) sum += x;
-        }
-        at -= sum - nb;
-        rank = __builtin_ctzll(__ballot(at >= 0 && at < nb) | (1ull << 63));
-        level = __builtin_amdgcn_readlane(nb - at, rank);
-      }
-      w.start = __builtin_amdgcn_readlane(s, rank);
-      w.len = __builtin_amdgcn_readlane(n, rank);
-      w.level = level;
+  int all;
+  if (a.list) {
+    all = a.list[0];
+    if (id < all) {
+      const int* e = a.list + 4 + 4 * (int64_t)id;
+      w.start = e[0];
+      w.len = e[1];
+      w.level = e[2];
       return w;
     }
-    before += all;
+  } else {
+    int s;
+    const int n = sequence(a.cu, a.B, T, lane, s);
+    const int nb = (n + rows - 1) / rows;
+    all = wave_sum(nb);
+    if (id < all) {
+      int lo = 1, hi = (T + rows - 1) / rows + 1, above = 0;
+      while (hi - lo > 1) {                  // blocks of level lo or more: > id
+        const int mid = (lo + hi) >> 1;
+        const int more = wave_sum(nb >= mid ? nb - mid + 1 : 0);
+        if (more > id) {
+          lo = mid;
+        } else {
+          hi = mid;
+          above = more;
+        }
+      }
+      int rank = id - above;                 // among the sequences that have it
+      unsigned long long has = __ballot(nb >= lo);
+      for (int i = 0; i < rank; ++i) has &= has - 1;
+      rank = __builtin_ctzll(has | (1ull << 63));
+      w.start = __builtin_amdgcn_readlane(s, rank);
+      w.len = __builtin_amdgcn_readlane(n, rank);
+      w.level = lo;
+      return w;
+    }
   }
-  int end = B > 0 ? cu[B] : 0;
+  int end = a.B > 0 ? a.cu[a.B] : 0;
   end = end < 0 ? 0 : (end > T ? T : end);
-  const int64_t tail = end + (int64_t)(id - before) * rows;
+  const int64_t tail = end + (int64_t)(id - all) * rows;
   w.tail = tail < T ? (int)tail : T;
   return w;
+}
+
+// ===========================================================================
+// The blocks of more than 64 sequences, those with the most work first:
+// list[0] of them, entry i at list[4 + 4 i ..]: start, length, level. One
+// workgroup counts the blocks of each level in LDS and then gives each block
+// the next place of its level; levels from LEVELS on are not told apart. Places
+// are taken in no fixed order, which moves work between workgroups and changes no
+// result. Walking through cu in every workgroup instead, 16384 tokens of 32:8 heads
+// x 128 took, forward: in 65 sequences 111 us, with the list 110; in 256 142 and
+// 102; in 1024 533 and 312; in 16384 43.8 ms and 4.6.
+// ===========================================================================
+#define LEVELS 1024
+
+// inclusive sum over the 1024 threads of a workgroup
+DEV_INLINE int block_scan(int x, int* ws) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  #pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();                           // the last call's reads are done
+  if (lane == 63) ws[wave] = x;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) x += ws[i];
+  return x;
+}
+
+__global__ __launch_bounds__(LEVELS)
+void packed_list_kernel(const int* cu, int B, int T, int rows, int cap,
+                        int* list) {
+  __shared__ int at[LEVELS], ws[LEVELS / 64], top;
+  __shared__ unsigned long long total;
+  const int tid = threadIdx.x, lane = tid & 63;
+  at[tid] = 0;
+  if (tid == 0) {
+    total = 0;
+    top = 0;
+  }
+  __syncthreads();
+  for (int b0 = 0; b0 < B; b0 += LEVELS) {   // sequences by their blocks
+    int s;
+    const int n = sequence(cu, B, T, b0 + tid, s);
+    const int nb = (n + rows - 1) / rows;
+    if (nb > 0) atomicAdd(&at[(nb < LEVELS ? nb : LEVELS) - 1], 1);
+    if (nb >= LEVELS) atomicAdd(&top, nb - LEVELS + 1);
+    const int sum = wave_sum(nb);
+    if (lane == 0) atomicAdd(&total, (unsigned long long)sum);
+  }
+  __syncthreads();
+  // level LEVELS - tid: the sequences that have it, then the places before it
+  const int have = block_scan(at[LEVELS - 1 - tid], ws);
+  const int blocks = tid == 0 ? top : have;
+  const int first = block_scan(blocks, ws) - blocks;
+  __syncthreads();
+  at[LEVELS - 1 - tid] = first;
+  __syncthreads();
+  // borders that fall may make more blocks than there are rows for: none then
+  const bool ok = total <= (unsigned long long)cap;
+  if (tid == 0) list[0] = ok ? (int)total : 0;
+  if (!ok) return;
+  auto put = [&](int s, int n, int level) {
+    const int i = atomicAdd(&at[(level < LEVELS ? level : LEVELS) - 1], 1);
+    if (i >= 0 && i < cap)
+      *reinterpret_cast<intx4*>(list + 4 + 4 * (int64_t)i) =
+          intx4{s, n, level, 0};
+  };
+  for (int b0 = 0; b0 < B; b0 += LEVELS) {
+    int s;
+    const int n = sequence(cu, B, T, b0 + tid, s);
+    const int nb = (n + rows - 1) / rows;
+    for (int l = nb < 8 ? nb : 8; l > 0; --l) put(s, n, l);
+    unsigned long long big = __ballot(nb > 8);   // by their wave together
+    while (big) {
+      const int j = __builtin_ctzll(big);
+      big &= big - 1;
+      const int sj = __builtin_amdgcn_readlane(s, j);
+      const int nj = __builtin_amdgcn_readlane(n, j);
+      const int bj = __builtin_amdgcn_readlane(nb, j);
+      for (int l = 9 + lane; l <= bj; l += 64) put(sj, nj, l);
+    }
+  }
 }
 
 // Heads that share keys and values are given to one XCD (workgroups go round
@@ -373,7 +455,7 @@ void packed_fwd_kernel(const PackedArgs a) {
   constexpr int IMG = FK * Img<DP>::BYTES;
   __shared__ char lds[4 * IMG];              // [2][K image, V image]
   const int h = head_of(blockIdx.x % a.H, a.H);
-  const Work w = find_work(a.cu, a.B, a.T, blockIdx.x / a.H, FQ);
+  const Work w = find_work(a, blockIdx.x / a.H, FQ);
   if (w.tail >= 0) {
     zero_rows(a.out, a.H, h, a.D, w.tail, a.T, FQ);
     return;
@@ -518,7 +600,7 @@ void packed_dq_kernel(const PackedArgs a) {
   constexpr int OWN = GO_LDS ? 32 * Img<DP>::BYTES : 0;
   __shared__ char lds[4 * IMG + BW * OWN];
   const int h = head_of(blockIdx.x % a.H, a.H);
-  const Work w = find_work(a.cu, a.B, a.T, blockIdx.x / a.H, BQ);
+  const Work w = find_work(a, blockIdx.x / a.H, BQ);
   if (w.tail >= 0) {
     zero_rows(a.dq, a.H, h, a.D, w.tail, a.T, BQ);
     return;
@@ -663,7 +745,7 @@ void packed_dkdv_kernel(const PackedArgs a) {
   const int hk = head_of(id % a.HKV, a.HKV);
   id /= a.HKV;
   const int split = id % a.splits;
-  const Work w = find_work(a.cu, a.B, a.T, id / a.splits, BKV);
+  const Work w = find_work(a, id / a.splits, BKV);
   if (w.tail >= 0) {
     if (split == 0) {
       zero_rows(a.dk, a.HKV, hk, a.D, w.tail, a.T, BKV);
@@ -872,8 +954,22 @@ static int64_t max_blocks(const PackedArgs& a, int rows) {
   return a.T / rows + a.B + 1;
 }
 
+// Lists the blocks if there are more sequences than a wave has lanes.
+static hipError_t list_blocks(PackedArgs& a, int* list, int rows,
+                              hipStream_t stream) {
+  a.list = list;
+  if (!list) return hipSuccess;
+  const int64_t cap = max_blocks(a, rows);
+  packed_list_kernel<<<dim3(1), dim3(LEVELS), 0, stream>>>(
+      a.cu, a.B, a.T, rows, (int)cap, list);
+  HIP_CHECK_LAST();
+  return hipSuccess;
+}
+
 template <int DP>
-static hipError_t run_fwd(const PackedArgs& a, hipStream_t stream) {
+static hipError_t run_fwd(PackedArgs& a, int* list, hipStream_t stream) {
+  const hipError_t err = list_blocks(a, list, Fwd<DP>::Q, stream);
+  if (err != hipSuccess) return err;
   const int64_t n = max_blocks(a, Fwd<DP>::Q) * a.H;
   if (n > 0x7fffffff) return hipErrorInvalidValue;
   packed_fwd_kernel<DP><<<dim3((uint32_t)n), dim3(2 * Fwd<DP>::Q), 0,
@@ -883,7 +979,10 @@ static hipError_t run_fwd(const PackedArgs& a, hipStream_t stream) {
 }
 
 template <int DP>
-static hipError_t run_bwd(const PackedArgs& a, hipStream_t stream) {
+static hipError_t run_bwd(PackedArgs& a, int* list, hipStream_t stream) {
+  static_assert(BQ == BKV, "one list for both kernels");
+  const hipError_t err = list_blocks(a, list, BQ, stream);
+  if (err != hipSuccess) return err;
   const int64_t n = max_blocks(a, BQ) * a.H;
   if (n > 0x7fffffff) return hipErrorInvalidValue;
   packed_dq_kernel<DP><<<dim3((uint32_t)n), dim3(64 * BW), 0, stream>>>(a);
@@ -911,17 +1010,17 @@ static void fill(PackedArgs& a, const int64_t* st, const int* cu, int T, int B,
 }
 
 #define DISPATCH_DP(W, FN)                                                   \
-  if ((W) <= 64) return FN<64>(a, stream);                                   \
-  if ((W) <= 96) return FN<96>(a, stream);                                   \
-  if ((W) <= 128) return FN<128>(a, stream);                                 \
-  if ((W) <= 160) return FN<160>(a, stream);                                 \
-  if ((W) <= 192) return FN<192>(a, stream);                                 \
+  if ((W) <= 64) return FN<64>(a, list, stream);                                   \
+  if ((W) <= 96) return FN<96>(a, list, stream);                                   \
+  if ((W) <= 128) return FN<128>(a, list, stream);                                 \
+  if ((W) <= 160) return FN<160>(a, list, stream);                                 \
+  if ((W) <= 192) return FN<192>(a, list, stream);                                 \
   return hipErrorInvalidValue;
 
 extern "C" hipError_t lumina_packed_attn_fwd(
     const void* q, const void* k, const void* v, void* out, void* rest,
-    float* lse, const int* cu, const int64_t* strides, int T, int B, int H, int HKV, int W,
-    int D, float scale, hipStream_t stream) {
+    float* lse, const int* cu, int* list, const int64_t* strides, int T, int B,
+    int H, int HKV, int W, int D, float scale, hipStream_t stream) {
   PackedArgs a = {};
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
   a.out = (uint16_t*)out; a.rest = (uint16_t*)rest; a.lse = lse;
@@ -931,9 +1030,10 @@ extern "C" hipError_t lumina_packed_attn_fwd(
 
 extern "C" hipError_t lumina_packed_attn_bwd(
     const void* q, const void* k, const void* v, const void* o,
-    const void* rest, const void* go, const float* lse, float* delta, void* dq, void* dk, void* dv, float* part,
-    int splits, const int* cu, const int64_t* strides, int T, int B, int H,
-    int HKV, int W, int D, float scale, hipStream_t stream) {
+    const void* rest, const void* go, const float* lse, float* delta, void* dq,
+    void* dk, void* dv, float* part, int splits, const int* cu, int* list,
+    const int64_t* strides, int T, int B, int H, int HKV, int W, int D,
+    float scale, hipStream_t stream) {
   PackedArgs a = {};
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
   a.o = (const uint16_t*)o; a.go = (const uint16_t*)go;

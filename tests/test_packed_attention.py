@@ -291,6 +291,28 @@ def test_as_many_sequences_as_are_taken(dev):
     _check(got, *_oracle(q, k, v, go, [n for n in lens if n], 64 ** -0.5))
 
 
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("D", [64, 192])
+def test_more_sequences_than_lanes(dev, D):
+    """Many sequences of one block, a few of many, empty ones between them."""
+    lens = [(7 * b) % 23 for b in range(75)]
+    lens[3], lens[70], lens[74] = 1300, 129, 257
+    q, k, v, go = _inputs(lens, 9, 2, 1, D, dev)
+    _check(_run(q, k, v, go, _cu(lens, dev)),
+           *_oracle(q, k, v, go, lens, D ** -0.5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[131200, 1, 60, 0, 300], [5, 700, 0, 2000]])
+def test_listed_blocks_give_the_same_bits(lens):
+    """The same sequences with empty ones behind them, past 64, and past the
+    levels that the list tells apart."""
+    q, k, v, go = _inputs(lens, 3, 2, 1, 64, "cuda")
+    a = _run(q, k, v, go, _cu(lens, "cuda"))
+    b = _run(q, k, v, go, _cu(lens + [0] * 70, "cuda"))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_border_refusals_on_the_cpu():
     q, k, v, _ = _inputs([6], 0, 4, 2, 64, "cpu")
     for cu in ([0, 7], [1, 6], [0, 4, 2]):
@@ -368,7 +390,8 @@ def test_borders_out_of_range_stay_inside():
     q, k, v, go = _inputs([T], 0, H, HKV, D, "cuda")
     room[T:2 * T] = q
     for cu in ([0, 10 ** 9], [-50, 64], [5, 20, 64], [0, 40, 20, 64],
-               [0, -1, 64]):
+               [0, -1, 64], [0, 64] * 50, [5] * 90 + [100], [64, 0] * 50,
+               [-9, 2 ** 31 - 1] * 50, list(range(200, 0, -1))):
         c = torch.tensor(cu, dtype=torch.int32, device="cuda")
         _run(room[T:2 * T], k, v, go, c)
     torch.cuda.synchronize()
