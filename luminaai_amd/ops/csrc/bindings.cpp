@@ -79,7 +79,7 @@ hipError_t lumina_moe_combine_bwd_w(const void*, const void*, const int64_t*, fl
 hipError_t lumina_packed_attn_fwd(const void*, const void*, const void*, void*, void*, float*, const int*, int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_packed_attn_bwd(const void*, const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, float*, int, const int*, int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_pack_rows(const void* const*, void* const*, const int64_t*, const int*, int, int64_t, int, hipStream_t);
-hipError_t lumina_paged_attn(const void*, const void*, const void*, void*, const int*, const int*, float*, float*, const int64_t*, int64_t, int, int, int, int, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_paged_attn(const void*, const void*, const void*, void*, const int*, const int*, float*, float*, int*, const int64_t*, int64_t, int, int, int, int, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_paged_append(const void*, const void*, void*, void*, const int*, const int*, const int*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int, int, hipStream_t);
 hipError_t lumina_copy_pages(void* const*, int, const int64_t*, const int64_t*, int, int64_t, const int*, const int*, int64_t, hipStream_t);
 hipError_t lumina_logprob_fwd(const void*, int, const void*, int, float*, float*, float*, float*, int64_t*, int64_t, int, int64_t, int, int64_t, hipStream_t);
@@ -810,37 +810,43 @@ at::Tensor paged_attn(const at::Tensor& q_, const at::Tensor& kp,
                     "block_table and seq_lens need a row for each of the ", B,
                     " sequences");
   const int64_t M = table.size(1), cap = M << shift;
-  TORCH_CHECK_VALUE(cap < (1ll << 31) - 4096, "block_table holds ", cap,
-                    " tokens: fewer than 2^31 - 4096 are supported");
+  TORCH_CHECK_VALUE(cap < (1 << 29), "a row of block_table holds ", cap,
+                    " tokens: fewer than 2^29 are supported");
   auto o = at::empty({B, H, D}, q.options());
   if (B == 0) return o;
   if (cap == 0 || kp.size(0) == 0) return o.zero_();
-  // Chunks of the context, a workgroup each: about 1024 workgroups (four on
-  // each of the 256 units, 16 waves) where there is that much, and no fewer
-  // than 128 tokens (one step of each of its four waves), for the join's sake no
-  // more than 1024. Twice and four times as many workgroups, and limits of 512 and
-  // 2048, measured alike from one row of 2041 to 64 of 32690.
-  const int64_t G = H / HKV, rows = B * HKV * ((G + 15) / 16);
-  int64_t chunk = 128;
-  while (chunk < 1024 && rows * cap > chunk * 1024) chunk *= 2;
-  const int64_t S = (cap + chunk - 1) / chunk;
-  at::Tensor ws;
+  // Workgroups wanted for all chunks together: 512 (two of the three that a unit
+  // holds), until a chunk has 1024 tokens, then up to 4096 of them, as far as the
+  // table has room for that much; the kernel sets the chunks' length by it. 512 /
+  // 768 / 1024 at first: 8 rows of up to 4096 tokens 16.3 / 16.4 / 19.8 us, 64 of
+  // 1000 44.7 / 52.4 / 50.8, one of 30000 28 / 30 / 32 (32:8 heads x 128). 1024 /
+  // 2048 / 4096 for long ones: 64 rows of up to 32690 tokens 802 / 767 / 754.
+  const int64_t R = HKV * ((H / HKV + 15) / 16), steps = (cap + 127) / 128;
+  TORCH_CHECK_VALUE(B * steps <= (1 << 24), "block_table holds ", B * cap,
+                    " tokens: up to 2^31 are supported");
+  const int64_t few = std::max<int64_t>(1, 512 / R);
+  const int64_t many = std::max(few, std::min(4096 / R, B * steps / 8));
+  const int64_t chunks = std::min(many + B + 1, B * steps + B);
+  at::Tensor ws, where;
   float* part = nullptr;
   float* ml = nullptr;
-  if (S > 1) {
-    ws = at::empty({B * H * S * (D + 2)}, q.options().dtype(at::kFloat));
+  int* wh = nullptr;
+  if (steps > 1) {
+    ws = at::empty({chunks * H * (D + 2)}, q.options().dtype(at::kFloat));
     ml = ws.data_ptr<float>();
-    part = ml + B * H * S * 2;
+    part = ml + chunks * H * 2;
+    where = at::empty({B, 2}, lens.options());
+    wh = where.data_ptr<int>();
   }
   const int64_t strides[9] = {q.stride(0), q.stride(1), kp.stride(0),
                               kp.stride(1), kp.stride(2), vp.stride(0),
                               vp.stride(1), vp.stride(2), table.stride(0)};
   check_hip(lumina_paged_attn(q.data_ptr(), kp.data_ptr(), vp.data_ptr(),
                               o.data_ptr(), table.data_ptr<int>(),
-                              lens.data_ptr<int>(), part, ml, strides,
+                              lens.data_ptr<int>(), part, ml, wh, strides,
                               kp.size(0), (int)B, (int)H, (int)HKV, (int)D,
-                              (int)kp.size(3), shift, (int)M, (int)chunk,
-                              (int)S, (float)scale, cur_stream()),
+                              (int)kp.size(3), shift, (int)M, (int)few, (int)many,
+                              (int)chunks, (float)scale, cur_stream()),
             "paged_attention");
   return o;
 }

@@ -65,6 +65,22 @@ DEV_INLINE uintx4 load8_ragged(const uint16_t* row, int c, int D) {
   return v;
 }
 
+// inclusive sum over the wave's lanes up to this one
+DEV_INLINE int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // row_bcast
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);
+  return x;
+}
+
+// sum over the wave, the same in every lane
+DEV_INLINE int wave_sum(int x) {
+  return __builtin_amdgcn_readlane(wave_scan(x), 63);
+}
+
 // generic element accessors so kernels template over T in {float, bf16-as-u16}
 struct F32Elem {
   using storage = float;

@@ -71,17 +71,6 @@ struct Work {
   int tail;                    // >= 0: rows behind the last sequence start here
 };
 
-// sum over the wave, the same in every lane
-DEV_INLINE int wave_sum(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // row_bcast
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);
-  return __builtin_amdgcn_readlane(x, 63);
-}
-
 // Start and length of sequence b. cu[0] counts as 0 and the rest is cut to [0, T],
 // so that no content of it leads outside the tensors; past the last one, 0.
 DEV_INLINE int sequence(const int* cu, int B, int T, int b, int& s) {

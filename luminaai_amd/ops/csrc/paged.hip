@@ -42,14 +42,20 @@ DEV_INLINE uint32_t pack_bf16(float lo, float hi) {
 // mantissa): the matrix pipe is idle anyway, and the result's error is
 // that of its own rounding.
 //
-// Work is split over the context in chunks of `chunk` tokens; a sequence that
-// fits one chunk is finished here, the others are joined by
-// paged_attn_join_kernel in the order of their chunks.
+// Work is split over the contexts in chunks of a length that follows from the sum
+// of the lengths, so that the wanted number comes out however wide the table is:
+// chunk c of all sequences goes to workgroups c HKV HG .., without gaps. The
+// hardware deals workgroups out to the units in turn, and gaps in a regular
+// pattern leave units idle: with a fixed number of chunks a sequence, 64 rows of
+// 1000 tokens took 83 us in a table of 4096 columns and 124 in one of 131072, and
+// take 45 in any; 8 rows 16 and 35, now 12. A sequence that fits one chunk is
+// finished here, the others are joined by paged_attn_join_kernel in the order of
+// their chunks.
 //
 // Measured, join included: 64 rows of 32:8 heads x 128 with 1001 .. 32690 tokens,
-// 4.4 GB: 760 us, 5.8 TB/s (a large copy moves 5.1). Small calls wait for a chain
-// of loads (length, page number, K and V) and for the second launch: eight rows of
-// up to 4096 tokens, 52 MB: 18.4 us; one of 2041 with 12:4 x 159, 5 MB: 10.0, of
+// 4.4 GB: 756 us, 5.8 TB/s (a large copy moves 5.1). Small calls wait for a chain
+// of loads (lengths, page number, K and V) and for the second launch: eight rows of
+// up to 4096 tokens, 52 MB: 16.3 us; one of 2041 with 12:4 x 159, 5 MB: 10.3, of
 // which the join takes 2.8.
 // ===========================================================================
 struct PagedAttnArgs {
@@ -59,19 +65,43 @@ struct PagedAttnArgs {
   uint16_t* o;
   const int* table;
   const int* lens;
-  float* part;                 // [B, H, S, D] unnormalised partial outputs
-  float* ml;                   // [B, H, S, 2] their maximum and sum
+  float* part;                 // [chunks, H, D] unnormalised partial outputs
+  float* ml;                   // [chunks, H, 2] their maximum and sum
   int64_t q_sb, q_sh;          // strides in elements
   int64_t k_sp, k_sh, k_st;
   int64_t v_sp, v_sh, v_st;
   int64_t table_sb;
   int64_t P;
-  int B, H, HKV, D, W, page_shift, M, chunk, S, HG;
+  int B, H, HKV, D, W, page_shift, M, HG;
+  int2* where;                 // [B] a sequence's first chunk and how many
+  float inv_few, inv_many;     // 1 / the chunks wanted, see steps_of_chunk
   float scale2;                // scale * log2(e)
 };
 
 DEV_INLINE int clampi(int x, int lo, int hi) {
   return x < lo ? lo : (x > hi ? hi : x);
+}
+
+// a length longer than the table's row is cut to it
+DEV_INLINE int length_of(const PagedAttnArgs& a, int b) {
+  return b < a.B ? clampi(a.lens[b], 0, a.M << a.page_shift) : 0;
+}
+
+// Steps (128 tokens, 32 for each of the four waves) of a chunk, for the sum of the
+// sequences' steps: more than all / few, but where that passes 8 only as much
+// more than 8 as exceeds all / many. Hence there are no more than many + B chunks,
+// an empty sequence's one among them.
+DEV_INLINE int steps_of_chunk(const PagedAttnArgs& a, int all) {
+  const int few = (int)((float)all * a.inv_few) + 1;
+  const int many = (int)((float)all * a.inv_many) + 1;
+  return few <= 8 ? few : clampi(many, 8, 1 << 22);     // 2^29 tokens: a row
+}
+
+// steps / n upwards and at least 1, inv = 1 / n. Rounding may make it one more
+// than that, and the last chunk empty.
+DEV_INLINE int chunks_of(int steps, int n, float inv) {
+  const int q = (int)((float)steps * inv);
+  return q * n < steps || q == 0 ? q + 1 : q;
 }
 
 template <int NDW>             // W <= 32 * NDW
@@ -82,25 +112,41 @@ void paged_attn_kernel(const PagedAttnArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.H / a.HKV;
 
-  // workgroup -> (sequence, chunk, kv head, group of 16 heads); neighbours
-  // share a chunk's pages
-  int64_t id = blockIdx.x;
-  const int hg = (int)(id % a.HG);
-  id /= a.HG;
-  const int hkv = (int)(id % a.HKV);
-  id /= a.HKV;
-  const int split = (int)(id % a.S);
-  const int b = (int)(id / a.S);
+  // workgroup -> (chunk of all sequences, kv head, group of 16 heads);
+  // neighbours share a chunk's pages
+  const uint32_t hg = blockIdx.x % (uint32_t)a.HG;
+  const uint32_t rest = blockIdx.x / (uint32_t)a.HG;
+  const int hkv = (int)(rest % (uint32_t)a.HKV);
+  const int item = (int)(rest / (uint32_t)a.HKV);
 
-  // a length longer than the table's row is cut to it
-  const int cap = a.M << a.page_shift;
-  const int len = clampi(a.lens[b], 0, cap);
-  const int t_begin = split * a.chunk;
-  if (t_begin >= len && split > 0) return;
-  const int t_end = len < t_begin + a.chunk ? len : t_begin + a.chunk;
+  int steps = 0;
+  for (int i = lane; i < a.B; i += 64) steps += (length_of(a, i) + 127) >> 7;
+  const int per = steps_of_chunk(a, wave_sum(steps)), chunk = 128 * per;
+  const float inv = 1.f / (float)per;
+  int b = -1, len = 0, split = 0, count = 0, before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int n = length_of(a, b0 + lane);
+    const int c = b0 + lane < a.B ? chunks_of((n + 127) >> 7, per, inv) : 0;
+    const int upto = before + wave_scan(c);
+    const unsigned long long more = __ballot(upto > item);
+    if (more) {
+      const int j = __builtin_ctzll(more);
+      b = b0 + j;
+      len = __builtin_amdgcn_readlane(n, j);
+      count = __builtin_amdgcn_readlane(c, j);
+      split = item - (__builtin_amdgcn_readlane(upto, j) - count);
+      break;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  if (b < 0) return;                         // fewer chunks than there could be
+  if (a.where && split == 0 && hkv == 0 && hg == 0 && threadIdx.x == 0)
+    a.where[b] = int2{item, count};
+  const int t_begin = split * chunk;
+  const int t_end = len - t_begin < chunk ? len : t_begin + chunk;
 
   const int g = lane >> 4, c16 = lane & 15;
-  const int gh = hg * 16 + c16;            // this lane's head in the group
+  const int gh = (int)hg * 16 + c16;       // this lane's head in the group
   const bool head_ok = gh < G;
   const int h = hkv * G + (head_ok ? gh : 0);
 
@@ -241,7 +287,7 @@ void paged_attn_kernel(const PagedAttnArgs a) {
   // ---- join the four waves: LDS holds [wave][head of 16][2 + D]
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  const int nh = G - hg * 16 < 16 ? G - hg * 16 : 16;
+  const int nh = G - (int)hg * 16 < 16 ? G - (int)hg * 16 : 16;
   const int rowf = a.D + 2;
   if (c16 < nh) {
     float* row = lds + ((int64_t)wave * nh + c16) * rowf;
@@ -270,16 +316,17 @@ void paged_attn_kernel(const PagedAttnArgs a) {
       ls += f * lds[(w * nh + hh) * rowf + 1];
       os += f * lds[(w * nh + hh) * rowf + 2 + d];
     }
-    const int head = hkv * G + hg * 16 + hh;
-    const int64_t bh = (int64_t)b * a.H + head;
-    if (len <= a.chunk) {
+    const int head = hkv * G + (int)hg * 16 + hh;
+    if (count == 1) {
       // an empty sequence gives zeros
-      a.o[bh * a.D + d] = f32_to_bf16(ls == 0.f ? 0.f : os / ls);
+      a.o[((int64_t)b * a.H + head) * a.D + d] =
+          f32_to_bf16(ls == 0.f ? 0.f : os / ls);
     } else {
-      a.part[(bh * a.S + split) * a.D + d] = os;
+      const int64_t at = (int64_t)item * a.H + head;
+      a.part[at * a.D + d] = os;
       if (d == 0) {
-        a.ml[(bh * a.S + split) * 2] = mm;
-        a.ml[(bh * a.S + split) * 2 + 1] = ls;
+        a.ml[at * 2] = mm;
+        a.ml[at * 2 + 1] = ls;
       }
     }
   }
@@ -295,12 +342,14 @@ void paged_attn_join_kernel(const PagedAttnArgs a) {
   constexpr int U = 4;
   const int64_t bh = blockIdx.x;
   const int b = (int)(bh / a.H);
-  const int len = clampi(a.lens[b], 0, a.M << a.page_shift);
-  if (len <= a.chunk) return;                  // finished by its only chunk
-  const int n = (len + a.chunk - 1) / a.chunk;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const float* ml = a.ml + bh * a.S * 2;
-  const float* part = a.part + bh * a.S * a.D;
+  const int2 at = a.where[b];
+  const int n = at.y;
+  if (n == 1) return;                          // finished by its only chunk
+  const int64_t first = (int64_t)at.x * a.H + (bh - (int64_t)b * a.H);
+  const float* ml = a.ml + first * 2;
+  const float* part = a.part + first * a.D;
+  const int64_t step = a.H;                    // from chunk to chunk
   float m = -FLT_MAX, l = 0.f, acc[3] = {0.f, 0.f, 0.f};
   for (int s0 = wave; s0 < n; s0 += 4 * U) {
     float cm[U], cl[U], x[U][3];
@@ -308,13 +357,13 @@ void paged_attn_join_kernel(const PagedAttnArgs a) {
     for (int u = 0; u < U; ++u) {
       // past the end the last one again, with weight 0
       const bool ok = s0 + 4 * u < n;
-      const int s = ok ? s0 + 4 * u : n - 1;
+      const int64_t s = step * (ok ? s0 + 4 * u : n - 1);
       cm[u] = ml[2 * s];
       cl[u] = ml[2 * s + 1];
       #pragma unroll
       for (int i = 0; i < 3; ++i) {
         const int d = lane + 64 * i;
-        x[u][i] = d < a.D ? part[(int64_t)s * a.D + d] : 0.f;
+        x[u][i] = d < a.D ? part[s * a.D + d] : 0.f;
       }
       if (!ok) cm[u] = -INFINITY;
     }
@@ -360,9 +409,10 @@ void paged_attn_join_kernel(const PagedAttnArgs a) {
 
 extern "C" hipError_t lumina_paged_attn(
     const void* q, const void* k, const void* v, void* o, const int* table,
-    const int* lens, float* part, float* ml, const int64_t* strides, int64_t P,
-    int B, int H, int HKV, int D, int W, int page_shift, int M, int chunk,
-    int S, float scale, hipStream_t stream) {
+    const int* lens, float* part, float* ml, int* where,
+    const int64_t* strides, int64_t P, int B, int H, int HKV, int D, int W,
+    int page_shift, int M, int few, int many, int chunks, float scale,
+    hipStream_t stream) {
   PagedAttnArgs a;
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
   a.o = (uint16_t*)o; a.table = table; a.lens = lens; a.part = part; a.ml = ml;
@@ -371,11 +421,12 @@ extern "C" hipError_t lumina_paged_attn(
   a.v_sp = strides[5]; a.v_sh = strides[6]; a.v_st = strides[7];
   a.table_sb = strides[8];
   a.P = P; a.B = B; a.H = H; a.HKV = HKV; a.D = D; a.W = W;
-  a.page_shift = page_shift; a.M = M; a.chunk = chunk; a.S = S;
+  a.page_shift = page_shift; a.M = M;
+  a.where = (int2*)where; a.inv_few = 1.f / few; a.inv_many = 1.f / many;
   const int G = H / HKV;
   a.HG = (G + 15) / 16;
   a.scale2 = scale * LOG2E;
-  const int64_t blocks = (int64_t)B * S * HKV * a.HG;
+  const int64_t blocks = (int64_t)chunks * HKV * a.HG;
   if (blocks > 0x7fffffff || (int64_t)B * H > 0x7fffffff)
     return hipErrorInvalidValue;
   const int nh = G < 16 ? G : 16;
@@ -391,7 +442,7 @@ extern "C" hipError_t lumina_paged_attn(
     default: return hipErrorInvalidValue;
   }
   HIP_CHECK_LAST();
-  if (S > 1) {
+  if (part) {
     paged_attn_join_kernel<<<dim3((uint32_t)((int64_t)B * H)), block, 0,
                              stream>>>(a);
     HIP_CHECK_LAST();

@@ -322,6 +322,21 @@ def test_huge_scores(dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("lens", [
+    [(37 * b) % 200 for b in range(130)], [0] * 64 + [900],
+    [900] + [0] * 70 + [1, 300], [128, 129, 256, 257, 1023, 1024, 1025]])
+def test_rows_and_widths(dev, lens):
+    """More rows than lanes, empty ones among them; however wide the table is,
+    the result is the same."""
+    q, k, v, table, n, dense = _scene(lens, 4, 2, 64, 16, dev)
+    o, tol = _oracle(q, dense, 64)
+    wide = torch.nn.functional.pad(table, (0, 3000 - table.shape[1]), value=-1)
+    for t in (table, wide):
+        got = ops.paged_attention(q, k, v, t, n).double().cpu()
+        assert ((got - o).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_columns_of_one(dev):
     """A table or lengths of one entry have no order that could be wrong."""
     q, k, v, table, n, _ = _scene([9], 4, 2, 64, 16, dev)
@@ -340,6 +355,11 @@ def test_gpu_refusals():
         ops.paged_attention(q, k, v, table.cpu(), n)
     with pytest.raises(ValueError, match="k_pages is on cpu"):
         ops.paged_attention(q, k.cpu(), v, table, n)
+    for rows, cols in ((1, 2 ** 25), (2 ** 10, 2 ** 18)):
+        far = table.new_zeros(1, cols).expand(rows, cols)
+        with pytest.raises(ValueError, match="2\\^29|2\\^31"):
+            ops.paged_attention(q[:1].expand(rows, 4, 64), k, v, far,
+                                n[:1].repeat(rows))
     with pytest.raises(ValueError, match="16-byte aligned"):
         odd = torch.zeros(k.numel() + 1, dtype=k.dtype,
                           device="cuda")[1:].view(k.shape)
