@@ -16,8 +16,11 @@
 // largest logit (a little less will do), so only the elements of threads whose own
 // maximum reaches it are looked at again (from L2); the candidates go to LDS, where
 // each is ranked by counting. Ties go to the lowest index: value and index make one
-// 64-bit key. Rows with more candidates than fit (many equal logits) take k rounds
-// of a maximum over the row. Eight rows of 50304 in fp32 with 20 alternatives take
+// 64-bit key. More candidates than fit mean many equal logits, a mask's usually:
+// then the bound is made exact, and what lies above it is taken with the first of
+// those equal to it (eight rows of five tokens beside a mask, 20 alternatives: 19
+// us). If that does not fit either, k rounds of a maximum over the row are taken
+// (368 us there). Eight rows of 50304 in fp32 with 20 alternatives take
 // 10.8 us: few rows wait for one row's chain of reductions, not for bytes.
 #include "common.h"
 
@@ -122,7 +125,7 @@ void logprob_fwd_kernel(const LogprobArgs a) {
   __shared__ float gmax[TOP ? NW : 1][64];
   __shared__ uint64_t cand[TOP ? LP_CAP : 1];
   __shared__ uint64_t best[NW];
-  __shared__ int n_cand;
+  __shared__ int n_cand, equals[NW];
   __shared__ float thr;
 
   const int64_t row = blockIdx.x;
@@ -216,22 +219,23 @@ void logprob_fwd_kernel(const LogprobArgs a) {
   }
   if (!TOP) return;
 
-  if (wave == 0) {
+  // the order key's upper bits, from bit `last` on, of the k-th largest group
+  // maximum, by bisection; at least k of them are that or more
+  auto bound = [&](int last) {
     float g = gmax[0][lane];
     #pragma unroll
     for (int w = 1; w < NW; ++w) g = fmaxf(g, gmax[w][lane]);
-    // T: the upper half of the order key of the k-th largest maximum, by
-    // bisection over its bits; at least k of them are T or more
     const uint32_t key = order_key(g);
     uint32_t lo = 0;
     #pragma unroll
-    for (int bit = 31; bit >= 16; --bit) {
+    for (int bit = 31; bit >= last; --bit) {
       const uint32_t mid = lo | (1u << bit);
       if (__builtin_popcountll(__ballot(key >= mid)) >= a.k) lo = mid;
     }
     if (lane == 0)                         // keys below -inf's are no numbers
       thr = lo < 0x007fffffu ? -INFINITY : from_order_key(lo);
-  }
+  };
+  if (wave == 0) bound(16);
   __syncthreads();
   const float T = thr;
   // Threads whose maximum reaches T (or that met a NaN) have their vectors looked
@@ -245,14 +249,15 @@ void logprob_fwd_kernel(const LogprobArgs a) {
       if (hits && lane >> 4 == u) owner = wave * 64 + __builtin_ctzll(hits);
       hits &= hits - 1;                      // 0 & -1 stays 0
     }
-    if (owner < 0) continue;
-    for (int q = owner + (lane & 15) * BLOCK; q < nvec; q += 16 * BLOCK) {
+    int at = 0;
+    for (int q = owner < 0 ? nvec : owner + (lane & 15) * BLOCK; q < nvec;
+         q += 16 * BLOCK) {
       const Vec8<S> v = load8(x + 8 * (int64_t)q);
       int n = 0;
       #pragma unroll
       for (int j = 0; j < 8; ++j) n += E::get(v.v[j]) < T ? 0 : 1;
       if (n == 0) continue;
-      int at = atomicAdd(&n_cand, n);
+      at = atomicAdd(&n_cand, n);
       #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float f = E::get(v.v[j]);
@@ -262,6 +267,7 @@ void logprob_fwd_kernel(const LogprobArgs a) {
         }
       }
     }
+    if (__any(at > LP_CAP)) hits = 0;        // they do not fit, see below
   }
   if (tail < a.V && threadIdx.x < 8) {
     const float f = E::get(x[tail]);
@@ -276,7 +282,49 @@ void logprob_fwd_kernel(const LogprobArgs a) {
     a.top_lp[row * a.k + rank] =
         from_order_key((uint32_t)(key >> 32)) - r.m - LN2 * ls;
   };
-  const int n = n_cand;
+  int n = n_cand;
+  if (n > LP_CAP) {
+    __syncthreads();                       // all have read it
+    if (threadIdx.x == 0) n_cand = 0;
+    if (wave == 0) bound(0);
+    __syncthreads();
+    const float B = thr;
+    auto keep = [&](float f, int idx) {
+      const int at = atomicAdd(&n_cand, 1);
+      if (at < LP_CAP) cand[at] = pair_key(f, idx);
+    };
+    if (!(mx <= B))
+      for (int q = threadIdx.x; q < nvec; q += BLOCK) {
+        const Vec8<S> v = load8(x + 8 * (int64_t)q);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!(E::get(v.v[j]) <= B)) keep(E::get(v.v[j]), 8 * q + j);
+      }
+    if (tail < a.V && threadIdx.x < 8 && !(E::get(x[tail]) <= B))
+      keep(E::get(x[tail]), tail);
+    __syncthreads();
+    const int strict = n_cand;
+    n = strict;
+    // fewer than k above it: then the k-th is equal to it, and the first of its
+    // equals fill up, in order
+    for (int q0 = 0; n < a.k && q0 < a.V; q0 += BLOCK) {
+      const int q = q0 + threadIdx.x;
+      const bool eq = q < a.V && E::get(x[q]) == B;
+      const unsigned long long who = __ballot(eq);
+      __syncthreads();                     // the last round's counts are read
+      if (lane == 0) equals[wave] = __builtin_popcountll(who);
+      __syncthreads();
+      int at = n + __builtin_popcountll(who & ((1ull << lane) - 1));
+      #pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        if (w < wave) at += equals[w];
+        n += equals[w];
+      }
+      if (eq && at < a.k) cand[at] = pair_key(B, q);
+    }
+    if (strict < a.k && n > a.k) n = a.k;
+    __syncthreads();
+  }
   if (n <= LP_CAP) {
     // a wave ranks a candidate: 64 comparisons at once
     for (int c = wave; c < n; c += NW) {

@@ -245,6 +245,32 @@ def test_refusals(dev):
         ops.token_logprobs(x[:, :0], tok)
 
 
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", [-math.inf, "lowest", -1e30, 0.0, -0.0])
+def test_alternatives_among_many_equal(dev, dtype, mask):
+    """Rows with few tokens beside a mask: the first masked tokens follow."""
+    V, N, k = 9003, 6, 20
+    g = torch.Generator().manual_seed(0)
+    mask = torch.finfo(dtype).min if mask == "lowest" else mask
+    x = torch.full((N, V), mask).to(dtype)
+    some = torch.randn(N, 5, generator=g).to(dtype)
+    x[0, 100:105] = some[0]
+    x[1, [0, 7, 8999, 9000, 9002]] = some[1]
+    x[2, 8000:] = torch.randn(1003, generator=g).to(dtype)
+    x[3, :8990] = -math.inf                   # the mask's equals come last
+    x[4, ::64] = 1.0                          # more equals than fit, above it
+    x[5, torch.arange(V) // 8 % 64 != 5] = torch.randn(
+        int((torch.arange(V) // 8 % 64 != 5).sum()), generator=g).to(dtype)
+    for kk in (1, k, 64):
+        r = ops.token_logprobs(x.to(dev), torch.zeros(N, dtype=torch.long,
+                                                      device=dev), kk)
+        # falling value, then index (the two zeros are equal)
+        order = torch.sort(x.double() + 0.0, dim=1, descending=True,
+                           stable=True).indices[:, :kk]
+        assert torch.equal(r.top_ids.cpu(), order)
+
+
 @pytest.mark.gpu
 def test_capture_and_replay():
     x = torch.randn(40, 5000, device="cuda").bfloat16().requires_grad_(True)
