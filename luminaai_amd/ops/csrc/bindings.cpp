@@ -2,6 +2,7 @@
 // Host-side code only; kernels live in the *.hip translation units and are
 // reached through extern "C" launchers taking hipStream_t.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/core/DeviceGuard.h>
 #include <hip/hip_runtime.h>
@@ -1037,6 +1038,74 @@ at::Tensor logprob_bwd(const at::Tensor& x, const at::Tensor& tok,
   return dx;
 }
 
+namespace {
+
+// Gradients that cannot be differentiated again: doing so raises. Small calls are
+// bound by the host, so these operators' gradients are recorded here and not by
+// Python functions (a row of log probabilities and its gradient: 56 us of
+// host time for 96, packed attention of 64 tokens 73 for 125).
+torch::autograd::variable_list once(
+    torch::autograd::variable_list grads,
+    const torch::autograd::variable_list& inputs) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::variable_list in;
+  for (const auto& g : grads)
+    if (g.defined()) in.push_back(g.detach().requires_grad_(true));
+  in.insert(in.end(), inputs.begin(), inputs.end());   // leads back to them
+  const auto fn = std::make_shared<torch::autograd::DelayedError>(
+      "this gradient can be taken once only", (int)in.size());
+  const auto out = (*fn)(std::move(in));
+  size_t i = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = out[i++];
+  return grads;
+}
+
+class LogprobFn : public torch::autograd::Function<LogprobFn> {
+ public:
+  static torch::autograd::variable_list forward(
+      torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+      const at::Tensor& tok, int64_t k, int64_t ignore) {
+    const auto [lp, ent, tl, ti, stat] = logprob_fwd(x, tok, k, ignore, true);
+    ctx->save_for_backward({x, tok, stat, ent});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({tl, ti});
+    return {lp, ent, tl, ti};
+  }
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list g) {
+    at::Tensor dx;
+    const auto s = ctx->get_saved_variables();
+    if (g[0].defined() || g[1].defined()) {
+      const at::NoGradGuard no_grad;
+      auto grad = [](const at::Tensor& t) {
+        return t.defined() ? std::optional<at::Tensor>(t.contiguous())
+                           : std::nullopt;
+      };
+      dx = logprob_bwd(s[0], s[1], s[2], s[3], grad(g[0]), grad(g[1]),
+                       ctx->saved_data["ignore"].toInt());
+    }
+    auto out = once({dx}, {s[0]});
+    return {out[0], at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+}  // namespace
+
+// logits [N, V] with contiguous rows, tokens [N] -> logprobs, entropy,
+// alternatives and their ids
+std::vector<at::Tensor> token_logprobs(const at::Tensor& x,
+                                       const at::Tensor& tok, int64_t k,
+                                       int64_t ignore) {
+  if (at::GradMode::is_enabled() && x.requires_grad())
+    return LogprobFn::apply(x, tok, k, ignore);
+  const auto r = logprob_fwd(x, tok, k, ignore, false);
+  return {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r)};
+}
+
 // ---- packed attention ------------------------------------------------------
 namespace {
 // Rows as the kernels take them: whole aligned 16-byte pieces, and tokens no
@@ -1189,6 +1258,49 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attn_bwd(
   return {dq, dk, dv};
 }
 
+namespace {
+
+class PackedAttnFn : public torch::autograd::Function<PackedAttnFn> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx,
+                            const at::Tensor& q, const at::Tensor& k,
+                            const at::Tensor& v, const at::Tensor& cu,
+                            double scale) {
+    // rows that start between 16 bytes were copied: the copies are kept
+    const auto [o, rest, lse, qr, kr, vr] =
+        packed_attn_fwd(q, k, v, cu, scale, true);
+    ctx->save_for_backward({qr, kr, vr, o, rest, lse, cu});
+    ctx->saved_data["scale"] = scale;
+    return o;
+  }
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    at::Tensor dq, dk, dv;
+    {
+      const at::NoGradGuard no_grad;
+      std::tie(dq, dk, dv) =
+          packed_attn_bwd(g[0], s[3], s[4], s[5], s[0], s[1], s[2], s[6],
+                          ctx->saved_data["scale"].toDouble());
+    }
+    auto out = once({dq, dk, dv}, {s[0], s[1], s[2]});
+    return {out[0], out[1], out[2], at::Tensor(), at::Tensor()};
+  }
+};
+
+}  // namespace
+
+at::Tensor packed_attn(const at::Tensor& q, const at::Tensor& k,
+                       const at::Tensor& v, const at::Tensor& cu,
+                       double scale) {
+  if (at::GradMode::is_enabled() &&
+      (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return PackedAttnFn::apply(q, k, v, cu, scale);
+  return std::get<0>(packed_attn_fwd(q, k, v, cu, scale, false));
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("attn_fwd", &attn_fwd,
           "causal GQA flash attention forward -> (O, LSE2) (gfx950)");
@@ -1244,11 +1356,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("ce_bwd", &ce_bwd, "fused CE backward (gfx950)");
   mod.def("l2norm_sq", &l2norm_sq, "flat L2 norm squared (gfx950)");
   mod.def("adamw_step", &adamw_step, "fused clip+AdamW on flat buffers (gfx950)");
-  mod.def("packed_attn_fwd", &packed_attn_fwd, "packed causal attention");
-  mod.def("packed_attn_bwd", &packed_attn_bwd, "gradient of packed_attn_fwd");
+  mod.def("packed_attn", &packed_attn,
+          "packed causal attention, with its gradient");
   mod.def("paged_attn", &paged_attn, "single-token attention over pages");
   mod.def("paged_append", &paged_append, "append keys and values to pages");
   mod.def("copy_pages", &copy_pages, "copy pages within pools");
-  mod.def("logprob_fwd", &logprob_fwd, "token log probabilities and entropy");
-  mod.def("logprob_bwd", &logprob_bwd, "gradient of logprob_fwd");
+  mod.def("token_logprobs", &token_logprobs,
+          "token log probabilities and entropy, with their gradient");
 }

@@ -18,30 +18,6 @@ class TokenLogprobs(NamedTuple):
     top_ids: torch.Tensor        # [..., top_k] int64
 
 
-class _TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, top_k, ignore_index):
-        lp, ent, tl, ti, stat = get_ext().logprob_fwd(logits, tokens, top_k,
-                                                      ignore_index, True)
-        ctx.save_for_backward(logits, tokens, stat, ent)
-        ctx.ignore_index = ignore_index
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(tl, ti)
-        return lp, ent, tl, ti
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_lp, g_ent, _gtl, _gti):
-        if g_lp is None and g_ent is None:
-            return None, None, None, None
-        logits, tokens, stat, ent = ctx.saved_tensors
-        dx = get_ext().logprob_bwd(
-            logits, tokens, stat, ent,
-            None if g_lp is None else g_lp.contiguous(),
-            None if g_ent is None else g_ent.contiguous(), ctx.ignore_index)
-        return dx, None, None, None
-
-
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
                    ignore_index: int = -100) -> TokenLogprobs:
     """logits [..., V] (bf16, fp16 or fp32), tokens [...] int64 or int32.
@@ -53,8 +29,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
     sums in fp32. -inf logits are tokens of probability 0; a row of nothing
     else has no distribution and gives NaN.
 
-    logprobs and entropy have a gradient with respect to logits (once
-    differentiable); the alternatives have none."""
+    logprobs and entropy have a gradient with respect to logits (taken
+    once, on the GPU); the alternatives have none."""
     shape = tokens.shape
     if logits.shape[:-1] != shape:
         raise ValueError(f"tokens {tuple(shape)} do not match logits "
@@ -69,11 +45,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
             x = x.contiguous()
         if not t.is_contiguous():
             t = t.contiguous()
-        if torch.is_grad_enabled() and x.requires_grad:
-            lp, ent, tl, ti = _TokenLogprobsFn.apply(x, t, top_k, ignore_index)
-        else:
-            lp, ent, tl, ti, _ = get_ext().logprob_fwd(x, t, top_k,
-                                                       ignore_index, False)
+        lp, ent, tl, ti = get_ext().token_logprobs(x, t, top_k, ignore_index)
     else:
         lp, ent, tl, ti = ref.token_logprobs(
             logits.reshape(tokens.numel(), logits.shape[-1]),

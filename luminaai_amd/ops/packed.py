@@ -17,46 +17,25 @@ from . import reference as ref
 from .interface import get_ext, use_hip
 
 
-class _PackedAttnFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, cu_seqlens, scale):
-        # rows that start between 16 bytes were copied: the copies are kept
-        o, rest, lse, q, k, v = get_ext().packed_attn_fwd(
-            q, k, v, cu_seqlens, scale, True)
-        ctx.save_for_backward(q, k, v, o, rest, lse, cu_seqlens)
-        ctx.scale = scale
-        return o
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, go):
-        q, k, v, o, rest, lse, cu_seqlens = ctx.saved_tensors
-        dq, dk, dv = get_ext().packed_attn_bwd(go, o, rest, lse, q, k, v,
-                                               cu_seqlens, ctx.scale)
-        return dq, dk, dv, None, None
-
-
 def flash_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                            cu_seqlens: torch.Tensor,
                            scale: Optional[float] = None) -> torch.Tensor:
     """Causal GQA attention inside each packed sequence.
 
     q [T, H, D], k and v [T, kv_heads, D] (bf16 on the GPU, D <= 192, any
-    strides), H a multiple of kv_heads, and at most 65536
-    sequences. Returns [T, H, D]. `scale` (positive) defaults to D ** -0.5. Rows behind the last sequence give zeros and get zero
-    gradients. The gradient is once differentiable and has one order of
-    summation, so it is the same each time. The CPU refuses borders that fall or
-    pass T; the GPU, which does not read them, cuts them to T and computes
-    nothing outside the tensors, and what such borders give is not defined.
+    strides), H a multiple of kv_heads, and at most 65536 sequences. Returns
+    [T, H, D]. `scale` (positive) defaults to D ** -0.5. Rows behind the last
+    sequence give zeros and get zero gradients. The gradient can be taken once
+    (on the GPU) and has one order of summation, so it is the same each time.
+    The CPU refuses borders that fall or pass T; the GPU, which does not read
+    them, cuts them to T and computes nothing outside the tensors, and what such
+    borders give is not defined.
 
     Values that are not finite may reach earlier queries of their sequence."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if use_hip(q):
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
-                                        or v.requires_grad):
-            return _PackedAttnFn.apply(q, k, v, cu_seqlens, scale)
-        return get_ext().packed_attn_fwd(q, k, v, cu_seqlens, scale, False)[0]
+        return get_ext().packed_attn(q, k, v, cu_seqlens, scale)
     return ref.flash_attention_packed(q, k, v, cu_seqlens, scale)
 
 

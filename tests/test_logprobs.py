@@ -272,6 +272,20 @@ def test_alternatives_among_many_equal(dev, dtype, mask):
 
 
 @pytest.mark.gpu
+def test_gradient_is_taken_once():
+    x = torch.randn(5, 700, device="cuda", requires_grad=True)
+    tok = torch.randint(0, 700, (5,), device="cuda")
+    r = ops.token_logprobs(x, tok)
+    plain, = torch.autograd.grad(r.logprobs.sum(), x, retain_graph=True)
+    dx, = torch.autograd.grad(r.logprobs.sum(), x, create_graph=True)
+    assert torch.equal(plain, dx) and dx.requires_grad
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(dx.sum(), x)
+    # only the alternatives are used: no gradient reaches the logits
+    assert not ops.token_logprobs(x, tok, 3).top_logprobs.requires_grad
+
+
+@pytest.mark.gpu
 def test_capture_and_replay():
     x = torch.randn(40, 5000, device="cuda").bfloat16().requires_grad_(True)
     tok = torch.randint(0, 5000, (40,), device="cuda")

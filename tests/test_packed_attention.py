@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from luminaai_amd import ops
 
@@ -311,6 +312,29 @@ def test_listed_blocks_give_the_same_bits(lens):
     a = _run(q, k, v, go, _cu(lens, "cuda"))
     b = _run(q, k, v, go, _cu(lens + [0] * 70, "cuda"))
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 53])
+def test_gradient_is_taken_once(D):
+    q, k, v, go = _inputs([20, 30], 0, 4, 2, D, "cuda")
+    cu = _cu([20, 30], "cuda")
+    q = q.requires_grad_(True)               # k and v need none
+    o = ops.flash_attention_packed(q, k, v, cu)
+    plain, = torch.autograd.grad(o, q, go, retain_graph=True)
+    dq, = torch.autograd.grad(o, q, go, create_graph=True)
+    assert torch.equal(plain, dq) and dq.requires_grad
+    # (the copies of rows of 53 do not lead back to q)
+    with pytest.raises(RuntimeError,
+                       match="once" if D == 64 else "not have been used"):
+        torch.autograd.grad(dq.sum(), q)
+    assert torch.equal(plain, _run(q, k, v, go, cu)[1])
+    # checkpointing runs the forward again
+    c = torch.utils.checkpoint.checkpoint(
+        lambda *a: ops.flash_attention_packed(*a), q, k, v, cu,
+        use_reentrant=False)
+    again, = torch.autograd.grad(c, q, go)
+    assert torch.equal(plain, again)
 
 
 def test_border_refusals_on_the_cpu():
