@@ -428,21 +428,25 @@ DEV_INLINE void zero_rows(uint16_t* out, int heads, int head, int D, int from,
 // exponentials run under the other's products, and causal blocks of half the
 // length are levelled better. 8192 tokens, four / eight waves: 32:8 heads x 128
 // 257 / 268 us (800 TFLOP/s), 12:4 x 159 95 / 105; 483 tokens of 8:4 x 64
-// 7.9 / 9.7. At 192 the images of two do not fit into LDS.
+// 7.9 / 9.7. At 192 the images of two do not fit into LDS. Where there are few
+// blocks, a second set of waves takes the other half of a step's keys (PARTS = 2)
+// and both sets' maximum, sum and result are joined at the end.
 // ===========================================================================
-#define FK 64                  // keys of a step
-
-template <int DP> struct Fwd {
-  static constexpr int W = DP <= 160 ? 4 : 8;      // waves
-  static constexpr int Q = 32 * W;                 // query rows of a workgroup
+template <int DP, int PARTS> struct Fwd {
+  static constexpr int W = DP <= 160 ? 4 * PARTS : 8;    // waves
+  static constexpr int Q = 32 * W / PARTS;               // rows of a workgroup
+  static constexpr int K = DP <= 160 ? 64 * PARTS : 64;  // keys of a step
 };
 
-template <int DP>
-__global__ __launch_bounds__(64 * Fwd<DP>::W, 2)
+template <int DP, int PARTS>
+__global__ __launch_bounds__((64 * Fwd<DP, PARTS>::W), 2)
 void packed_fwd_kernel(const PackedArgs a) {
-  constexpr int DT = DP / 32, KS = DP / 16, FQ = Fwd<DP>::Q, NT = 2 * FQ;
+  constexpr int DT = DP / 32, KS = DP / 16;
+  constexpr int FQ = Fwd<DP, PARTS>::Q, NT = 64 * Fwd<DP, PARTS>::W;
+  constexpr int FK = Fwd<DP, PARTS>::K, KEYS = FK / PARTS;  // of a step, a wave's
   constexpr int IMG = FK * Img<DP>::BYTES;
-  __shared__ char lds[4 * IMG];              // [2][K image, V image]
+  constexpr int JOIN = PARTS == 1 ? 0 : 256 * FQ / 32 * (16 * DT + 2);
+  __shared__ char lds[4 * IMG > JOIN ? 4 * IMG : JOIN];  // [2][K, V image]
   const int h = head_of(blockIdx.x % a.H, a.H);
   const Work w = find_work(a, blockIdx.x / a.H, FQ);
   if (w.tail >= 0) {
@@ -452,7 +456,8 @@ void packed_fwd_kernel(const PackedArgs a) {
   const int lane = threadIdx.x & 63, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hk = h / (a.H / a.HKV);
-  const int q0 = (w.level - 1) * FQ, qw = q0 + 32 * wave;
+  const int group = wave % (FQ / 32), part = wave / (FQ / 32);
+  const int q0 = (w.level - 1) * FQ, qw = q0 + 32 * group;
   const int last = w.len - 1;
   const uint16_t* kb = a.k + w.start * a.k_st + hk * a.k_sh;
   const uint16_t* vb = a.v + w.start * a.v_st + hk * a.v_sh;
@@ -488,18 +493,18 @@ void packed_fwd_kernel(const PackedArgs a) {
   sv.store(lds + IMG);
   __syncthreads();
   for (int t = 0; t < steps; ++t) {
-    const char* ki = lds + (t & 1) * 2 * IMG;
+    const char* ki = lds + (t & 1) * 2 * IMG + KEYS * part * Img<DP>::BYTES;
     const char* vi = ki + IMG;
     {
       const int64_t r = (int64_t)(t + 1 < steps ? t + 1 : t) * FK;
       sk.load(kb + r * a.k_st, a.k_st, last - (int)r);
       sv.load(vb + r * a.v_st, a.v_st, last - (int)r);
     }
-    const int k0 = t * FK;
+    const int k0 = t * FK + KEYS * part;
     if (k0 <= qw + 31) {                     // else all masked for this wave
-      float p[FK / 32][16];
+      float p[KEYS / 32][16];
       #pragma unroll
-      for (int kk = 0; kk < FK / 32; ++kk) {
+      for (int kk = 0; kk < KEYS / 32; ++kk) {
         f32x16 s = zero16();
         #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
@@ -507,9 +512,9 @@ void packed_fwd_kernel(const PackedArgs a) {
         #pragma unroll
         for (int r = 0; r < 16; ++r) p[kk][r] = s[r];
       }
-      if (k0 + FK - 1 > qw) {                // touches the diagonal
+      if (k0 + KEYS - 1 > qw) {                // touches the diagonal
         #pragma unroll
-        for (int kk = 0; kk < FK / 32; ++kk)
+        for (int kk = 0; kk < KEYS / 32; ++kk)
           #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int kt = k0 + 32 * kk + 8 * (r >> 2) + 4 * hi + (r & 3);
@@ -518,7 +523,7 @@ void packed_fwd_kernel(const PackedArgs a) {
       }
       float pm = p[0][0];
       #pragma unroll
-      for (int kk = 0; kk < FK / 32; ++kk)
+      for (int kk = 0; kk < KEYS / 32; ++kk)
         #pragma unroll
         for (int r = 0; r < 16; ++r) pm = fmaxf(pm, p[kk][r]);
       pm *= c2;                              // c2 > 0
@@ -534,7 +539,7 @@ void packed_fwd_kernel(const PackedArgs a) {
         for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
       }
       #pragma unroll
-      for (int kk = 0; kk < FK / 32; ++kk) {
+      for (int kk = 0; kk < KEYS / 32; ++kk) {
         #pragma unroll
         for (int r = 0; r < 16; ++r) {
           p[kk][r] = __builtin_amdgcn_exp2f(
@@ -554,6 +559,26 @@ void packed_fwd_kernel(const PackedArgs a) {
     sk.store(next);
     sv.store(next + IMG);
     __syncthreads();
+  }
+  if (PARTS == 2) {                          // the second part's state joins
+    float* other = reinterpret_cast<float*>(lds) + group * 64 * (16 * DT + 2)
+                   + lane;
+    if (part == 1) {
+      #pragma unroll
+      for (int i = 0; i < 16 * DT; ++i) other[64 * i] = o[i / 16][i & 15];
+      other[64 * 16 * DT] = m;
+      other[64 * (16 * DT + 1)] = l;
+    }
+    __syncthreads();
+    if (part == 1) return;
+    const float m1 = other[64 * 16 * DT], mn = fmaxf(m, m1);
+    const float f0 = __builtin_amdgcn_exp2f(m - mn);
+    const float f1 = __builtin_amdgcn_exp2f(m1 - mn);
+    m = mn;
+    l = l * f0 + other[64 * (16 * DT + 1)] * f1;
+    #pragma unroll
+    for (int i = 0; i < 16 * DT; ++i)
+      o[i / 16][i & 15] = o[i / 16][i & 15] * f0 + other[64 * i] * f1;
   }
   l += __shfl_xor(l, 32, 64);
   const int64_t tok = w.start + qi;
@@ -955,16 +980,29 @@ static hipError_t list_blocks(PackedArgs& a, int* list, int rows,
   return hipSuccess;
 }
 
-template <int DP>
-static hipError_t run_fwd(PackedArgs& a, int* list, hipStream_t stream) {
-  const hipError_t err = list_blocks(a, list, Fwd<DP>::Q, stream);
+template <int DP, int PARTS>
+static hipError_t launch_fwd(PackedArgs& a, int* list, hipStream_t stream) {
+  constexpr int Q = Fwd<DP, PARTS>::Q;
+  const hipError_t err = list_blocks(a, list, Q, stream);
   if (err != hipSuccess) return err;
-  const int64_t n = max_blocks(a, Fwd<DP>::Q) * a.H;
+  const int64_t n = max_blocks(a, Q) * a.H;
   if (n > 0x7fffffff) return hipErrorInvalidValue;
-  packed_fwd_kernel<DP><<<dim3((uint32_t)n), dim3(2 * Fwd<DP>::Q), 0,
-                          stream>>>(a);
+  packed_fwd_kernel<DP, PARTS><<<dim3((uint32_t)n),
+                                 dim3(64 * Fwd<DP, PARTS>::W), 0, stream>>>(a);
   HIP_CHECK_LAST();
   return hipSuccess;
+}
+
+template <int DP>
+static hipError_t run_fwd(PackedArgs& a, int* list, hipStream_t stream) {
+  // Two parts up to 512 blocks of 128 rows, which leave units idle and each other
+  // room, and not for the short sequences that 512 tokens can be. One / two parts,
+  // one sequence: 2048 tokens of 12:4 x 160 63.8 / 52.8 us, of 8:4 x 64 29.9 / 25.0,
+  // of 4:4 x 192 80 / 51, of 32:8 x 128 55.3 / 54.2, 1024 of these 26.8 / 24.2, 256
+  // 10.0 / 10.5; 8192 in four sequences 257 / 318.
+  if (a.T > 512 && (int64_t)a.T * a.H <= 65536)
+    return launch_fwd<DP, 2>(a, list, stream);
+  return launch_fwd<DP, 1>(a, list, stream);
 }
 
 template <int DP>

@@ -103,6 +103,16 @@ def test_packed_attention(dev, H, HKV, D):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("H,HKV,D", [(2, 1, 5), (8, 4, 64), (2, 2, 80),
+                                     (8, 2, 128), (6, 2, 159), (4, 4, 192)])
+def test_few_tokens(dev, H, HKV, D):
+    lens = [1, 0, 33, 129, 300]
+    q, k, v, go = _inputs(lens, 7, H, HKV, D, dev, seed=1)
+    _check(_run(q, k, v, go, _cu(lens, dev)),
+           *_oracle(q, k, v, go, lens, D ** -0.5))
+
+
+@pytest.mark.parametrize("dev", DEVS)
 @pytest.mark.parametrize("lens,tail", [([], 5), ([0, 0], 3), ([1], 0),
                                        ([257], 0), ([1] * 150, 1),
                                        ([700, 3, 520], 300)])
