@@ -80,7 +80,7 @@ hipError_t lumina_moe_combine_bwd_w(const void*, const void*, const int64_t*, fl
 hipError_t lumina_packed_attn_fwd(const void*, const void*, const void*, void*, void*, float*, const int*, int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_packed_attn_bwd(const void*, const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*, void*, float*, int, const int*, int*, const int64_t*, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_pack_rows(const void* const*, void* const*, const int64_t*, const int*, int, int64_t, int, hipStream_t);
-hipError_t lumina_paged_attn(const void*, const void*, const void*, void*, const int*, const int*, float*, float*, int*, const int64_t*, int64_t, int, int, int, int, int, int, int, int, int, int, float, hipStream_t);
+hipError_t lumina_paged_attn(const void*, const void*, const void*, void*, const int*, const int*, float*, float*, int*, int*, const int64_t*, int64_t, int, int, int, int, int, int, int, int, int, int, float, hipStream_t);
 hipError_t lumina_paged_append(const void*, const void*, void*, void*, const int*, const int*, const int*, const int64_t*, int64_t, int64_t, int, int, int, int, int, int, int, hipStream_t);
 hipError_t lumina_copy_pages(void* const*, int, const int64_t*, const int64_t*, int, int64_t, const int*, const int*, int64_t, hipStream_t);
 hipError_t lumina_logprob_fwd(const void*, int, const void*, int, float*, float*, float*, float*, int64_t*, int64_t, int, int64_t, int, int64_t, hipStream_t);
@@ -828,7 +828,7 @@ at::Tensor paged_attn(const at::Tensor& q_, const at::Tensor& kp,
   const int64_t few = std::max<int64_t>(1, 512 / R);
   const int64_t many = std::max(few, std::min(4096 / R, B * steps / 8));
   const int64_t chunks = std::min(many + B + 1, B * steps + B);
-  at::Tensor ws, where;
+  at::Tensor ws, where, plan;
   float* part = nullptr;
   float* ml = nullptr;
   int* wh = nullptr;
@@ -839,12 +839,15 @@ at::Tensor paged_attn(const at::Tensor& q_, const at::Tensor& kp,
     where = at::empty({B, 2}, lens.options());
     wh = where.data_ptr<int>();
   }
+  if (B > 128) plan = at::empty({4 + 2 * chunks}, lens.options());
   const int64_t strides[9] = {q.stride(0), q.stride(1), kp.stride(0),
                               kp.stride(1), kp.stride(2), vp.stride(0),
                               vp.stride(1), vp.stride(2), table.stride(0)};
   check_hip(lumina_paged_attn(q.data_ptr(), kp.data_ptr(), vp.data_ptr(),
                               o.data_ptr(), table.data_ptr<int>(),
-                              lens.data_ptr<int>(), part, ml, wh, strides,
+                              lens.data_ptr<int>(), part, ml, wh,
+                              plan.defined() ? plan.data_ptr<int>() : nullptr,
+                              strides,
                               kp.size(0), (int)B, (int)H, (int)HKV, (int)D,
                               (int)kp.size(3), shift, (int)M, (int)few, (int)many,
                               (int)chunks, (float)scale, cur_stream()),

@@ -81,6 +81,21 @@ DEV_INLINE int wave_sum(int x) {
   return __builtin_amdgcn_readlane(wave_scan(x), 63);
 }
 
+// inclusive sum over a workgroup's threads; ws: an int for each wave
+DEV_INLINE int block_scan(int x, int* ws) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  #pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();                           // the last call's reads are done
+  if (lane == 63) ws[wave] = x;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) x += ws[i];
+  return x;
+}
+
 // generic element accessors so kernels template over T in {float, bf16-as-u16}
 struct F32Elem {
   using storage = float;

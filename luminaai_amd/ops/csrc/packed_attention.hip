@@ -150,21 +150,6 @@ DEV_INLINE Work find_work(const PackedArgs& a, int id, int rows) {
 // ===========================================================================
 #define LEVELS 1024
 
-// inclusive sum over the 1024 threads of a workgroup
-DEV_INLINE int block_scan(int x, int* ws) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();                           // the last call's reads are done
-  if (lane == 63) ws[wave] = x;
-  __syncthreads();
-  for (int i = 0; i < wave; ++i) x += ws[i];
-  return x;
-}
-
 __global__ __launch_bounds__(LEVELS)
 void packed_list_kernel(const int* cu, int B, int T, int rows, int cap,
                         int* list) {

@@ -324,7 +324,8 @@ def test_huge_scores(dev):
 @pytest.mark.parametrize("dev", DEVS)
 @pytest.mark.parametrize("lens", [
     [(37 * b) % 200 for b in range(130)], [0] * 64 + [900],
-    [900] + [0] * 70 + [1, 300], [128, 129, 256, 257, 1023, 1024, 1025]])
+    [900] + [0] * 70 + [1, 300], [128, 129, 256, 257, 1023, 1024, 1025],
+    [2, 0, 1] * 350 + [700, 3]])
 def test_rows_and_widths(dev, lens):
     """More rows than lanes, empty ones among them; however wide the table is,
     the result is the same."""
