@@ -430,3 +430,24 @@ def test_borders_out_of_range_stay_inside():
         _run(room[T:2 * T], k, v, go, c)
     torch.cuda.synchronize()
     assert (room[:T] == 7).all() and (room[2 * T:] == 7).all()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls under way on two streams, over the list of blocks and without it."""
+    sides = []
+    for seed, lens in ((0, [700, 3, 520]), (1, [9] * 90)):
+        q, k, v, go = _inputs(lens, 4, 4, 2, 96, "cuda", seed=seed)
+        cu = _cu(lens, "cuda")
+        sides.append((q, k, v, go, cu, _run(q, k, v, go, cu)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sides]
+    got = [[], []]
+    for _ in range(8):
+        for out, st, (q, k, v, go, cu, _ref) in zip(got, streams, sides):
+            with torch.cuda.stream(st):
+                out.append(_run(q, k, v, go, cu))
+    torch.cuda.synchronize()
+    for outs, side in zip(got, sides):
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, side[-1]))

@@ -437,3 +437,43 @@ def test_other_stream():
     s.synchronize()
     ref, tol = _oracle(q, dense, 128)
     assert ((o.double().cpu() - ref).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls under way on two streams, with planned chunks and without."""
+    sides = []
+    for lens in ([3000, 17, 900], [40, 0, 300] * 60):
+        q, k, v, table, n, _ = _scene(lens, 8, 2, 64, 16, "cuda")
+        sides.append((q, k, v, table, n))
+    ref = [ops.paged_attention(*a) for a in sides]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sides]
+    got = [[], []]
+    for _ in range(20):
+        for out, st, a in zip(got, streams, sides):
+            with torch.cuda.stream(st):
+                out.append(ops.paged_attention(*a))
+    torch.cuda.synchronize()
+    for outs, r in zip(got, ref):
+        assert all(torch.equal(o, r) for o in outs)
+
+
+@pytest.mark.gpu
+def test_planned_chunks_in_a_graph():
+    """More rows than a workgroup looks through; lengths change between
+    replays."""
+    lens = [40, 0, 300] * 60
+    q, k, v, table, n, _ = _scene(lens, 8, 2, 64, 16, "cuda")
+    with torch.no_grad():
+        ops.paged_attention(q, k, v, table, n)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.paged_attention(q, k, v, table, n)
+        for step in range(4):
+            n.copy_(torch.tensor([max(0, x - 7 * step) for x in lens]).int())
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out.clone(), ops.paged_attention(q, k, v, table,
+                                                                n))
