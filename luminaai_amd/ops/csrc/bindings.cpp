@@ -730,6 +730,7 @@ void check_same_device(const at::Tensor& t, const at::Tensor& first,
 // Whether two elements of t may share memory (an expanded tensor, or strides
 // that step over less than they span): what is written there is not defined.
 bool overlaps(const at::Tensor& t) {
+  if (t.is_non_overlapping_and_dense()) return false;
   std::vector<std::pair<int64_t, int64_t>> dims;     // stride, size
   for (int64_t i = 0; i < t.dim(); ++i)
     if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
@@ -929,8 +930,13 @@ void copy_pages(const std::vector<at::Tensor>& pools,
     check_same_device(t, pools[0], "pool");
     TORCH_CHECK_VALUE(t.size(0) > 0 && t.size(1) > 0 && t.numel() > 0,
                       "a pool is empty");
-    TORCH_CHECK_VALUE(t[0][0].is_contiguous(), "a pool's pages must be "
-                      "contiguous");
+    int64_t span = 1;
+    bool contiguous = true;
+    for (int64_t i = t.dim() - 1; i >= 2; --i) {
+      contiguous = contiguous && (t.size(i) == 1 || t.stride(i) == span);
+      span *= t.size(i);
+    }
+    TORCH_CHECK_VALUE(contiguous, "a pool's pages must be contiguous");
     TORCH_CHECK_VALUE(!overlaps(t), "a pool's memory overlaps");
     TORCH_CHECK_VALUE(t.size(1) <= INT32_MAX, "a pool has too many pages");
     if (!d.empty())
@@ -978,7 +984,7 @@ int logit_dtype(const at::Tensor& t) {
 }  // namespace
 
 // logits [N, V] with contiguous rows. stat [N, 2] (row maximum, log2 of the sum)
-// is what the gradient needs; empty where want_stat is false.
+// is what the gradient needs; undefined where want_stat is false.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
 logprob_fwd(const at::Tensor& x, const at::Tensor& tok, int64_t k,
             int64_t ignore, bool want_stat) {
@@ -1000,7 +1006,8 @@ logprob_fwd(const at::Tensor& x, const at::Tensor& tok, int64_t k,
   const c10::DeviceGuard guard(x.device());
   const auto f32 = x.options().dtype(at::kFloat);
   auto lp = at::empty({N}, f32), ent = at::empty({N}, f32);
-  auto stat = at::empty({want_stat ? N : 0, 2}, f32);
+  at::Tensor stat;
+  if (want_stat) stat = at::empty({N, 2}, f32);
   auto tl = at::empty({N, k}, f32);
   auto ti = at::empty({N, k}, x.options().dtype(at::kLong));
   if (N > 0)

@@ -521,7 +521,7 @@ extern "C" hipError_t lumina_paged_attn(
 // Appending: k_pages[page(t), h, row(t), :] = k[t, h, :], zero past head_dim,
 // and the same for v. A thread writes 8 elements of a row. Bound by bytes: 8179
 // tokens of 4 heads x 159, 42 MB: 10.3 us, 4.1 TB/s. Small calls by the launch: 64
-// tokens of 8 x 128: 4.3 us.
+// tokens of 8 x 128: 4.4 us.
 // ===========================================================================
 struct PagedAppendArgs {
   const char* src[2];
@@ -615,7 +615,7 @@ extern "C" hipError_t lumina_paged_append(
 // call copies nothing to the device and may be captured. A workgroup moves
 // COPY_PIECE bytes of one page. Bound by bytes: 301 pages of 32 layers x 8 x 64 x
 // 128, keys and values, 5.0 GB: 970 us, 5.2 TB/s; 3 pages of 31 layers x 4 x 16 x
-// 160: 6.1 us, the launch.
+// 160: 5.1 us, the launch.
 // ===========================================================================
 #define COPY_PAIRS 256
 #define COPY_PIECE 16384

@@ -63,13 +63,12 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
     position (padding), one past the table, or a sequence or page that does not
     exist. Two tokens for one place leave one of them there, it is not said
     which. Nothing flows back through the pool."""
-    k, v = k.detach(), v.detach()
     if use_hip(k):
         get_ext().paged_append(k, v, k_pages, v_pages, block_table, positions,
                                seq_ids)
         return
-    ref.paged_kv_append(k, v, k_pages, v_pages, block_table, positions,
-                        seq_ids)
+    ref.paged_kv_append(k.detach(), v.detach(), k_pages, v_pages, block_table,
+                        positions, seq_ids)
 
 
 def copy_pages(pools: Sequence[torch.Tensor], src: List[int],
