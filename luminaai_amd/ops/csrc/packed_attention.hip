@@ -325,6 +325,20 @@ DEV_INLINE bf16x8 pack_frag(const float* p) {
   return __builtin_bit_cast(bf16x8, u);
 }
 
+// what rounding two numbers to u left over
+DEV_INLINE uint32_t left_over(float lo, float hi, uint32_t u) {
+  return pack2(lo - __builtin_bit_cast(float, u << 16),
+               hi - __builtin_bit_cast(float, u & 0xffff0000u));
+}
+
+// what pack_frag's rounding left over, as a fragment
+DEV_INLINE bf16x8 pack_rest(const float* p, bf16x8 f) {
+  const uintx4 u = __builtin_bit_cast(uintx4, f);
+  const uintx4 v = {left_over(p[0], p[1], u[0]), left_over(p[2], p[3], u[1]),
+                    left_over(p[4], p[5], u[2]), left_over(p[6], p[7], u[3])};
+  return __builtin_bit_cast(bf16x8, v);
+}
+
 DEV_INLINE f32x16 zero16() {
   f32x16 z;
   #pragma unroll
@@ -368,11 +382,6 @@ DEV_INLINE void store8(uint16_t* row, uint32_t a0, uint32_t a1, uint32_t b0,
     for (int j = 0; j < 7; ++j)
       if (d + j < D) row[d + j] = (uint16_t)(u[j >> 1] >> (16 * (j & 1)));
   }
-}
-
-DEV_INLINE uint32_t left_over(float lo, float hi, uint32_t u) {
-  return pack2(lo - __builtin_bit_cast(float, u << 16),
-               hi - __builtin_bit_cast(float, u & 0xffff0000u));
 }
 
 template <int DT>
@@ -587,7 +596,7 @@ void packed_fwd_kernel(const PackedArgs a) {
 #define BQ (32 * BW)
 #define BK 32                  // keys of a step
 
-template <int DP>
+template <int DP, bool FINE>
 __global__ __launch_bounds__(64 * BW, DP <= 160 ? 2 : 1)
 void packed_dq_kernel(const PackedArgs a) {
   constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * BW;
@@ -624,8 +633,8 @@ void packed_dq_kernel(const PackedArgs a) {
   {
     const uint16_t* qr = a.q + tok * a.q_st + h * a.q_sh;
     const uint16_t* gr = a.go + tok * a.go_st + h * a.go_sh;
-    // delta from o with what its rounding left over: the rounding alone would
-    // add a third to the error of dQ and dK (2.5e-3 for 2.4e-3 in all)
+    // delta from o with what its rounding left over: without, the error of dQ and
+    // dK is 2.5e-3 to 2.6e-3 for 2.4e-3
     const uint16_t* orow = a.o + (tok * a.H + h) * a.D;
     const uint16_t* rrow = a.rest + (tok * a.H + h) * a.W;
     #pragma unroll
@@ -695,9 +704,13 @@ void packed_dq_kernel(const PackedArgs a) {
       #pragma unroll
       for (int st = 0; st < 2; ++st) {
         const bf16x8 f = pack_frag(&ds[8 * st]);
+        const bf16x8 rest = pack_rest(&ds[8 * st], f);
         #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          dq[dt] = mfma(cols.get(ki, 16 * st, dt), f, dq[dt]);
+        for (int dt = 0; dt < DT; ++dt) {
+          const bf16x8 c = cols.get(ki, 16 * st, dt);
+          if (FINE) dq[dt] = mfma(c, rest, dq[dt]);
+          dq[dt] = mfma(c, f, dq[dt]);
+        }
       }
     }
     char* next = lds + ((t + 1) & 1) * 2 * IMG;
@@ -732,7 +745,7 @@ void packed_dq_kernel(const PackedArgs a) {
 #define BQT 32                 // queries of a step
 #define BKW 8                  // waves: 4 of each kind
 
-template <int DP>
+template <int DP, bool FINE>
 __global__ __launch_bounds__(64 * BKW, 2)
 void packed_dkdv_kernel(const PackedArgs a) {
   constexpr int DT = DP / 32, KS = DP / 16, NT = 64 * BKW;
@@ -883,10 +896,14 @@ void packed_dkdv_kernel(const PackedArgs a) {
       #pragma unroll
       for (int st = 0; st < 2; ++st) {
         const bf16x8 pf = pack_frag(&p[8 * st]);
+        const bf16x8 rest = pack_rest(&p[8 * st], pf);
         __builtin_amdgcn_s_setprio(1);
         #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          acc[dt] = mfma(cols.get(ci, 16 * st, dt), pf, acc[dt]);
+        for (int dt = 0; dt < DT; ++dt) {
+          const bf16x8 c = cols.get(ci, 16 * st, dt);
+          if (FINE) acc[dt] = mfma(c, rest, acc[dt]);
+          acc[dt] = mfma(c, pf, acc[dt]);
+        }
         __builtin_amdgcn_s_setprio(0);
       }
     }
@@ -990,19 +1007,19 @@ static hipError_t run_fwd(PackedArgs& a, int* list, hipStream_t stream) {
   return launch_fwd<DP, 1>(a, list, stream);
 }
 
-template <int DP>
-static hipError_t run_bwd(PackedArgs& a, int* list, hipStream_t stream) {
+template <int DP, bool FINE>
+static hipError_t launch_bwd(PackedArgs& a, int* list, hipStream_t stream) {
   static_assert(BQ == BKV, "one list for both kernels");
   const hipError_t err = list_blocks(a, list, BQ, stream);
   if (err != hipSuccess) return err;
   const int64_t n = max_blocks(a, BQ) * a.H;
   if (n > 0x7fffffff) return hipErrorInvalidValue;
-  packed_dq_kernel<DP><<<dim3((uint32_t)n), dim3(64 * BW), 0, stream>>>(a);
+  packed_dq_kernel<DP, FINE><<<dim3((uint32_t)n), dim3(64 * BW), 0, stream>>>(a);
   HIP_CHECK_LAST();
   const int64_t m = max_blocks(a, BKV) * a.HKV * a.splits;
   if (m > 0x7fffffff) return hipErrorInvalidValue;
-  packed_dkdv_kernel<DP><<<dim3((uint32_t)m), dim3(64 * BKW), 0,
-                                stream>>>(a);
+  packed_dkdv_kernel<DP, FINE><<<dim3((uint32_t)m), dim3(64 * BKW), 0,
+                                 stream>>>(a);
   HIP_CHECK_LAST();
   if (a.splits > 1) {
     const int64_t each = (int64_t)a.T * a.HKV * ((a.D + 3) / 4);
@@ -1011,6 +1028,18 @@ static hipError_t run_bwd(PackedArgs& a, int* list, hipStream_t stream) {
     HIP_CHECK_LAST();
   }
   return hipSuccess;
+}
+
+template <int DP>
+static hipError_t run_bwd(PackedArgs& a, int* list, hipStream_t stream) {
+  // P and dS enter dV, dK and dQ as bf16; FINE adds what that rounding left over, in
+  // a second product. Small calls take it: the host needs 70 us for them anyway, and
+  // the roundings of few terms do not average out. Forward and gradient, without /
+  // with it: 52 tokens of 2:1 x 64 18.7 / 19.6 us with an error of dQ of 2.6e-3 /
+  // 1.9e-3 (the result's own rounding is 1.7e-3), 256 of 32:8 x 128 49.8 / 53.1,
+  // 2048 262 / 295, 8192 1084 / 1270 (2.4e-3 without).
+  if ((int64_t)a.T * a.H <= 8192) return launch_bwd<DP, true>(a, list, stream);
+  return launch_bwd<DP, false>(a, list, stream);
 }
 
 static void fill(PackedArgs& a, const int64_t* st, const int* cu, int T, int B,

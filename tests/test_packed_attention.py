@@ -113,6 +113,30 @@ def test_few_tokens(dev, H, HKV, D):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("H,HKV,D", [(8, 1, 15), (8, 4, 64), (8, 8, 80),
+                                     (8, 2, 128), (9, 3, 159), (8, 8, 192)])
+def test_more_tokens(dev, H, HKV, D):
+    lens = [700, 1, 0, 400]
+    q, k, v, go = _inputs(lens, 7, H, HKV, D, dev, seed=2)
+    _check(_run(q, k, v, go, _cu(lens, dev)),
+           *_oracle(q, k, v, go, lens, D ** -0.5))
+
+
+@pytest.mark.gpu
+def test_few_roundings_of_a_small_call():
+    """P and dS of a small call enter their products with 16 bits, so the
+    gradients are little further off than their own rounding: a half of what
+    a second rounding of the same size would add to its square."""
+    lens = [43, 9]
+    q, k, v, go = _inputs(lens, 5, 2, 1, 64, "cuda")
+    got = _run(q, k, v, go, _cu(lens, "cuda"))
+    val, _ = _oracle(q, k, v, go, lens, 0.125)
+    for x, y in list(zip(got, val))[1:]:
+        alone = (y.bfloat16().double() - y).norm()
+        assert (x.double().cpu() - y).norm() <= 1.5 ** 0.5 * alone
+
+
+@pytest.mark.parametrize("dev", DEVS)
 @pytest.mark.parametrize("lens,tail", [([], 5), ([0, 0], 3), ([1], 0),
                                        ([257], 0), ([1] * 150, 1),
                                        ([700, 3, 520], 300)])
