@@ -312,7 +312,8 @@ void paged_attn_kernel(const PagedAttnArgs a) {
     uint32_t ph[4], pl[4];
     #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(s[j] - m), p1 = __builtin_amdgcn_exp2f(s[j + 1] - m);
+      const float p0 = __builtin_amdgcn_exp2f(s[j] - m);
+      const float p1 = __builtin_amdgcn_exp2f(s[j + 1] - m);
       l += p0 + p1;
       const uint32_t u = pack_bf16(p0, p1);
       ph[j / 2] = u;

@@ -37,8 +37,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor,
 
     q [B, H, D] (bf16 on the GPU, D <= 192), pages as above with H a multiple
     of kv_heads, block_table [B, M] int32, seq_lens [B] int32 (the new token
-    included); a table's row has room for fewer
-    than 2^29 tokens, all together for 2^31. Returns [B, H, D] in q's type; a sequence of length 0 gives
+    included); a table's row has room for fewer than 2^29 tokens, all together
+    for 2^31. Returns [B, H, D] in q's type; a sequence of length 0 gives
     zeros. `scale` defaults to D ** -0.5. There is no gradient. Nothing behind
     a sequence's end is read; a live value that is not finite makes its
     sequence's result NaN or infinite."""
