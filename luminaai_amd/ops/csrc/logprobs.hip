@@ -69,9 +69,10 @@ DEV_INLINE float max_nan(float a, float b) {
   return __builtin_elementwise_maximum(a, b);
 }
 
-// orders floats as unsigned numbers; NaN above all, the two zeros equal
+// orders floats as unsigned numbers; NaN above all, the two zeros equal. No key is
+// all ones, so that of a NaN at index 0 stays below 2^64 - 1 (pair_key).
 DEV_INLINE uint32_t order_key(float f) {
-  if (f != f) return 0xffffffffu;
+  if (f != f) return 0xfffffffeu;
   const uint32_t u = __builtin_bit_cast(uint32_t, f + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
@@ -364,7 +365,7 @@ void logprob_fwd_kernel(const LogprobArgs a) {
     }
     return;
   }
-  uint64_t prev = ~0ull;                 // above every key: indexes are >= 0
+  uint64_t prev = ~0ull;                 // above every key
   for (int rank = 0; rank < a.k; ++rank) {
     uint64_t b = 0;
     for (int q = threadIdx.x; q < a.V; q += BLOCK) {

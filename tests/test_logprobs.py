@@ -271,6 +271,35 @@ def test_alternatives_among_many_equal(dev, dtype, mask):
         assert torch.equal(r.top_ids.cpu(), order)
 
 
+def _nan_first(x, k):
+    """Alternatives with NaN above all, then falling values, ties to the lowest
+    index."""
+    x = x.double() + 0.0
+    key = torch.where(x.isnan(), math.inf, x)
+    order = torch.sort(key, dim=1, descending=True, stable=True).indices
+    last = torch.sort(x.isnan().gather(1, order).int(), dim=1, descending=True,
+                      stable=True).indices
+    return order.gather(1, last)[:, :k]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_alternatives_of_many_nan(dev, dtype):
+    """More NaN than fit beside each other, from the first token on."""
+    V = 3000
+    x = torch.randn(4, V, generator=torch.Generator().manual_seed(0))
+    x[0] = math.nan
+    x[1, :1500] = math.nan
+    x[2, 1:1500] = math.nan
+    x[3, ::2] = math.nan
+    x = x.to(dtype)
+    tok = torch.zeros(4, dtype=torch.long, device=dev)
+    for k in (1, 3, 64):
+        r = ops.token_logprobs(x.to(dev), tok, k)
+        assert torch.equal(r.top_ids.cpu(), _nan_first(x, k))
+        assert r.top_logprobs.isnan().all()
+
+
 @pytest.mark.gpu
 def test_gradient_is_taken_once():
     x = torch.randn(5, 700, device="cuda", requires_grad=True)
