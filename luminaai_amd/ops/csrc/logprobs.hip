@@ -321,7 +321,9 @@ void logprob_fwd_kernel(const LogprobArgs a) {
       const int at = atomicAdd(&n_cand, 1);
       if (at < LP_CAP) cand[at] = pair_key(f, idx);
     };
-    if (!(mx <= B))
+    // a thread that met a NaN (s != s) may hold any of them: its maximum started
+    // anew behind it
+    if (!(mx <= B) || s != s)
       for (int q = threadIdx.x; q < nvec; q += BLOCK) {
         const Vec8<S> v = load8(x + 8 * (int64_t)q);
         #pragma unroll

@@ -300,6 +300,28 @@ def test_alternatives_of_many_nan(dev, dtype):
         assert r.top_logprobs.isnan().all()
 
 
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", [-math.inf, -1e30, 0.0])
+def test_alternatives_beside_a_nan_and_a_mask(dev, dtype, mask):
+    """A NaN early in the row, larger logits beside it and elsewhere, and more
+    equal logits than fit."""
+    V, k = 50304, 20
+    x = torch.full((4, V), mask).to(dtype)
+    x[0, 3] = math.nan
+    x[0, 5], x[0, 20], x[0, 50303] = 2.0, 1.0, 3.0
+    x[1, 40000] = math.nan
+    x[1, 40001] = 1.5
+    x[2, [0, 9000, 50303]] = math.nan
+    x[2, 30] = math.inf
+    x[3, ::4096] = math.nan
+    x[3, 1::4096] = 1.0
+    tok = torch.zeros(4, dtype=torch.long, device=dev)
+    for kk in (1, k, 64):
+        r = ops.token_logprobs(x.to(dev), tok, kk)
+        assert torch.equal(r.top_ids.cpu(), _nan_first(x, kk))
+
+
 @pytest.mark.gpu
 def test_gradient_is_taken_once():
     x = torch.randn(5, 700, device="cuda", requires_grad=True)
