@@ -25,7 +25,8 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass, field
-from typing import Callable, Dict, List, Optional, Tuple, Union
+from typing import (Callable, Dict, List, NamedTuple, Optional, Tuple,
+                    Union)
 
 import torch
 import torch.nn as nn
@@ -574,8 +575,11 @@ class MoEFFNLayer(nn.Module):
         nn.init.normal_(self.w_down, std=init_std)
         nn.init.normal_(self.gate.weight, std=init_std)
 
-    def forward(self, x) -> Tuple[torch.Tensor, torch.Tensor]:
-        """x: [B, S, h] -> (out [B, S, h], aux_loss scalar)."""
+    def forward(self, x, seqs: Optional["_Sequences"] = None
+                ) -> Tuple[torch.Tensor, torch.Tensor]:
+        """x: [B, S, h] -> (out [B, S, h], aux_loss scalar). seqs: the tokens
+        belong to sequences that have nothing to do with each other, and each
+        has the capacity that it would have alone."""
         B, S, h = x.shape
         N = B * S
         xf = x.reshape(N, h)
@@ -601,7 +605,18 @@ class MoEFFNLayer(nn.Module):
         C = max(1, int(math.ceil(N * k / E * self.capacity_factor)))
         placement = getattr(self, "placement", None)
         route_idx = topi if placement is None else placement[topi]
-        plan = ops.interface.moe_routing_plan(route_idx, E, C)
+        if seqs is None:
+            plan = ops.interface.moe_routing_plan(route_idx, E, C)
+        elif seqs.lens is None:
+            # a token's experts differ: one token is never dropped
+            C = N
+            plan = ops.interface.moe_routing_plan(route_idx, E, C)
+        else:
+            limit = (seqs.lens.double() * k / E * self.capacity_factor) \
+                .ceil().clamp(min=1).long()
+            C = min(N, C + limit.shape[0])           # room for all of them
+            plan = ops.interface.moe_routing_plan(route_idx, E, C, seqs.seq,
+                                                  limit)
         counts = plan.counts if placement is None \
             else plan.counts[placement]        # back to per-expert order
         bufv = ops.interface.moe_dispatch(xf, plan).view(E, C, h)
@@ -795,6 +810,20 @@ class MoEFFNLayer(nn.Module):
         self._reshard_experts(full_gu[kt], full_dn[kt], len(keep))
 
 
+class _Sequences(NamedTuple):
+    """Which sequence each token of a forward belongs to (MoEFFNLayer)."""
+
+    seq: Optional[torch.Tensor]     # [T] long; None: every token is its own
+    lens: Optional[torch.Tensor]    # [n + 1] long, the rest of the row last
+
+    @classmethod
+    def packed(cls, cu_seqlens: torch.Tensor, total: int) -> "_Sequences":
+        tok = torch.arange(total, dtype=torch.int32, device=cu_seqlens.device)
+        seq = torch.searchsorted(cu_seqlens[1:].contiguous(), tok, right=True)
+        ends = F.pad(cu_seqlens.long(), (0, 1), value=total)
+        return cls(seq, ends.diff().clamp(0, total))
+
+
 # ======================================================================
 class MoDRouter(nn.Module):
     """Mixture-of-Depths token router: sigmoid importance scores, per-sequence
@@ -848,13 +877,13 @@ class TransformerBlock(nn.Module):
         self._mod_skip_frac = 0.0
 
     def _inner(self, x, rope_cs, pos, pos_offset, kv_cache, attn_mask,
-               cu_seqlens=None):
+               cu_seqlens=None, seqs=None):
         """attention + FFN with residuals; returns (out, aux_loss)."""
         h = self.attention(self.input_norm(x), rope_cs, pos, pos_offset,
                            kv_cache, attn_mask, cu_seqlens)
         x = x + h
         if self.is_moe:
-            f, aux = self.ffn(self.post_attn_norm(x))
+            f, aux = self.ffn(self.post_attn_norm(x), seqs)
         else:
             f = self.ffn(self.post_attn_norm(x))
             aux = x.new_zeros(())
@@ -863,13 +892,14 @@ class TransformerBlock(nn.Module):
     def forward(self, x, rope_cs, pos: Optional[torch.Tensor] = None,
                 pos_offset: int = 0, kv_cache: Optional[KVCache] = None,
                 attn_mask: Optional[torch.Tensor] = None,
-                cu_seqlens: Optional[torch.Tensor] = None):
+                cu_seqlens: Optional[torch.Tensor] = None,
+                seqs: Optional[_Sequences] = None):
         B, S, H = x.shape
         run_mod = (self.use_mod and kv_cache is None and S > 1
                    and int(S * self.mod_capacity) < S)
         if not run_mod:
             return self._inner(x, rope_cs, pos, pos_offset, kv_cache,
-                               attn_mask, cu_seqlens)
+                               attn_mask, cu_seqlens, seqs)
         if cu_seqlens is not None:
             raise ValueError("mixture-of-depths layers choose tokens of a whole "
                              "row: packed sequences are not supported")
@@ -976,7 +1006,9 @@ class DeepSeekTransformer(nn.Module):
         sequences one after the other, each with positions from 0 and
         attention inside itself (ops.flash_attention_packed). Not together
         with an attention_mask, unpaged caches, sequence parallelism or
-        mixture-of-depths layers in training."""
+        mixture-of-depths layers in training. In eval mode each of them (and each
+        row over a paged cache) has the experts' capacity to itself, so its
+        logits are those that it has alone."""
         B, S = input_ids.shape
         paged = kv_caches is not None and getattr(kv_caches[0], "paged", False)
         if cu_seqlens is not None:
@@ -1033,6 +1065,16 @@ class DeepSeekTransformer(nn.Module):
             attn_mask = torch.zeros(B, 1, S, L, device=x.device,
                                     dtype=x.dtype).masked_fill(~keep, -1e4)
 
+        # Sequences of a packed or paged forward are not related: in eval mode
+        # none of them takes the experts' capacity from another. In training the
+        # row shares it, as a padded batch does.
+        seqs = None
+        if not self.training and any(l.is_moe for l in self.layers):
+            if cu_seqlens is not None:
+                seqs = _Sequences.packed(cu_seqlens, S)
+            elif paged:
+                seqs = _Sequences(None, None)
+
         total_aux = x.new_zeros(())
         aux_losses: Dict[str, torch.Tensor] = {}
         hidden_states = [] if return_hidden_states else None
@@ -1044,7 +1086,7 @@ class DeepSeekTransformer(nn.Module):
                     cu_seqlens, use_reentrant=False)
             else:
                 x, aux = layer(x, rope_cs, pos, pos_offset, cache, attn_mask,
-                               cu_seqlens)
+                               cu_seqlens, seqs)
             if layer.is_moe:
                 total_aux = total_aux + aux
                 aux_losses[f"layer_{i}_moe"] = aux.detach()

@@ -459,21 +459,38 @@ class MoERoutingPlan:
 
 
 @torch.no_grad()
-def moe_routing_plan(topi: torch.Tensor, num_experts: int,
-                     capacity: int) -> MoERoutingPlan:
+def moe_routing_plan(topi: torch.Tensor, num_experts: int, capacity: int,
+                     seq: Optional[torch.Tensor] = None,
+                     limit: Optional[torch.Tensor] = None) -> MoERoutingPlan:
     """topi [N, k] long -> gather plan. Tokens beyond an expert's capacity
     are dropped (stable order: earlier tokens win), matching the reference's
-    capacity_factor semantics (model.py:1219-1242)."""
+    capacity_factor semantics (model.py:1219-1242).
+
+    seq [N] and limit [S] (long): token t belongs to sequence seq[t], of which an
+    expert takes limit[seq[t]] tokens at most, the first ones."""
     N, k = topi.shape
     Nk = N * k
     E, C = num_experts, capacity
     dev = topi.device
     flat_e = topi.reshape(-1)                        # token-major
-    order = torch.argsort(flat_e, stable=True)
-    sorted_e = flat_e[order]
     counts = torch.bincount(flat_e, minlength=E)
     offs = torch.cumsum(counts, 0) - counts
-    pos = torch.arange(Nk, device=dev) - offs[sorted_e]
+    if limit is None:
+        order = torch.argsort(flat_e, stable=True)
+        sorted_e = flat_e[order]
+        pos = torch.arange(Nk, device=dev) - offs[sorted_e]
+    else:
+        S = limit.shape[0]
+        group = flat_e * S + seq.repeat_interleave(k)    # (expert, sequence)
+        order = torch.argsort(group, stable=True)
+        sorted_e, group = flat_e[order], group[order]
+        n = torch.zeros(E * S, dtype=torch.long, device=dev)
+        n.scatter_add_(0, group, torch.ones_like(group))
+        rank = torch.arange(Nk, device=dev) - (torch.cumsum(n, 0) - n)[group]
+        kept = torch.minimum(n.view(E, S), limit).view(-1)
+        before = torch.cumsum(kept, 0) - kept
+        pos = before[group] - before[sorted_e * S] + rank
+        pos = torch.where(rank < kept[group], pos, C)
     dest_sorted = torch.where(pos < C, sorted_e * C + pos,
                               torch.full_like(pos, E * C))
     slot_tm = torch.empty(Nk, dtype=torch.long, device=dev)

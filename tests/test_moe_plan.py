@@ -83,3 +83,48 @@ def test_plan_counts():
     topi = torch.tensor([[0], [0], [1], [3]])
     plan = moe_routing_plan(topi, 4, 8)
     assert plan.counts.tolist() == [2, 1, 0, 1]
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(
+    "cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("k", [1, 2, 3])
+def test_limits_of_each_sequence(dev, k):
+    """Each sequence keeps what a plan of it alone keeps."""
+    torch.manual_seed(k)
+    E, lens = 4, [1, 9, 0, 30, 2, 17]
+    N = sum(lens)
+    topi = torch.stack([torch.randperm(E)[:k] for _ in range(N)])
+    topi[:20, 0] = 1
+    limit = torch.tensor([max(1, -(-n * k * 5 // (E * 4))) for n in lens])
+    seq = torch.repeat_interleave(torch.arange(6), torch.tensor(lens))
+    C = int(limit.sum())
+    plan = moe_routing_plan(topi.to(dev), E, C, seq.to(dev), limit.to(dev))
+    slot = plan.slot_tm.cpu().view(N, k)
+    at = 0
+    for n, most in zip(lens, limit.tolist()):
+        if n:
+            alone = moe_routing_plan(topi[at:at + n], E, most)
+            kept = alone.slot_tm.view(n, k) < E * most
+            assert torch.equal(slot[at:at + n] < E * C, kept)
+        at += n
+    kept = slot < E * C
+    assert torch.equal(slot[kept] // C, topi[kept])     # in the right bucket
+    assert slot[kept].unique().numel() == int(kept.sum())
+    fill = plan.fill_mask.cpu().nonzero()[:, 0]
+    assert torch.equal(fill, slot[kept].sort().values)
+    assert torch.equal(plan.inv.cpu()[slot[kept]],
+                       torch.arange(N * k).view(N, k)[kept])
+    assert torch.equal(plan.counts.cpu(),
+                       torch.bincount(topi.reshape(-1), minlength=E))
+
+
+@pytest.mark.parametrize("C", [1, 5, 40])
+def test_limits_with_any_sequence_numbers(C):
+    """Numbers that fall, and limits past the bucket, lead nowhere outside."""
+    torch.manual_seed(0)
+    topi = torch.randint(0, 4, (50, 2))
+    seq = torch.randint(0, 7, (50,))
+    plan = moe_routing_plan(topi, 4, C, seq, torch.full((7,), 9))
+    assert 0 <= int(plan.slot_tm.min()) and int(plan.slot_tm.max()) <= 4 * C
+    kept = plan.slot_tm[plan.slot_tm < 4 * C]
+    assert kept.unique().numel() == kept.numel() == int(plan.fill_mask.sum())

@@ -201,6 +201,59 @@ def test_packed_moe(tiny_moe_config):
     assert all(x is None or bool(x.isfinite().all()) for x in grads)
 
 
+def _dropping_moe(cfg):
+    """Experts that many tokens want: a forward drops a good part of them."""
+    cfg.num_layers, cfg.num_experts, cfg.seq_length = 3, 8, 64
+    m = _moe(cfg).eval()
+    g = torch.Generator().manual_seed(7)
+    with torch.no_grad():
+        for p in m.parameters():
+            if p.dim() > 1:
+                p.copy_(0.2 * torch.randn(p.shape, generator=g))
+    return m
+
+
+def _sequences(*lens):
+    g = torch.Generator().manual_seed(5)
+    return [torch.randint(1, 500, (n,), generator=g).tolist() for n in lens]
+
+
+def test_moe_forward_of_each_packed_sequence_is_its_own(tiny_moe_config):
+    m = _dropping_moe(tiny_moe_config)
+    seqs = [torch.tensor(s) for s in _sequences(12, 1, 60, 33)]
+    cu = torch.tensor([0, 12, 13, 13, 73, 106], dtype=torch.int32)
+    pad = torch.ones(4, dtype=torch.long)        # behind the last sequence
+    with torch.no_grad():
+        out = m(torch.cat([*seqs, pad])[None], cu_seqlens=cu)[0][0]
+        at = 0
+        for s in seqs:
+            alone = m(s[None])[0][0]
+            assert torch.allclose(out[at:at + len(s)], alone, atol=1e-4)
+            at += len(s)
+
+
+def test_moe_scores_do_not_depend_on_the_batch(tiny_moe_config, tokenizer):
+    solo = GenerationEngine(_dropping_moe(tiny_moe_config), tokenizer)
+    seqs = _sequences(12, 33, 60, 25)
+    for s, r in zip(seqs, solo.score(seqs)):
+        alone = solo.score([s])[0]
+        for k in ("logprobs", "entropy"):
+            assert torch.allclose(torch.tensor(r[k]), torch.tensor(alone[k]),
+                                  atol=1e-4)
+
+
+def test_paged_moe_answers_do_not_depend_on_the_batch(tiny_moe_config,
+                                                      tokenizer):
+    m = _dropping_moe(tiny_moe_config)
+    prompts = _sequences(12, 33, 40, 25)
+    solo = GenerationEngine(m, tokenizer)
+    refs = [solo.generate(p, _cfg(8)) for p in prompts]
+    eng = _engine(m, tokenizer)
+    assert eng.run_to_completion(prompts, _cfg(8)) == refs
+    assert eng.run_to_completion(prompts, _cfg(8),
+                                 admit_schedule=[0, 2, 2, 5]) == refs
+
+
 def test_paged_engine_with_quantized_moe(tiny_moe_config, tokenizer):
     from luminaai_amd.ops.quant import quantize_model
     m = _moe(tiny_moe_config).eval()
@@ -518,3 +571,22 @@ def test_gpu_packed_training_step(gpu_model):
     out, _, _ = m(torch.cat(seqs)[None].cuda(), cu_seqlens=cu.cuda())
     for x, y in zip(grads(m, out[0][:, :512]), b):
         assert (x.float().cpu() - y).norm() <= 21 * 2 ** -8 * y.norm()
+
+
+@pytest.mark.gpu
+def test_gpu_paged_moe(tiny_moe_config, tokenizer):
+    """Every answer has its length, and its tokens are the likeliest of what the
+    model says where it stands."""
+    m = _dropping_moe(tiny_moe_config).to("cuda", torch.bfloat16)
+    eng = _engine(m, tokenizer)
+    # log probabilities are taken before penalties: without one, the greedy token
+    # is the likeliest
+    cfg = _cfg(8, logprobs=1, repetition_penalty=1.0)
+    slots = eng.admit_many(_sequences(12, 33, 40, 25), [cfg] * 4)
+    while eng.n_active():
+        eng.step()
+    for b in slots:
+        s = eng.slots[b]
+        assert len(s.result) == 8
+        for t, e in zip(s.result, s.logprobs):
+            assert e["top"][0][0] == t and math.isfinite(e["logprob"])
