@@ -121,6 +121,8 @@ class ContinuousBatchingEngine:
         b = self.free_slot()
         if b is None:
             raise RuntimeError("no free slot — poll can_admit first")
+        # before anything is taken: a bad list must not leave a slot behind
+        stops = set(cfg.stop_token_ids) | {self.tokenizer.eos_token_id}
         ids = prompt_ids[-min(cfg.max_context, self.max_len - 1):] \
             or [self._pad]
         P = len(ids)
@@ -165,7 +167,7 @@ class ContinuousBatchingEngine:
         s = self.slots[b]
         s.active = True
         s.cfg = cfg
-        s.stops = set(cfg.stop_token_ids) | {self.tokenizer.eos_token_id}
+        s.stops = stops
         s.recent = list(ids)
         s.out = []
         s.cb = stream_callback

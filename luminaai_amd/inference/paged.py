@@ -256,19 +256,33 @@ class PagedKVCache:
 
 class _Slot:
     __slots__ = ("active", "cfg", "stops", "recent", "out", "cb", "done",
-                 "result", "logprobs")
+                 "result", "logprobs", "error")
 
     def __init__(self):
         self.active = False
         self.result = None
         self.logprobs = None
+        self.error = None
+
+    def start(self, cfg, stops, recent, out, logprobs, cb):
+        self.cfg = cfg
+        self.stops = stops
+        self.recent = recent
+        self.out = out
+        self.logprobs = logprobs
+        self.cb = cb
+        self.done = threading.Event()
+        self.result = None
+        self.error = None
+        self.active = True
 
 
 class PagedBatchingEngine:
     """Iteration-level scheduler over a PagedKVCache, with the interface of
     ContinuousBatchingEngine and forks and log probabilities besides. A slot
     that finds no page for its next token ends with what it has; the default
-    pool holds max_batch sequences of max_len."""
+    pool holds max_batch sequences of max_len. A slot whose next token cannot
+    be sampled ends too, with the exception in its `error`; the others go on."""
 
     def __init__(self, model, tokenizer, max_batch: int = 8,
                  max_len: int = 2048, page_size: int = 64,
@@ -327,45 +341,47 @@ class PagedBatchingEngine:
             return []
         configs = configs or [None] * len(prompts)
         callbacks = callbacks or [None] * len(prompts)
+        if not len(prompts) == len(configs) == len(callbacks):
+            raise ValueError(f"{len(prompts)} prompts, {len(configs)} configs "
+                             f"and {len(callbacks)} callbacks")
         cfgs = [c or GenerationConfig() for c in configs]
-        for c in cfgs:
-            if c.logprobs is not None and not 0 <= c.logprobs <= 64:
-                raise ValueError("logprobs must be 0 to 64, got "
-                                 f"{c.logprobs}")
+        stops = [self._stops(c) for c in cfgs]
         slots = self.free_slots()[:len(prompts)]
         if len(slots) < len(prompts):
             raise RuntimeError("no free slot — poll can_admit first")
         ids = [p[-min(c.max_context, self.max_len - 1):] or [self._pad]
                for p, c in zip(prompts, cfgs)]
         check_tokens(ids, self.model)
-        caches, cu = self.cache.prefill(slots, [len(x) for x in ids])
         flat = [t for x in ids for t in x]
         try:
+            caches, cu = self.cache.prefill(slots, [len(x) for x in ids])
             logits, _, _ = self.model(
                 torch.tensor([flat], dtype=torch.long).to(self.device),
                 kv_caches=caches, cu_seqlens=cu)
+            last = logits[0].index_select(0, (cu[1:] - 1).long()).float()
+            if self.last_logits is None:
+                self.last_logits = last.new_zeros(self.max_batch,
+                                                  last.shape[-1])
+            for i, b in enumerate(slots):
+                self.last_logits[b] = last[i]
         except Exception:
             for b in slots:
                 self.cache.free(b)
             raise
-        last = logits[0].index_select(0, (cu[1:] - 1).long()).float()
-        if self.last_logits is None:
-            self.last_logits = last.new_zeros(self.max_batch, last.shape[-1])
         for i, b in enumerate(slots):
-            self.last_logits[b] = last[i]
-            s = self.slots[b]
-            s.active = True
-            s.cfg = cfgs[i]
-            s.stops = set(cfgs[i].stop_token_ids) \
-                | {self.tokenizer.eos_token_id}
-            s.recent = list(ids[i])
-            s.out = []
-            s.logprobs = []
-            s.cb = callbacks[i]
-            s.done = threading.Event()
-            s.result = None
+            self.slots[b].start(cfgs[i], stops[i], list(ids[i]), [], [],
+                                callbacks[i])
         self.stats["admitted"] += len(slots)
         return slots
+
+    def _stops(self, cfg: GenerationConfig) -> set:
+        """Checks a configuration; the tokens that end its answer."""
+        if cfg.logprobs is not None and not 0 <= cfg.logprobs <= 64:
+            raise ValueError(f"logprobs must be 0 to 64, got {cfg.logprobs}")
+        if not all(isinstance(t, int) for t in cfg.stop_token_ids):
+            raise ValueError("stop_token_ids must be whole numbers, got "
+                             f"{cfg.stop_token_ids}")
+        return set(cfg.stop_token_ids) | {self.tokenizer.eos_token_id}
 
     def admit(self, prompt_ids: List[int],
               cfg: Optional[GenerationConfig] = None,
@@ -383,17 +399,12 @@ class PagedBatchingEngine:
         if not free:
             raise RuntimeError("no free slot — poll can_admit first")
         b = free[0]
-        self.cache.fork(slot, b)
+        cfg = cfg or src.cfg
+        stops = self._stops(cfg)
         self.last_logits[b] = self.last_logits[slot]
-        s = self.slots[b]
-        s.active = True
-        s.cfg = cfg or src.cfg
-        s.stops = set(s.cfg.stop_token_ids) | {self.tokenizer.eos_token_id}
-        s.recent, s.out = list(src.recent), list(src.out)
-        s.logprobs = list(src.logprobs)
-        s.cb = stream_callback
-        s.done = threading.Event()
-        s.result = None
+        self.cache.fork(slot, b)
+        self.slots[b].start(cfg, stops, list(src.recent), list(src.out),
+                            list(src.logprobs), stream_callback)
         self.stats["admitted"] += 1
         return b
 
@@ -407,13 +418,25 @@ class PagedBatchingEngine:
         for b, s in enumerate(self.slots):
             if not s.active:
                 continue
-            nid = sample_token(self.last_logits[b].clone(), s.cfg,
-                               s.recent[-s.cfg.rep_window:])
-            if nid in s.stops or len(s.out) >= s.cfg.max_new_tokens:
+            try:
+                nid = sample_token(self.last_logits[b].clone(), s.cfg,
+                                   s.recent[-s.cfg.rep_window:])
+                ends = nid in s.stops or len(s.out) >= s.cfg.max_new_tokens
+            except Exception as e:  # noqa: BLE001
+                s.error = e
+                ends = True
+            if ends:
                 finished.append(b)
                 continue
             tok_of[b] = nid
-        self._record_logprobs(tok_of)
+        rows = [b for b in tok_of if self.slots[b].cfg.logprobs is not None]
+        try:
+            self._record_logprobs(rows, tok_of)
+        except Exception as e:  # noqa: BLE001
+            for b in rows:
+                self.slots[b].error = e
+                finished.append(b)
+                del tok_of[b]
         for b, nid in tok_of.items():
             s = self.slots[b]
             s.out.append(nid)
@@ -449,10 +472,9 @@ class PagedBatchingEngine:
         self.stats["tokens_out"] += len(tok_of)
         return finished
 
-    def _record_logprobs(self, tok_of: Dict[int, int]):
-        """Log probabilities of this step's tokens, under the model's own
+    def _record_logprobs(self, rows: List[int], tok_of: Dict[int, int]):
+        """Log probabilities of the rows' next tokens, under the model's own
         distribution (before penalties and temperature)."""
-        rows = [b for b in tok_of if self.slots[b].cfg.logprobs is not None]
         if not rows:
             return
         k = min(max(self.slots[b].cfg.logprobs for b in rows),
@@ -510,6 +532,8 @@ class PagedBatchingEngine:
             self.step()
             for i, b in list(slot_of.items()):
                 if not self.slots[b].active:
+                    if self.slots[b].error is not None:
+                        raise self.slots[b].error
                     results[i] = self.slots[b].result
                     del slot_of[i]
             t += 1

@@ -204,9 +204,14 @@ class _ContinuousWorker:
                         item["err"] = e
                         item["evt"].set()
                     tracked.clear()
+                    for b, s in enumerate(self.eng.slots):
+                        if s.active:
+                            self.eng._retire(b)
             for b, (item, i) in list(tracked.items()):
                 s = self.eng.slots[b]
                 if not s.active and s.result is not None:
+                    if getattr(s, "error", None) is not None:
+                        item["err"] = s.error
                     item["out"][i] = (s.result, getattr(s, "logprobs", None))
                     del tracked[b]
                     if None not in item["out"]:

@@ -481,6 +481,77 @@ def test_server_paged(small_model, tokenizer):
     assert [c["text"] for c in got["choices"]] == [one["choices"][0]["text"]]
 
 
+def _worker(model, tokenizer, paged=True, **kw):
+    from luminaai_amd.inference.server import _ContinuousWorker
+    return _ContinuousWorker(model.eval(), tokenizer, max_len=64, paged=paged,
+                             **{"max_batch": 3, **kw})
+
+
+@pytest.mark.timeout(60)
+@pytest.mark.parametrize("paged", [True, False])
+def test_a_bad_request_leaves_the_server_as_it_was(small_model, tokenizer,
+                                                   paged):
+    """On a fresh server and on slots that were used before."""
+    w = _worker(small_model, tokenizer, paged)
+    want = GenerationEngine(small_model.eval(), tokenizer).generate([5, 6, 7],
+                                                                    _cfg(4))
+    for _ in range(4):                      # more than there are slots
+        with pytest.raises(Exception, match="unhashable|whole numbers"):
+            w.submit([1, 2, 3], GenerationConfig(stop_token_ids=[[1]]))
+        assert w.eng.n_active() == 0
+        assert w.submit([5, 6, 7], _cfg(4)) == want
+    if paged:
+        assert w.eng.cache.free_pages == w.eng.cache.pages
+
+
+@pytest.mark.timeout(60)
+def test_a_request_that_cannot_be_sampled_fails_alone(small_model, tokenizer):
+    """temperature is not a number: the answer beside it goes on."""
+    import threading
+    w = _worker(small_model, tokenizer)
+    want = GenerationEngine(small_model.eval(), tokenizer).generate([5, 6, 7],
+                                                                    _cfg(30))
+    got = []
+    first = threading.Event()
+    t = threading.Thread(target=lambda: got.append(
+        w.submit([5, 6, 7], _cfg(30), lambda _: first.set())))
+    t.start()
+    assert first.wait(30)
+    for n in (1, 2):
+        with pytest.raises(RuntimeError):
+            w.submit_n([1, 2], GenerationConfig(temperature=math.nan), n)
+    t.join(30)
+    assert got == [want]
+    assert w.submit([5, 6, 7], _cfg(30)) == want
+    assert w.eng.cache.free_pages == w.eng.cache.pages
+
+
+def test_engine_takes_nothing_for_a_request_it_refuses(small_model, tokenizer):
+    eng = _engine(small_model, tokenizer)
+    a = eng.admit([1, 2, 3], _cfg(4, logprobs=1))
+    free, slots = eng.cache.free_pages, eng.free_slots()
+    bad = GenerationConfig(stop_token_ids=["x"])
+    for call in (lambda: eng.admit([1, 2], bad), lambda: eng.fork(a, bad),
+                 lambda: eng.admit_many([[1], [2]], [None, bad]),
+                 lambda: eng.admit_many([[1], [2]], [None]),
+                 lambda: eng.admit_many([[1], [2]], None, [None])):
+        with pytest.raises(ValueError):
+            call()
+        assert (eng.cache.free_pages, eng.free_slots()) == (free, slots)
+        _check(eng.cache)
+    # what fails while a row's log probabilities are taken ends that row
+    b = eng.admit([4, 5], _cfg(4))
+    eng.slots[a].cfg.logprobs = "x"
+    while eng.n_active():
+        eng.step()
+    assert isinstance(eng.slots[a].error, TypeError)
+    assert eng.slots[a].result == [] and eng.slots[b].error is None
+    assert len(eng.slots[b].result) == 4
+    with pytest.raises(RuntimeError):
+        eng.run_to_completion([[1, 2]],
+                              GenerationConfig(temperature=math.nan))
+
+
 # ------------------------------------------------------------ on the GPU
 @pytest.fixture
 def gpu_model(tiny_config):
