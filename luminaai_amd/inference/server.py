@@ -17,6 +17,7 @@ Run: python serve.py --checkpoint PATH [--port 8000] [--quantize int8]
 from __future__ import annotations
 
 import json
+import math
 import queue
 import threading
 import time
@@ -28,6 +29,8 @@ from .engine import GenerationConfig, GenerationEngine
 
 
 def _gen_config(body: Dict) -> GenerationConfig:
+    """The request's generation options; raises TypeError or ValueError for
+    values that sampling would stumble over."""
     cfg = GenerationConfig.from_mode(body.get("mode", "standard"))
     if "max_tokens" in body:
         cfg.max_new_tokens = int(body["max_tokens"])
@@ -41,6 +44,14 @@ def _gen_config(body: Dict) -> GenerationConfig:
         cfg.repetition_penalty = float(body["repetition_penalty"])
     if "stop_token_ids" in body:
         cfg.stop_token_ids = list(body["stop_token_ids"])
+        if not all(type(t) is int for t in cfg.stop_token_ids):
+            raise ValueError("stop_token_ids must be whole numbers")
+    if not (math.isfinite(cfg.temperature) and math.isfinite(cfg.top_p)):
+        raise ValueError("temperature and top_p must be finite")
+    if 0 < cfg.temperature < 1e-6:          # logits / temperature would overflow
+        cfg.temperature = 0.0
+    if not 1e-3 <= cfg.repetition_penalty <= 1e3:
+        raise ValueError("repetition_penalty must be 0.001 to 1000")
     return cfg
 
 
@@ -280,14 +291,16 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
         return [(t, lp if cfg.logprobs is not None else None)
                 for t, lp in outs]
 
-    def _options(body: Dict, cfg: GenerationConfig):
-        """(n, refusal); other modes take one answer and ignore both fields."""
-        if serving != "paged":
-            return 1, None
+    def _options(body: Dict):
+        """(generation options, n, refusal); only paged serving takes more
+        than one answer and log probabilities, other modes ignore both."""
         try:
-            return _paged_options(body, cfg, max_batch), None
-        except (TypeError, ValueError) as e:
-            return 1, JSONResponse({"error": str(e)}, status_code=400)
+            cfg = _gen_config(body)
+            n = _paged_options(body, cfg, max_batch) \
+                if serving == "paged" else 1
+            return cfg, n, None
+        except (TypeError, ValueError, OverflowError) as e:
+            return None, 1, JSONResponse({"error": str(e)}, status_code=400)
 
     def _sse_stream(prompt_ids: List[int], cfg: GenerationConfig,
                     wrap, endpoint: str = "completions") -> StreamingResponse:
@@ -341,8 +354,7 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
     @app.post("/v1/completions")
     def completions(body: Dict):
         prompt = body.get("prompt", "")
-        cfg = _gen_config(body)
-        n, refusal = _options(body, cfg)
+        cfg, n, refusal = _options(body)
         if refusal is not None:
             return refusal
         ids = tokenizer.encode(prompt)
@@ -376,8 +388,7 @@ def create_app(model, tokenizer, model_name: str = "luminaai-amd",
     @app.post("/v1/chat/completions")
     def chat_completions(body: Dict):
         messages = body.get("messages", [])
-        cfg = _gen_config(body)
-        n, refusal = _options(body, cfg)
+        cfg, n, refusal = _options(body)
         if refusal is not None:
             return refusal
         ids: List[int] = []

@@ -1,6 +1,7 @@
 """Paged cache bookkeeping, paged serving, packed forwards and scoring (CPU), and
 the same runs on the kernels."""
 
+import json
 import math
 
 import pytest
@@ -550,6 +551,35 @@ def test_engine_takes_nothing_for_a_request_it_refuses(small_model, tokenizer):
     with pytest.raises(RuntimeError):
         eng.run_to_completion([[1, 2]],
                               GenerationConfig(temperature=math.nan))
+
+
+@pytest.mark.timeout(60)
+@pytest.mark.parametrize("serving", ["paged", "continuous", "dynamic"])
+def test_server_refuses_malformed_options(small_model, tokenizer, serving):
+    pytest.importorskip("fastapi")
+    from fastapi.testclient import TestClient
+    from luminaai_amd.inference.server import create_app
+    client = TestClient(create_app(small_model.eval(), tokenizer,
+                                   serving=serving, max_len=64, max_batch=2),
+                        raise_server_exceptions=False)
+    ask = {"/v1/completions": {"prompt": "hello"},
+           "/v1/chat/completions": {"messages": [{"role": "user",
+                                                  "content": "hi"}]}}
+    for path, body in ask.items():
+        for bad in ('"stop_token_ids": [[1]]', '"stop_token_ids": ["a"]',
+                    '"stop_token_ids": 3', '"stop_token_ids": null',
+                    '"temperature": NaN', '"temperature": Infinity',
+                    '"temperature": "warm"', '"max_tokens": null',
+                    '"max_tokens": 1e999', '"top_p": NaN',
+                    '"repetition_penalty": 0'):
+            text = json.dumps({"max_tokens": 2, **body})[:-1] + f", {bad}}}"
+            r = client.post(path, content=text,
+                            headers={"content-type": "application/json"})
+            assert r.status_code == 400, (path, bad, r.text)
+        for good in ({"temperature": 1e-30}, {"stop_token_ids": [1]},
+                     {"top_k": -1}):
+            r = client.post(path, json={"max_tokens": 2, **body, **good})
+            assert r.status_code == 200, (path, good, r.text)
 
 
 # ------------------------------------------------------------ on the GPU
