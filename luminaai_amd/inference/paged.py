@@ -320,13 +320,18 @@ class PagedBatchingEngine:
     def can_admit(self, prompt_len: int, n: int = 1) -> bool:
         """Whether a prompt and n - 1 forks of it fit now, each with room for
         its first token."""
-        if len(self.free_slots()) < n or prompt_len + 1 > self.max_len:
-            return False
-        c = self.cache
-        need = c.pages_for(prompt_len + 1)
-        if n > 1:        # the page that each of them writes into
-            need += n - 1
-        return need <= c.free_pages
+        return len(self.free_slots()) >= n and \
+            prompt_len + 1 <= self.max_len and \
+            self._pages_to_admit(prompt_len, n) <= self.cache.free_pages
+
+    def can_ever_admit(self, prompt_len: int, n: int = 1) -> bool:
+        """Whether they fit when nothing else is served."""
+        return n <= self.max_batch and prompt_len + 1 <= self.max_len and \
+            self._pages_to_admit(prompt_len, n) <= self.cache.pages
+
+    def _pages_to_admit(self, prompt_len: int, n: int) -> int:
+        # beside the prompt's, the page that each fork writes into
+        return self.cache.pages_for(prompt_len + 1) + n - 1
 
     # --------------------------------------------------------------- admit
     @torch.no_grad()

@@ -195,7 +195,9 @@ class _ContinuousWorker:
                 fits = self.eng.can_admit(len(item["ids"]), item["n"]) \
                     if self.paged else self.eng.can_admit(len(item["ids"]))
                 if not fits:
-                    if self.eng.n_active() == 0:
+                    if self.eng.n_active() == 0 or self.paged and \
+                            not self.eng.can_ever_admit(len(item["ids"]),
+                                                        item["n"]):
                         item["err"] = RuntimeError(
                             "prompt exceeds the serving context window")
                         item["evt"].set()

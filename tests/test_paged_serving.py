@@ -582,6 +582,74 @@ def test_server_refuses_malformed_options(small_model, tokenizer, serving):
             assert r.status_code == 200, (path, good, r.text)
 
 
+class _Gate:
+    """Lets the server's loop take one step at a time."""
+
+    def __init__(self, worker):
+        import threading
+        self.worker = worker
+        self.free = threading.Semaphore(0)
+        self.at = threading.Semaphore(0)       # the loop waits before a step
+        step = worker.eng.step
+
+        def gated():
+            self.at.release()
+            assert self.free.acquire(timeout=30)
+            return step()
+        worker.eng.step = gated
+        self.threads = []
+
+    def ask(self, ids, cfg, n=1):
+        """A request in a thread of its own; its result or exception."""
+        import threading
+        import time
+        got = []
+
+        def run():
+            try:
+                got.append(self.worker.submit_n(ids, cfg, n))
+            except Exception as e:  # noqa: BLE001
+                got.append(e)
+        before = self.worker.q.qsize()
+        busy = bool(self.threads)
+        self.threads.append(threading.Thread(target=run, daemon=True))
+        self.threads[-1].start()
+        while busy and self.worker.q.qsize() == before:  # in order of asking
+            time.sleep(0.001)
+        return got
+
+    def step(self, n=1):
+        for _ in range(n):
+            self.free.release()
+            assert self.at.acquire(timeout=30)
+
+    def run(self):
+        """Until every request is answered."""
+        for _ in range(1000):
+            self.free.release()
+        for t in self.threads:
+            t.join(30)
+            assert not t.is_alive()
+
+
+@pytest.mark.timeout(60)
+def test_server_refuses_what_never_fits_at_once(small_model, tokenizer):
+    """While another request is served."""
+    gate = _Gate(_worker(small_model, tokenizer))
+    a = gate.ask([5, 6], _cfg(40))
+    assert gate.at.acquire(timeout=30)
+    long = gate.ask([5] * 64, _cfg(2))          # max_len is 64
+    many = gate.ask([5, 6], _cfg(2), 4)         # of 3 slots
+    gate.step(3)
+    assert not a
+    for r in (long, many):
+        assert isinstance(r[0], RuntimeError) and "context" in str(r[0])
+    fits = gate.ask([5] * 63, _cfg(5))
+    gate.run()
+    # one more token finds room in the cache, and one is drawn behind it
+    assert len(a[0][0][0]) == 40 and len(fits[0][0][0]) == 2
+
+
 # ------------------------------------------------------------ on the GPU
 @pytest.fixture
 def gpu_model(tiny_config):
