@@ -202,6 +202,8 @@ class _ContinuousWorker:
                             "prompt exceeds the serving context window")
                         item["evt"].set()
                         pending.remove(item)
+                    elif self.paged:
+                        break       # nothing that came later overtakes it
                     continue
                 try:
                     self._admit(item, tracked)

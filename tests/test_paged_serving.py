@@ -650,6 +650,27 @@ def test_server_refuses_what_never_fits_at_once(small_model, tokenizer):
     assert len(a[0][0][0]) == 40 and len(fits[0][0][0]) == 2
 
 
+@pytest.mark.timeout(60)
+def test_server_keeps_the_order_of_arrival(small_model, tokenizer):
+    """A request for three answers waits for three slots, and single ones that
+    come later do not take them as they are freed."""
+    gate = _Gate(_worker(small_model, tokenizer))
+    eng = gate.worker.eng
+    a = gate.ask([5, 6], _cfg(3))
+    assert gate.at.acquire(timeout=30)
+    b = gate.ask([5, 7], _cfg(6))
+    gate.step()
+    three = gate.ask([5, 8], _cfg(4), 3)
+    ones = [gate.ask([5, i], _cfg(4)) for i in range(9, 14)]
+    gate.step(4)                                # a's slot is free again
+    assert a and not b and eng.n_active() == 1
+    gate.step(4)
+    assert b and eng.n_active() == 3 and eng.stats["admitted"] == 5
+    gate.run()
+    assert [len(t) for t, _ in three[0]] == [4, 4, 4]
+    assert all(len(o[0][0][0]) == 4 for o in ones)
+
+
 # ------------------------------------------------------------ on the GPU
 @pytest.fixture
 def gpu_model(tiny_config):
