@@ -254,6 +254,10 @@ class PagedKVCache:
         return self._layers(step)
 
 
+# tokens of one packed prefill, whose activations and logits are held at once
+PREFILL_TOKENS = 32768
+
+
 class _Slot:
     __slots__ = ("active", "cfg", "stops", "recent", "out", "cb", "done",
                  "result", "logprobs", "error")
@@ -320,9 +324,20 @@ class PagedBatchingEngine:
     def can_admit(self, prompt_len: int, n: int = 1) -> bool:
         """Whether a prompt and n - 1 forks of it fit now, each with room for
         its first token."""
-        return len(self.free_slots()) >= n and \
-            prompt_len + 1 <= self.max_len and \
-            self._pages_to_admit(prompt_len, n) <= self.cache.free_pages
+        return self.admissible([(prompt_len, n)]) == 1
+
+    def admissible(self, requests: Sequence[Tuple[int, int]]) -> int:
+        """How many of these (prompt length, answers), from the first on, fit
+        now and go through one prefill: up to PREFILL_TOKENS, or one prompt."""
+        slots, pages, tokens = len(self.free_slots()), self.cache.free_pages, 0
+        for i, (length, n) in enumerate(requests):
+            slots -= n
+            pages -= self._pages_to_admit(length, n)
+            tokens += length
+            if slots < 0 or pages < 0 or length + 1 > self.max_len or \
+                    i and tokens > PREFILL_TOKENS:
+                return i
+        return len(requests)
 
     def can_ever_admit(self, prompt_len: int, n: int = 1) -> bool:
         """Whether they fit when nothing else is served."""
@@ -519,14 +534,9 @@ class PagedBatchingEngine:
         waiting = sorted(range(n), key=lambda i: sched[i])
         t = 0
         while None in results:
-            now, pages = [], 0
-            for i in waiting:
-                size = min(len(requests[i]), self.max_len - 1)
-                pages += self.cache.pages_for(size + 1)
-                if sched[i] > t or len(now) >= len(self.free_slots()) \
-                        or pages > self.cache.free_pages:
-                    break
-                now.append(i)
+            now = [i for i in waiting if sched[i] <= t]
+            now = now[:self.admissible(
+                [(min(len(requests[i]), self.max_len - 1), 1) for i in now])]
             if not now and not slot_of and sched[waiting[0]] <= t:
                 raise RuntimeError("the page pool does not hold a prompt of "
                                    f"{len(requests[waiting[0]])} tokens")

@@ -165,11 +165,63 @@ class _ContinuousWorker:
             raise item["err"]
         return item["out"]
 
-    def _admit(self, item: Dict, tracked: Dict):
-        b = self.eng.admit(item["ids"], item["cfg"], item.get("cb"))
-        tracked[b] = (item, 0)
-        for i in range(1, item["n"]):
-            tracked[self.eng.fork(b)] = (item, i)
+    @staticmethod
+    def _refuse(item: Dict, err: Exception):
+        item["err"] = err
+        item["evt"].set()
+
+    def _admit(self, items: List[Dict], tracked: Dict):
+        """Prefills the requests together (paged) or the only one."""
+        try:
+            if self.paged:
+                slots = self.eng.admit_many([i["ids"] for i in items],
+                                            [i["cfg"] for i in items],
+                                            [i["cb"] for i in items])
+            else:
+                slots = [self.eng.admit(i["ids"], i["cfg"], i["cb"])
+                         for i in items]
+        except Exception as e:  # noqa: BLE001
+            if len(items) == 1:
+                self._refuse(items[0], e)
+            else:                       # one of them is at fault
+                for item in items:
+                    self._admit([item], tracked)
+            return
+        for item, b in zip(items, slots):
+            tracked[b] = (item, 0)
+            try:
+                for i in range(1, item["n"]):
+                    tracked[self.eng.fork(b)] = (item, i)
+            except Exception as e:  # noqa: BLE001
+                self._refuse(item, e)
+
+    def _admit_in_order(self, pending: List[Dict], tracked: Dict):
+        """paged: all requests from the first on that fit now; what comes later
+        does not overtake one that has to wait."""
+        for item in list(pending):
+            if not self.eng.can_ever_admit(len(item["ids"]), item["n"]):
+                pending.remove(item)
+                self._refuse(item, RuntimeError(
+                    "prompt exceeds the serving context window"))
+        while True:
+            n = self.eng.admissible([(len(i["ids"]), i["n"])
+                                     for i in pending])
+            if n == 0:
+                return
+            items = pending[:n]
+            del pending[:n]
+            self._admit(items, tracked)
+
+    def _admit_any(self, pending: List[Dict], tracked: Dict):
+        """continuous: each request that fits now."""
+        for item in list(pending):
+            if self.eng.can_admit(len(item["ids"])):
+                pending.remove(item)
+                self._admit([item], tracked)
+            elif self.eng.n_active() == 0:
+                pending.remove(item)
+                self._refuse(item, RuntimeError(
+                    "prompt exceeds the serving context window"))
 
     def _loop(self):
         # slot -> (request, which of its answers)
@@ -191,33 +243,16 @@ class _ContinuousWorker:
                     pending.append(self.q.get_nowait())
                 except queue.Empty:
                     break
-            for item in list(pending):
-                fits = self.eng.can_admit(len(item["ids"]), item["n"]) \
-                    if self.paged else self.eng.can_admit(len(item["ids"]))
-                if not fits:
-                    if self.eng.n_active() == 0 or self.paged and \
-                            not self.eng.can_ever_admit(len(item["ids"]),
-                                                        item["n"]):
-                        item["err"] = RuntimeError(
-                            "prompt exceeds the serving context window")
-                        item["evt"].set()
-                        pending.remove(item)
-                    elif self.paged:
-                        break       # nothing that came later overtakes it
-                    continue
-                try:
-                    self._admit(item, tracked)
-                except Exception as e:  # noqa: BLE001
-                    item["err"] = e
-                    item["evt"].set()
-                pending.remove(item)
+            if self.paged:
+                self._admit_in_order(pending, tracked)
+            else:
+                self._admit_any(pending, tracked)
             if self.eng.n_active():
                 try:
                     self.eng.step()
                 except Exception as e:  # noqa: BLE001
                     for item, _ in tracked.values():
-                        item["err"] = e
-                        item["evt"].set()
+                        self._refuse(item, e)
                     tracked.clear()
                     for b, s in enumerate(self.eng.slots):
                         if s.active:

@@ -632,6 +632,15 @@ class _Gate:
             assert not t.is_alive()
 
 
+def _got(answers):
+    """What the thread of a request was answered."""
+    import time
+    end = time.monotonic() + 30
+    while not answers and time.monotonic() < end:
+        time.sleep(0.001)
+    return answers[0]
+
+
 @pytest.mark.timeout(60)
 def test_server_refuses_what_never_fits_at_once(small_model, tokenizer):
     """While another request is served."""
@@ -643,7 +652,7 @@ def test_server_refuses_what_never_fits_at_once(small_model, tokenizer):
     gate.step(3)
     assert not a
     for r in (long, many):
-        assert isinstance(r[0], RuntimeError) and "context" in str(r[0])
+        assert isinstance(_got(r), RuntimeError) and "context" in str(r[0])
     fits = gate.ask([5] * 63, _cfg(5))
     gate.run()
     # one more token finds room in the cache, and one is drawn behind it
@@ -663,12 +672,57 @@ def test_server_keeps_the_order_of_arrival(small_model, tokenizer):
     three = gate.ask([5, 8], _cfg(4), 3)
     ones = [gate.ask([5, i], _cfg(4)) for i in range(9, 14)]
     gate.step(4)                                # a's slot is free again
-    assert a and not b and eng.n_active() == 1
+    assert _got(a) and not b and eng.n_active() == 1
     gate.step(4)
-    assert b and eng.n_active() == 3 and eng.stats["admitted"] == 5
+    assert _got(b) and eng.n_active() == 3 and eng.stats["admitted"] == 5
     gate.run()
     assert [len(t) for t, _ in three[0]] == [4, 4, 4]
     assert all(len(o[0][0][0]) == 4 for o in ones)
+
+
+@pytest.mark.timeout(60)
+def test_server_prefills_together_what_comes_together(small_model, tokenizer):
+    """One forward for the prompts that wait, forks besides; a bad one among
+    them does not take the others along, and what never fits is refused though
+    another waits before it."""
+    gate = _Gate(_worker(small_model, tokenizer, max_batch=6))
+    eng = gate.worker.eng
+    sizes, admit = [], eng.admit_many
+    eng.admit_many = lambda p, *a: sizes.append(len(p)) or admit(p, *a)
+    solo = GenerationEngine(small_model.eval(), tokenizer)
+    a = gate.ask([5, 6], _cfg(12))
+    assert gate.at.acquire(timeout=30)
+    prompts = [[7, 8, 9], [10], [11] * 20]
+    got = [gate.ask(p, _cfg(4), n) for p, n in zip(prompts, (1, 2, 1))]
+    gate.step()
+    assert sizes == [1, 3] and eng.n_active() == 5
+    gate.step(6)
+    assert all(_got(g) for g in got) and not a
+    late = [gate.ask([12], _cfg(4)), gate.ask([10 ** 6], _cfg(4)),
+            gate.ask([13], _cfg(4), 6), gate.ask([3] * 70, _cfg(4))]
+    gate.step()
+    assert sizes == [1, 3, 2, 1, 1] and eng.n_active() == 2
+    assert isinstance(_got(late[1]), ValueError)
+    assert isinstance(_got(late[3]), RuntimeError)
+    gate.run()
+    for p, g in zip([[5, 6], *prompts, [12], [13]], [a, *got, late[0],
+                                                     late[2]]):
+        want = solo.generate(p, _cfg(len(g[0][0][0])))
+        assert all(t == want for t, _ in g[0])
+
+
+def test_a_prefill_holds_so_many_tokens(small_model, tokenizer, monkeypatch):
+    from luminaai_amd.inference import paged
+    monkeypatch.setattr(paged, "PREFILL_TOKENS", 30)
+    eng = _engine(small_model, tokenizer)
+    assert eng.admissible([(20, 1), (10, 1), (1, 1)]) == 2
+    assert eng.admissible([(40, 1), (1, 1)]) == 1
+    assert eng.admissible([(5, 3), (5, 1), (5, 1)]) == 2
+    assert eng.admissible([(64, 1)]) == eng.admissible([]) == 0
+    prompts = [[5] * 20, [6] * 12, [7] * 3]
+    outs = eng.run_to_completion(prompts, _cfg(3))
+    solo = GenerationEngine(small_model.eval(), tokenizer)
+    assert outs == [solo.generate(p, _cfg(3)) for p in prompts]
 
 
 # ------------------------------------------------------------ on the GPU
