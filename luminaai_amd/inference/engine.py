@@ -420,8 +420,9 @@ class GenerationEngine:
         groups: List[List[List[int]]] = []
         room = 0
         for s in sequences:
-            # a forward over up to 32768 tokens, or one sequence
-            if not packed or len(s) > room:
+            # a forward over up to 32768 tokens and as many sequences, or one
+            if not groups or not packed or len(s) > room or \
+                    len(groups[-1]) == 32768:
                 groups.append([])
                 room = 32768
             groups[-1].append(s)

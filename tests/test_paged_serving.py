@@ -422,6 +422,25 @@ def test_scores_do_not_depend_on_the_batch(small_model, tokenizer):
                               torch.tensor(alone[i % 3]), atol=1e-4)
 
 
+def test_scores_of_empty_sequences(small_model, tokenizer):
+    """Wherever they stand, and more of them than a packed row takes."""
+    solo = GenerationEngine(small_model.eval(), tokenizer)
+    want = solo.score([[1, 2]])[0]["logprobs"]
+    assert solo.score([]) == []
+    for seqs in ([[]], [[], [1, 2]], [[1, 2], []], [[], [], [1, 2], [5], []]):
+        out = solo.score(seqs, top_k=2)
+        assert [len(o["logprobs"]) for o in out] == \
+            [max(0, len(s) - 1) for s in seqs]
+        assert [len(o["top_ids"]) for o in out] == \
+            [max(0, len(s) - 1) for s in seqs]
+        for s, o in zip(seqs, out):
+            if s == [1, 2]:
+                assert abs(o["logprobs"][0] - want[0]) < 1e-5
+    out = solo.score([[1, 2]] + [[]] * 65536 + [[1, 2]])
+    assert len(out) == 65538
+    assert abs(out[-1]["logprobs"][0] - want[0]) < 1e-5
+
+
 def test_alternatives_of_a_small_vocabulary(tiny_config, tokenizer):
     from luminaai_amd.models import (DeepSeekTransformer,
                                      config_to_deepseek_config)
