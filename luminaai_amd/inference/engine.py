@@ -409,12 +409,13 @@ class GenerationEngine:
         entropy of the distribution that it was drawn from, and the top_k
         alternatives there (ops.token_logprobs). The sequences go through the
         model packed, in one row without padding; one by one where the model
-        does not take them so (mixture-of-depths layers; on the GPU, other
-        types than bf16)."""
+        does not take them so (mixture-of-depths layers, head_dim above 192;
+        on the GPU, other types than bf16)."""
         from .. import ops
         self.model.eval()
         p = next(self.model.parameters())
-        packed = not any(l.use_mod for l in self.model.layers) and \
+        packed = not any(l.use_mod or l.attention.head_dim > 192
+                         for l in self.model.layers) and \
             (self.device.type != "cuda" or p.dtype == torch.bfloat16)
         check_tokens(sequences, self.model)
         groups: List[List[List[int]]] = []

@@ -441,6 +441,20 @@ def test_scores_of_empty_sequences(small_model, tokenizer):
     assert abs(out[-1]["logprobs"][0] - want[0]) < 1e-5
 
 
+def test_scores_one_by_one_for_wide_heads(tiny_config, tokenizer):
+    from luminaai_amd.models import (DeepSeekTransformer,
+                                     config_to_deepseek_config)
+    tiny_config.hidden_size, tiny_config.num_heads = 400, 2
+    tiny_config.num_kv_heads = 1                       # heads of 200
+    torch.manual_seed(0)
+    m = DeepSeekTransformer(config_to_deepseek_config(tiny_config)).eval()
+    out = GenerationEngine(m, tokenizer).score([[], [1, 2, 3], [4, 5]])
+    assert [len(o["logprobs"]) for o in out] == [0, 2, 1]
+    with torch.no_grad():
+        lp = m(torch.tensor([[1, 2, 3]]))[0][0].float().log_softmax(-1)
+    assert abs(out[1]["logprobs"][1] - float(lp[1, 3])) < 1e-5
+
+
 def test_alternatives_of_a_small_vocabulary(tiny_config, tokenizer):
     from luminaai_amd.models import (DeepSeekTransformer,
                                      config_to_deepseek_config)
