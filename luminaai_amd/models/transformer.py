@@ -578,8 +578,7 @@ class MoEFFNLayer(nn.Module):
     def forward(self, x, seqs: Optional["_Sequences"] = None
                 ) -> Tuple[torch.Tensor, torch.Tensor]:
         """x: [B, S, h] -> (out [B, S, h], aux_loss scalar). seqs: the tokens
-        belong to sequences that have nothing to do with each other, and each
-        has the capacity that it would have alone."""
+        are those of packed or paged sequences."""
         B, S, h = x.shape
         N = B * S
         xf = x.reshape(N, h)
@@ -602,21 +601,21 @@ class MoEFFNLayer(nn.Module):
         # MoERoutingPlan — no atomics, no host sync, hipGraph-capturable).
         # `placement` (load balancer, parallel/load_balance.py) maps expert
         # id -> bucket slot so hot experts spread across EP ranks.
-        C = max(1, int(math.ceil(N * k / E * self.capacity_factor)))
+        tokens = N if seqs is None else seqs.tokens
+        C = max(1, int(math.ceil(tokens * k / E * self.capacity_factor)))
         placement = getattr(self, "placement", None)
         route_idx = topi if placement is None else placement[topi]
-        if seqs is None:
-            plan = ops.interface.moe_routing_plan(route_idx, E, C)
-        elif seqs.lens is None:
-            # a token's experts differ: one token is never dropped
-            C = N
-            plan = ops.interface.moe_routing_plan(route_idx, E, C)
-        else:
-            limit = (seqs.lens.double() * k / E * self.capacity_factor) \
-                .ceil().clamp(min=1).long()
-            C = min(N, C + limit.shape[0])           # room for all of them
-            plan = ops.interface.moe_routing_plan(route_idx, E, C, seqs.seq,
-                                                  limit)
+        limit = None
+        if seqs is not None and seqs.alone:
+            # a token's experts differ: no bucket takes more than all of them
+            C = min(tokens, C + seqs.count)
+            if seqs.lens is not None:
+                limit = (seqs.lens.double() * k / E * self.capacity_factor) \
+                    .ceil().clamp(min=1).long()
+            else:
+                C = tokens
+        plan = ops.interface.moe_routing_plan(
+            route_idx, E, C, None if limit is None else seqs.seq, limit)
         counts = plan.counts if placement is None \
             else plan.counts[placement]        # back to per-expert order
         bufv = ops.interface.moe_dispatch(xf, plan).view(E, C, h)
@@ -811,17 +810,35 @@ class MoEFFNLayer(nn.Module):
 
 
 class _Sequences(NamedTuple):
-    """Which sequence each token of a forward belongs to (MoEFFNLayer)."""
+    """Packed or paged sequences of a forward, for the experts' capacity
+    (MoEFFNLayer). Ranks that exchange tokens hold rows of different lengths and
+    need buckets of one size: `tokens` and `count` are the largest among them."""
 
-    seq: Optional[torch.Tensor]     # [T] long; None: every token is its own
-    lens: Optional[torch.Tensor]    # [n + 1] long, the rest of the row last
+    tokens: int                             # of the row
+    count: int                              # sequences, the rest of the row one
+    alone: bool                             # each has a capacity of its own
+    seq: Optional[torch.Tensor] = None      # [T] long: a token's sequence
+    lens: Optional[torch.Tensor] = None     # [count] long; None: one token each
 
     @classmethod
-    def packed(cls, cu_seqlens: torch.Tensor, total: int) -> "_Sequences":
-        tok = torch.arange(total, dtype=torch.int32, device=cu_seqlens.device)
-        seq = torch.searchsorted(cu_seqlens[1:].contiguous(), tok, right=True)
-        ends = F.pad(cu_seqlens.long(), (0, 1), value=total)
-        return cls(seq, ends.diff().clamp(0, total))
+    def of(cls, cu_seqlens: Optional[torch.Tensor], tokens: int, alone: bool,
+           ep_group, device) -> "_Sequences":
+        count = tokens if cu_seqlens is None else cu_seqlens.shape[0]
+        seq = lens = None
+        if alone and cu_seqlens is not None:
+            tok = torch.arange(tokens, dtype=torch.int32, device=device)
+            seq = torch.searchsorted(cu_seqlens[1:].contiguous(), tok,
+                                     right=True)
+            ends = F.pad(cu_seqlens.long(), (0, 1), value=tokens)
+            lens = ends.diff().clamp(0, tokens)
+        if ep_group is not None:
+            import torch.distributed as dist
+            if "nccl" not in dist.get_backend(ep_group):
+                device = "cpu"
+            most = torch.tensor([tokens, count], device=device)
+            dist.all_reduce(most, op=dist.ReduceOp.MAX, group=ep_group)
+            tokens, count = most.tolist()
+        return cls(tokens, count, alone, seq, lens)
 
 
 # ======================================================================
@@ -1069,11 +1086,11 @@ class DeepSeekTransformer(nn.Module):
         # none of them takes the experts' capacity from another. In training the
         # row shares it, as a padded batch does.
         seqs = None
-        if not self.training and any(l.is_moe for l in self.layers):
-            if cu_seqlens is not None:
-                seqs = _Sequences.packed(cu_seqlens, S)
-            elif paged:
-                seqs = _Sequences(None, None)
+        moe = [l.ffn for l in self.layers if l.is_moe]
+        if moe and (cu_seqlens is not None or paged):
+            ep = next((f.ep_group for f in moe if f.ep_size > 1), None)
+            seqs = _Sequences.of(cu_seqlens, B * S, not self.training, ep,
+                                 x.device)
 
         total_aux = x.new_zeros(())
         aux_losses: Dict[str, torch.Tensor] = {}
@@ -1083,7 +1100,7 @@ class DeepSeekTransformer(nn.Module):
             if self.gradient_checkpointing and self.training and cache is None:
                 x, aux = torch.utils.checkpoint.checkpoint(
                     layer, x, rope_cs, pos, pos_offset, None, attn_mask,
-                    cu_seqlens, use_reentrant=False)
+                    cu_seqlens, seqs, use_reentrant=False)
             else:
                 x, aux = layer(x, rope_cs, pos, pos_offset, cache, attn_mask,
                                cu_seqlens, seqs)

@@ -9,7 +9,8 @@ which is single-link bound.
 
 The exchanged buffers are capacity-bucketed and therefore STATIC-SHAPED
 ([ep, E_local, C, h]) — no length metadata exchange, no host syncs, and the
-pattern is hipGraph-capturable.
+pattern is hipGraph-capturable. Packed rows, whose lengths differ from rank to rank,
+agree on C once a forward (models/transformer.py _Sequences).
 """
 
 from __future__ import annotations

@@ -326,6 +326,133 @@ def test_zero2_matches_ddp():
 
 
 # ---- expert load balancing -------------------------------------------------
+def _packed_row(rank, step=0, lens=((30, 10), (5, 41, 1, 17))):
+    """Rows of 40 and 64 tokens, of different numbers of sequences."""
+    g = torch.Generator().manual_seed(50 + 2 * step + rank)
+    lens = lens[(rank + step) % 2]
+    ids = torch.randint(1, 512, (1, sum(lens)), generator=g)
+    labels = torch.randint(1, 512, (1, sum(lens)), generator=g)
+    cu = torch.tensor([0, *lens], dtype=torch.int32).cumsum(0).int()
+    return ids, labels, cu
+
+
+def _packed_moe(factor, checkpointing=False):
+    """The whole model and, with a mesh, this rank's shard of it."""
+    from luminaai_amd.models import DeepSeekTransformer
+    from luminaai_amd.parallel.mesh import init_mesh, reset_mesh
+    mcfg = _moe_model_cfg()
+    mcfg.capacity_factor = factor
+    torch.manual_seed(7)
+    full = DeepSeekTransformer(mcfg)
+    mesh = init_mesh(ep_size=2)
+    model = DeepSeekTransformer(mcfg)
+    model.gradient_checkpointing = checkpointing
+    EL = model.layers[0].ffn.num_local_experts
+    lo = mesh.ep_rank * EL
+    with torch.no_grad():
+        for (_, p), (_, q) in zip(model.named_parameters(),
+                                  full.named_parameters()):
+            p.copy_(q if p.shape == q.shape else q[lo:lo + EL])
+    reset_mesh()
+    return full, model, lo, EL
+
+
+def _packed_loss(m, row):
+    import torch.nn.functional as F
+    ids, labels, cu = row
+    logits, aux, _ = m(ids, cu_seqlens=cu)
+    return F.cross_entropy(logits[0].float(), labels[0]) + aux
+
+
+def ep_packed_worker(rank, world):
+    """Rows of different lengths on the two ranks: loss and gradients are those
+    of the whole model on each row, where nothing is dropped (a bucket holds
+    every token of the longest row)."""
+    for checkpointing in (False, True):
+        full, model, lo, EL = _packed_moe(4.0, checkpointing)
+        model.train()
+        full.train()
+        loss = _packed_loss(model, _packed_row(rank))
+        loss.backward()
+        want = _packed_loss(full, _packed_row(rank))
+        assert abs(float(loss) - float(want)) < 1e-5
+        want.backward()
+        mine = {n: p.grad.clone() for n, p in full.named_parameters()}
+        _packed_loss(full, _packed_row(1 - rank)).backward()   # adds up
+        for n, p in model.named_parameters():
+            if ".w_gate_up" in n or ".w_down" in n:
+                ref = dict(full.named_parameters())[n].grad[lo:lo + EL]
+            else:
+                ref = mine[n]
+            assert torch.allclose(p.grad, ref, atol=1e-5), n
+    # the eval rule: each sequence as it is alone, though many drop tokens
+    full, model, _, _ = _packed_moe(1.0)
+    full.eval()
+    model.eval()
+    ids, _, cu = _packed_row(rank)
+    with torch.no_grad():
+        out = model(ids, cu_seqlens=cu)[0][0]
+        for a, b in zip(cu.tolist(), cu[1:].tolist()):
+            alone = full(ids[:, a:b])[0][0]
+            assert torch.allclose(out[a:b], alone, atol=1e-4)
+    return True
+
+
+def ep_packed_train_worker(rank, world):
+    """Trainer steps and an evaluation over packed batches of each rank's own
+    lengths."""
+    from luminaai_amd.config import Config
+    from luminaai_amd.data import pack_collate
+    from luminaai_amd.data.tokenizer import ConversationTokenizer
+    from luminaai_amd.models import (DeepSeekTransformer,
+                                     config_to_deepseek_config)
+    from luminaai_amd.parallel.mesh import init_mesh, reset_mesh
+    from luminaai_amd.training import Trainer
+    cfg = Config(vocab_size=512, hidden_size=64, num_layers=2, num_heads=4,
+                 num_kv_heads=2, seq_length=64, intermediate_size=128,
+                 micro_batch_size=2, gradient_accumulation_steps=1,
+                 num_workers=0, use_moe=True, num_experts=4, moe_top_k=2,
+                 use_mod=False, zero_stage=1, precision="fp32",
+                 pack_sequences=True, experiment_name=f"ep_packed_{rank}",
+                 eval_every_n_batches=0, save_every_n_batches=0)
+    init_mesh(ep_size=2)
+    torch.manual_seed(99)
+    t = Trainer(DeepSeekTransformer(config_to_deepseek_config(cfg)),
+                ConversationTokenizer(), cfg)
+    t._setup_scheduler(10)
+    batches = []
+    for step in range(3):
+        ids, labels, cu = _packed_row(rank, step)
+        cut = [(a, b) for a, b in zip(cu.tolist(), cu[1:].tolist())]
+        batches.append(pack_collate([
+            {"input_ids": ids[0, a:b], "labels": labels[0, a:b],
+             "loss_weights": torch.ones(b - a)} for a, b in cut]))
+    t.engine.set_sync(True)
+    losses = []
+    for batch in batches:
+        losses.append(float(t.train_step(batch)["ce_loss"]))
+        t.optimizer_step()
+    res = t.evaluate(batches)
+    norm = t.optimizer.last_grad_norm()
+    emb = float(t.model.embed_tokens.weight.detach().double().sum())
+    reset_mesh()
+    return {"losses": losses, "eval": res["loss"], "norm": norm, "emb": emb}
+
+
+def test_ep_packed_rows_of_different_lengths():
+    assert _spawn("ep_packed_worker") == {0: True, 1: True}
+
+
+def test_ep_packed_training():
+    res = _spawn("ep_packed_train_worker")
+    for r in range(WORLD):
+        assert all(torch.isfinite(torch.tensor(v)).all()
+                   for v in res[r].values())
+    # the shared weights and the norm agree
+    assert res[0]["emb"] == pytest.approx(res[1]["emb"], abs=1e-6)
+    assert res[0]["norm"] == pytest.approx(res[1]["norm"], rel=1e-5)
+
+
 def ep_load_balance_worker(rank, world):
     """Applying a non-trivial placement must not change model outputs."""
     from luminaai_amd.models import DeepSeekTransformer
