@@ -231,6 +231,7 @@ void paged_attn_kernel(const PagedAttnArgs a) {
   #pragma unroll
   for (int i = 0; i < 2 * NDW; ++i) oacc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m = -FLT_MAX, l = 0.f;             // below every score
+  bool seen = false;                       // a token, whatever its score
   const int* tb = a.table + (int64_t)b * a.table_sb;
   const int pmask = (1 << a.page_shift) - 1;
   const uint16_t* kh = a.k + hkv * a.k_sh;
@@ -248,6 +249,7 @@ void paged_attn_kernel(const PagedAttnArgs a) {
       const int tt = t0 + 16 * i <= last ? t0 + 16 * i : (last & ~15);
       const int pg = tb[tt >> a.page_shift];
       ok[i] = pg >= 0 && pg < a.P;
+      seen |= ok[i] && t0 + 16 * i < t_end;
       const int64_t pgc = ok[i] ? pg : 0;
       const uint16_t* kp = kh + pgc * a.k_sp;
       const uint16_t* vp = vh + pgc * a.v_sp;
@@ -340,14 +342,16 @@ void paged_attn_kernel(const PagedAttnArgs a) {
     }
   }
 
-  // ---- join the four waves: LDS holds [wave][head of 16][2 + D]
+  // ---- join the four waves: LDS holds [wave][head of 16][2 + D]. A part without
+  // tokens has -inf as its maximum. No tokens at all give zeros; tokens whose scores
+  // are all -inf have no softmax: 0 / 0.
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
   const int nh = G - (int)hg * 16 < 16 ? G - (int)hg * 16 : 16;
   const int rowf = a.D + 2;
   if (c16 < nh) {
     float* row = lds + ((int64_t)wave * nh + c16) * rowf;
-    if (g == 0) { row[0] = m; row[1] = l; }
+    if (g == 0) { row[0] = seen ? m : -INFINITY; row[1] = l; }
     #pragma unroll
     for (int i = 0; i < 2 * NDW; ++i)
       #pragma unroll
@@ -359,12 +363,13 @@ void paged_attn_kernel(const PagedAttnArgs a) {
   __syncthreads();
   for (int i = threadIdx.x; i < nh * a.D; i += 256) {
     const int hh = i / a.D, d = i - hh * a.D;
-    float mw[4], mm = -FLT_MAX;
+    float mw[4], top = -INFINITY;
     #pragma unroll
     for (int w = 0; w < 4; ++w) {
       mw[w] = lds[(w * nh + hh) * rowf];
-      mm = fmaxf(mm, mw[w]);
+      top = fmaxf(top, mw[w]);
     }
+    const float mm = fmaxf(top, -FLT_MAX);
     float ls = 0.f, os = 0.f;
     #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -374,14 +379,13 @@ void paged_attn_kernel(const PagedAttnArgs a) {
     }
     const int head = hkv * G + (int)hg * 16 + hh;
     if (count == 1) {
-      // an empty sequence gives zeros
       a.o[((int64_t)b * a.H + head) * a.D + d] =
-          f32_to_bf16(ls == 0.f ? 0.f : os / ls);
+          f32_to_bf16(top == -INFINITY ? 0.f : os / ls);
     } else {
       const int64_t at = (int64_t)item * a.H + head;
       a.part[at * a.D + d] = os;
       if (d == 0) {
-        a.ml[at * 2] = mm;
+        a.ml[at * 2] = top;
         a.ml[at * 2 + 1] = ls;
       }
     }
@@ -407,6 +411,7 @@ void paged_attn_join_kernel(const PagedAttnArgs a) {
   const float* part = a.part + first * a.D;
   const int64_t step = a.H;                    // from chunk to chunk
   float m = -FLT_MAX, l = 0.f, acc[3] = {0.f, 0.f, 0.f};
+  float top = -INFINITY;
   for (int s0 = wave; s0 < n; s0 += 4 * U) {
     float cm[U], cl[U], x[U][3];
     #pragma unroll
@@ -423,9 +428,9 @@ void paged_attn_join_kernel(const PagedAttnArgs a) {
       }
       if (!ok) cm[u] = -INFINITY;
     }
-    float mn = m;
     #pragma unroll
-    for (int u = 0; u < U; ++u) mn = fmaxf(mn, cm[u]);
+    for (int u = 0; u < U; ++u) top = fmaxf(top, cm[u]);
+    const float mn = fmaxf(m, top);
     const float f = __builtin_amdgcn_exp2f(m - mn);
     l *= f;
     #pragma unroll
@@ -443,11 +448,12 @@ void paged_attn_join_kernel(const PagedAttnArgs a) {
   for (int i = 0; i < 3; ++i)
     if (lane + 64 * i < a.D) so[wave][lane + 64 * i] = acc[i];
   if (lane == 0) {
-    sm[wave] = m;
+    sm[wave] = top;
     sl[wave] = l;
   }
   __syncthreads();
-  const float mm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  const float mm = fmaxf(top, -FLT_MAX);
   float g[4], ls = 0.f;
   #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -459,7 +465,7 @@ void paged_attn_join_kernel(const PagedAttnArgs a) {
     float os = 0.f;
     #pragma unroll
     for (int w = 0; w < 4; ++w) os += g[w] * so[w][d];
-    a.o[bh * a.D + d] = f32_to_bf16(ls == 0.f ? 0.f : os / ls);
+    a.o[bh * a.D + d] = f32_to_bf16(top == -INFINITY ? 0.f : os / ls);
   }
 }
 

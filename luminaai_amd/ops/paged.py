@@ -40,8 +40,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor,
     included); a table's row has room for fewer than 2^29 tokens, all together
     for 2^31. Returns [B, H, D] in q's type; a sequence of length 0 gives
     zeros. `scale` defaults to D ** -0.5. There is no gradient. Nothing behind
-    a sequence's end is read; a live value that is not finite makes its
-    sequence's result NaN or infinite."""
+    a sequence's end is read. A live token with a score of -inf has no weight; a
+    sequence of nothing else has no softmax and gives NaN, as do other scores
+    that are not finite."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if use_hip(q):

@@ -143,6 +143,29 @@ def test_paged_attention_large_scores(dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("D", [40, 64, 159])
+def test_scores_of_minus_infinity(dev, D):
+    """Such tokens have no weight, also where a chunk holds nothing else; a
+    sequence of nothing else has no softmax, unlike one without tokens."""
+    lens = [20, 20, 3000, 3000, 0, 1, 16]
+    q, k, v, table, n, dense = _scene(lens, 4, 2, D, 16, dev)
+    q = q.abs() + 0.25
+    live = [torch.ones(x, dtype=torch.bool) for x in lens]
+    live[0][:] = live[3][:] = live[5][:] = False        # all of them
+    live[1][[0, 1, 2, 5, 19]] = False
+    live[2][:2500] = False                              # whole chunks
+    for b, keep in enumerate(live):
+        for t in (~keep).nonzero()[:, 0].tolist():
+            k[table[b, t // 16].long(), :, t % 16, :D] = -math.inf
+    o = ops.paged_attention(q, k, v, table, n)
+    assert o[[0, 3, 5]].isnan().all()
+    ref, tol = _oracle(q, dense, D, live)
+    rest = [1, 2, 4, 6]
+    assert ((o.double().cpu() - ref).abs() <= tol)[rest].all()
+    assert (o[4] == 0).all()
+
+
+@pytest.mark.parametrize("dev", DEVS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16,
                                    torch.float32])
 @pytest.mark.parametrize("D,page", [(159, 16), (64, 128), (15, 32)])
