@@ -53,7 +53,7 @@ struct PackedArgs {
   uint16_t* dk;                // [T, HKV, D]
   uint16_t* dv;
   float* part;                 // [2 (dk, dv), splits, T, HKV, D up to 4]
-  float* lse;                  // [H, T], log2 units; +inf where nothing summed
+  float* lse;                  // [H, T], log2 units
   float* delta;                // [H, T]
   const int* cu;               // [B + 1]
   const int* list;             // packed_list_kernel's blocks, or null
@@ -574,14 +574,14 @@ void packed_fwd_kernel(const PackedArgs a) {
     for (int i = 0; i < 16 * DT; ++i)
       o[i / 16][i & 15] = o[i / 16][i & 15] * f0 + other[64 * i] * f1;
   }
+  // l is 0 where all of a query's scores are -inf: 0 / 0, as it has no softmax
   l += __shfl_xor(l, 32, 64);
   const int64_t tok = w.start + qi;
   const int64_t at = tok * a.H + h;
   store_col<DT>(a.out + at * a.D, a.rest ? a.rest + at * a.W : nullptr, o,
-                l == 0.f ? 0.f : 1.f / l, hi, a.D, a.W, qi < w.len);
+                1.f / l, hi, a.D, a.W, qi < w.len);
   if (a.lse && hi == 0 && qi < w.len)
-    a.lse[(int64_t)h * a.T + tok] =
-        l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    a.lse[(int64_t)h * a.T + tok] = m + __builtin_amdgcn_logf(l);
 }
 
 // ===========================================================================

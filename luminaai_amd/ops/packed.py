@@ -31,7 +31,9 @@ def flash_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     them, cuts them to T and computes nothing outside the tensors, and what such
     borders give is not defined.
 
-    Values that are not finite may reach earlier queries of their sequence."""
+    A query whose scores are all -inf has no softmax and gives NaN. Values that
+    are not finite may reach every query and gradient of their sequence, and no
+    other."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if use_hip(q):

@@ -211,6 +211,33 @@ def test_late_maximum(dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [40, 900])
+def test_scores_of_minus_infinity(dev, D, n):
+    """A query with nothing else has no softmax; for the others such keys have
+    no weight; other sequences do not notice, nor do their gradients."""
+    lens = [20, n, 30]
+    q, k, v, go = _inputs(lens, 0, 4, 2, D, dev, seed=n)
+    q = q.abs() + 0.25
+    k = k.clone()
+    cu = _cu(lens, dev)
+    plain = _run(q, k, v, go, cu)
+    dead = n // 2
+    k[:20] = -math.inf
+    k[20:20 + dead] = -math.inf
+    got = _run(q, k, v, go, cu)
+    assert got[0][:20 + dead].isnan().all()
+    for a, b in zip(plain, got):
+        assert torch.equal(a[20 + n:], b[20 + n:])
+    # the oracle on the keys that are left, which sit behind the dead ones: each
+    # query sees those up to its own
+    left = slice(20 + dead, 20 + n)
+    val, tol = _oracle(q[left], k[left], v[left], go[left], [n - dead],
+                       D ** -0.5)
+    _check([got[0][left]], val[:1], tol[:1])
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_gradient_against_differences(dev):
     """sum(o go) at two points h apart along a direction, in 64 bits from the
     returned o, against the gradient's product with it. The difference is off by
