@@ -743,6 +743,11 @@ bool overlaps(const at::Tensor& t) {
   return false;
 }
 
+// t is written in place: autograd refuses a backward pass that saved it before.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Pages [P, HKV, page, W]; returns log2(page).
 int check_pages(const at::Tensor& t, const at::Tensor& like, const char* name,
                 int64_t heads, int64_t dim) {
@@ -909,6 +914,8 @@ void paged_append(const at::Tensor& k_, const at::Tensor& v_,
                                 (int)table.size(1), (int)k.element_size(),
                                 cur_stream()),
             "paged_kv_append");
+  written(kp);
+  written(vp);
 }
 
 void copy_pages(const std::vector<at::Tensor>& pools,
@@ -968,6 +975,7 @@ void copy_pages(const std::vector<at::Tensor>& pools,
                                 page_bytes(pools[i]), si.data(), di.data(),
                                 (int64_t)si.size(), cur_stream()),
               "copy_pages");
+    for (int j = 0; j < n; ++j) written(pools[i + j]);
     i += n;
   }
 }

@@ -272,6 +272,33 @@ def test_append_attend_fork(dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+def test_writes_are_seen_by_autograd(dev):
+    """A pool that a backward pass needs may not have been written since."""
+    k = torch.zeros(2, 6, 1, 16, 8, device=dev)
+    v = torch.zeros_like(k)
+    table = torch.zeros(1, 2, dtype=torch.int32, device=dev)
+    new = torch.ones(1, 1, 8, device=dev)
+    pos = torch.zeros(1, dtype=torch.int32, device=dev)
+    x = torch.ones(8, device=dev, requires_grad=True)
+    for write in (lambda: ops.paged_kv_append(new, new, k[0], v[0], table, pos),
+                  lambda: ops.copy_pages([k, v], [0], [1])):
+        for pool in (k, v):
+            before = pool._version
+            loss = (pool * x).sum()
+            write()
+            assert pool._version > before
+            with pytest.raises(RuntimeError, match="modified by an inplace"):
+                loss.backward()
+    # what was made in inference mode has no versions
+    with torch.inference_mode():
+        k, v = k.clone(), v.clone()
+        ops.paged_kv_append(new, new, k[0], v[0], table, pos)
+        ops.copy_pages([k, v], [0], [1])
+        # one row of 8 in page 0 and its copy in page 1
+        assert float(k.sum()) == float(v.sum()) == 16
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_refusals(dev):
     q, k, v, table, n, _ = _scene([20, 5], 4, 2, 64, 16, dev)
 
