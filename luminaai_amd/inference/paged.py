@@ -157,7 +157,8 @@ class PagedKVCache:
         """Slot dst continues what slot src holds, on the same pages."""
         if self.tables[dst]:
             raise ValueError(f"slot {dst} is in use")
-        self.tables[dst] = list(self.tables[src])
+        # room that was made ahead stays with src: nothing of it is written yet
+        self.tables[dst] = self.tables[src][:self.pages_for(self.lens[src])]
         self.lens[dst] = self.lens[src]
         for p in self.tables[dst]:
             self._refs[p] += 1

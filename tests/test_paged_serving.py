@@ -98,6 +98,29 @@ def test_cache_grow_fork_free_compact_resize():
     assert _read(c, 0) == [[5.0], [6.0]]
 
 
+@pytest.mark.parametrize("held", [0, 5, 16, 20])
+def test_room_made_ahead_is_not_shared(held):
+    """extend() takes pages before they are written; a fork shares what is
+    written and nothing else."""
+    c = _cache()
+    for t in range(held):
+        _write(c, 0, 100.0 + t)
+    c.extend([0], [40])
+    c.fork(0, 1)
+    used = [p for t in c.tables for p in t]
+    assert c._refs == [used.count(p) for p in range(c.pages)]
+    assert len(c.tables[1]) == c.pages_for(held)
+    for t in range(20):
+        _write(c, 0, 200.0 + t)
+        _write(c, 1, 300.0 + t)
+    base = [100.0 + t for t in range(held)]
+    assert _read(c, 0)[0] == base + [200.0 + t for t in range(20)]
+    assert _read(c, 1)[0] == base + [300.0 + t for t in range(20)]
+    c.free(0)
+    c.free(1)
+    assert c.free_pages == c.pages
+
+
 def test_cache_refusals_change_nothing():
     c = _cache(pages=2)
     c.prefill([0], [17])
