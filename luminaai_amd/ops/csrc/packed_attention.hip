@@ -997,12 +997,28 @@ static hipError_t launch_fwd(PackedArgs& a, int* list, hipStream_t stream) {
 
 template <int DP>
 static hipError_t run_fwd(PackedArgs& a, int* list, hipStream_t stream) {
-  // Two parts up to 512 blocks of 128 rows, which leave units idle and each other
-  // room, and not for the short sequences that 512 tokens can be. One / two parts,
-  // one sequence: 2048 tokens of 12:4 x 160 63.8 / 52.8 us, of 8:4 x 64 29.9 / 25.0,
-  // of 4:4 x 192 80 / 51, of 32:8 x 128 55.3 / 54.2, 1024 of these 26.8 / 24.2, 256
-  // 10.0 / 10.5; 8192 in four sequences 257 / 318.
-  if (a.T > 512 && (int64_t)a.T * a.H <= 65536)
+  // Two parts where few blocks leave units idle and a block's time is its chain of
+  // steps: there it is halved, while the wider steps and the join cost about 1 us. One
+  // / two parts, us:
+  //   1 sequence: 2048 tokens of 12:4 x 160 61.7 / 50.3, of 8:4 x 64 30.0 / 25.4, of
+  //     32:8 x 128 53.0 / 52.2, 8000 of 8:4 x 64 114 / 102
+  //   256 tokens each: 1024 of 12:4 x 160 13.3 / 13.3, of 32:8 x 128 11.3 / 11.8
+  //   338 each: 2708 of 2:1 x 64 9.3 / 8.6, of 2:2 x 128 12.4 / 12.2
+  //   512 each: 1024 of 32:8 x 128 16.1 / 15.9, 2048 of it 19.9 / 24.9
+  //   1000 each: 4000 of 12:4 x 160 37.7 / 35.5, 8000 of 8:4 x 64 19.4 / 21.8
+  //   64 each: 1024 of 8:4 x 64 5.2 / 6.4, of 32:8 x 128 8.8 / 17.2
+  // At 192 two parts are eight waves for 128 rows instead of 256 (4:4 heads): 125
+  // each 8000 15.7 / 15.2, 62 each 4000 11.0 / 11.5; 1000 each 16000 48.5 / 44.9, 500
+  // each 31.2 / 34.8.
+  // More than 64 sequences may be mostly empty ones, which fill up borders of a
+  // fixed size: then as long as one round of workgroups takes them (100 short ones
+  // of 2:1 x 64 8.6 / 9.6, of 4:2 x 64, 436 workgroups, 9.2 / 13.5).
+  const int64_t size = (int64_t)a.T * a.H;
+  const int each = a.T / (a.B > 1 ? a.B : 1);
+  const bool fits = a.B > 64 ? max_blocks(a, 128) * a.H <= 256
+      : (size <= 32768 && each >= (DP <= 160 ? 320 : 128))
+        || (size <= 65536 && each >= (DP <= 160 ? 1536 : 1000));
+  if (a.T > 512 && fits)
     return launch_fwd<DP, 2>(a, list, stream);
   return launch_fwd<DP, 1>(a, list, stream);
 }

@@ -238,6 +238,19 @@ def test_scores_of_minus_infinity(dev, D, n):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("H,HKV,D,lens", [
+    (8, 4, 64, [50] * 13), (8, 4, 64, [600, 700]), (8, 4, 64, [8, 900, 1] * 2),
+    (2, 1, 96, [10] * 70), (4, 2, 64, [10] * 70), (2, 2, 192, [130] * 5),
+    (2, 2, 192, [20] * 40)])
+def test_few_long_and_many_short(dev, H, HKV, D, lens):
+    """Both arrangements of the forward's waves, on either side of the sizes
+    that choose between them."""
+    q, k, v, go = _inputs(lens, 1, H, HKV, D, dev, seed=len(lens))
+    val, tol = _oracle(q, k, v, go, lens, D ** -0.5)
+    _check(_run(q, k, v, go, _cu(lens, dev)), val, tol)
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_gradient_against_differences(dev):
     """sum(o go) at two points h apart along a direction, in 64 bits from the
     returned o, against the gradient's product with it. The difference is off by
