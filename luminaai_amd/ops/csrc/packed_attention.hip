@@ -1147,9 +1147,11 @@ extern "C" hipError_t lumina_pack_rows(const void* const* src, void* const* dst,
   a.T = T;
   a.D = D;
   a.pieces = (D + 7) / 8;
-  // few tokens: a workgroup each, so that the call has enough of them. One / eight
-  // tokens a workgroup: 8192 tokens of 12:4:4 x 159 18.2 / 17.1 us.
-  a.per = T >= 4096 ? 8 : 1;
+  // Tokens of a workgroup: one, so that small calls have enough workgroups, or eight,
+  // which keep its threads busy. One / eight, with the forward behind it (sequences of
+  // 32), us: 12:4 x 159 64 tokens 9.3 / 11.3, 1024 17.2 / 18.6, 2048 27.4 / 26.7, 4096
+  // 40.8 / 39.5; 2:1 x 53 64 6.9 / 6.8, 1024 8.6 / 7.9, 4096 15.3 / 12.4.
+  a.per = T >= 2048 ? 8 : 1;
   for (int i = 0; i < n; ++i) {
     a.src[i] = (const uint16_t*)src[i];
     a.dst[i] = (uint16_t*)dst[i];

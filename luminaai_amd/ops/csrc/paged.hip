@@ -599,10 +599,13 @@ extern "C" hipError_t lumina_paged_append(
   a.P = P; a.B = B; a.HKV = HKV; a.D = D; a.chunks = W / 8;
   a.page_shift = page_shift; a.M = M;
   a.T = T;
-  // few tokens: a workgroup each, so that the call has enough of them. One / eight
-  // tokens a workgroup: 64 tokens of 8 x 128 3.3 / 5.7 us, 8179 of 4 x 159
-  // 14.5 / 10.5.
-  a.per = T >= 4096 ? 8 : 1;
+  // Tokens of a workgroup: one, so that small calls have enough workgroups, or eight,
+  // which keep its threads busy. One / eight, bf16, us: 8 x 128 64 tokens 2.7 / 4.7,
+  // 2048 5.4 / 6.2, 4096 8.4 / 8.8, 6000 12.0 / 11.5, 16384 27 / 23; 4 x 159 1024
+  // 3.7 / 4.5, 2048 5.2 / 5.2, 4096 8.0 / 6.7, 8192 14.3 / 10.2; 8 x 64 1536 3.7 /
+  // 3.9, 3000 5.0 / 4.8, 8192 9.7 / 7.9. fp32, written channel by channel: 4 x 64
+  // 1024 4.3 / 4.4, 3000 8.0 / 7.4, 8192 17.4 / 21.1.
+  a.per = elem_size == 2 && T >= (HKV * a.chunks <= 96 ? 2048 : 4096) ? 8 : 1;
   const int64_t blocks = (T + a.per - 1) / a.per;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   const dim3 grid((uint32_t)blocks, 2), block(256);

@@ -241,7 +241,7 @@ def test_scores_of_minus_infinity(dev, D, n):
 @pytest.mark.parametrize("H,HKV,D,lens", [
     (8, 4, 64, [50] * 13), (8, 4, 64, [600, 700]), (8, 4, 64, [8, 900, 1] * 2),
     (2, 1, 96, [10] * 70), (4, 2, 64, [10] * 70), (2, 2, 192, [130] * 5),
-    (2, 2, 192, [20] * 40)])
+    (2, 2, 192, [20] * 40), (2, 1, 53, [33] * 62), (2, 1, 53, [33] * 63)])
 def test_few_long_and_many_short(dev, H, HKV, D, lens):
     """Both arrangements of the forward's waves, on either side of the sizes
     that choose between them."""

@@ -246,6 +246,32 @@ def test_copy_pages(dev, dtype, tail, pairs):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("HKV,D,dtype", [(4, 159, torch.bfloat16),
+                                         (8, 128, torch.bfloat16),
+                                         (1, 20, torch.float32)])
+@pytest.mark.parametrize("T", [2047, 2051, 4099])
+def test_append_of_many_tokens(dev, HKV, D, dtype, T):
+    """On both sides of the sizes that a workgroup's share depends on."""
+    g = torch.Generator().manual_seed(T)
+    kv = torch.randn(2, T, HKV, D, generator=g).to(dtype).to(dev)
+    page, W = 64, ops.page_width(D)
+    n = -(-T // page) + 1
+    k, v = (torch.full((n, HKV, page, W), 7.0, dtype=dtype, device=dev)
+            for _ in range(2))
+    table = torch.randperm(n, generator=g).int()
+    pos = torch.arange(T, dtype=torch.int32)
+    pos[5::97] = -1
+    ops.paged_kv_append(kv[0], kv[1], k, v, table[None].to(dev), pos.to(dev),
+                        torch.zeros(T, dtype=torch.int32, device=dev))
+    live = pos >= 0
+    for new, pool in zip(kv, (k, v)):
+        seq = pool.cpu()[table.long()].transpose(1, 2).reshape(-1, HKV, W)
+        assert torch.equal(seq[:T][live][..., :D], new.cpu()[live])
+        assert (seq[:T][live][..., D:] == 0).all()
+        assert (seq[:T][~live] == 7).all() and (seq[T:] == 7).all()
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_append_attend_fork(dev):
     """A sequence is written token by token, forked inside a page, and both
     continue: each attends to what it wrote."""
