@@ -15,6 +15,7 @@ ops.paged_kv_append, ops.copy_pages, ops.token_logprobs.
 from __future__ import annotations
 
 import heapq
+import operator
 import threading
 from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
@@ -362,10 +363,10 @@ class PagedBatchingEngine:
             return []
         configs = configs or [None] * len(prompts)
         callbacks = callbacks or [None] * len(prompts)
-        if not len(prompts) == len(configs) == len(callbacks):
+        if min(len(configs), len(callbacks)) < len(prompts):
             raise ValueError(f"{len(prompts)} prompts, {len(configs)} configs "
                              f"and {len(callbacks)} callbacks")
-        cfgs = [c or GenerationConfig() for c in configs]
+        cfgs = [c or GenerationConfig() for c in configs[:len(prompts)]]
         stops = [self._stops(c) for c in cfgs]
         slots = self.free_slots()[:len(prompts)]
         if len(slots) < len(prompts):
@@ -399,10 +400,12 @@ class PagedBatchingEngine:
         """Checks a configuration; the tokens that end its answer."""
         if cfg.logprobs is not None and not 0 <= cfg.logprobs <= 64:
             raise ValueError(f"logprobs must be 0 to 64, got {cfg.logprobs}")
-        if not all(isinstance(t, int) for t in cfg.stop_token_ids):
+        try:
+            stops = {operator.index(t) for t in cfg.stop_token_ids}
+        except TypeError:
             raise ValueError("stop_token_ids must be whole numbers, got "
-                             f"{cfg.stop_token_ids}")
-        return set(cfg.stop_token_ids) | {self.tokenizer.eos_token_id}
+                             f"{cfg.stop_token_ids}") from None
+        return stops | {self.tokenizer.eos_token_id}
 
     def admit(self, prompt_ids: List[int],
               cfg: Optional[GenerationConfig] = None,

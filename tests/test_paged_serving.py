@@ -583,6 +583,21 @@ def test_a_request_that_cannot_be_sampled_fails_alone(small_model, tokenizer):
     assert w.eng.cache.free_pages == w.eng.cache.pages
 
 
+def test_stop_tokens_of_any_integer_type(small_model, tokenizer):
+    import numpy as np
+    solo = GenerationEngine(small_model.eval(), tokenizer)
+    stop = solo.generate([5, 6, 7], _cfg(6))[0]
+    eng = _engine(small_model, tokenizer)
+    for t in (stop, np.int64(stop), torch.tensor(stop)):
+        cfg = GenerationConfig(max_new_tokens=6, temperature=0.0,
+                               stop_token_ids=[t])
+        # a list may be longer than the prompts are
+        b, = eng.admit_many([[5, 6, 7]], [cfg, None], [None, None])
+        while eng.n_active():
+            eng.step()
+        assert eng.slots[b].result == []
+
+
 def test_engine_takes_nothing_for_a_request_it_refuses(small_model, tokenizer):
     eng = _engine(small_model, tokenizer)
     a = eng.admit([1, 2, 3], _cfg(4, logprobs=1))
