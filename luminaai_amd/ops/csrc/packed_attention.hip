@@ -421,10 +421,15 @@ DEV_INLINE void zero_rows(uint16_t* out, int heads, int head, int D, int from,
 // workgroups of four waves on a unit are better than one of eight: one's
 // exponentials run under the other's products, and causal blocks of half the
 // length are levelled better. 8192 tokens, four / eight waves: 32:8 heads x 128
-// 257 / 268 us (800 TFLOP/s), 12:4 x 159 95 / 105; 483 tokens of 8:4 x 64
-// 7.9 / 9.7. At 192 the images of two do not fit into LDS. Where there are few
+// 257 / 268 us (780 TFLOP/s), 12:4 x 159 95 / 105; 483 tokens of 8:4 x 64
+// 7.4 / 9.7. At 192 the images of two do not fit into LDS. Where there are few
 // blocks, a second set of waves takes the other half of a step's keys (PARTS = 2)
 // and both sets' maximum, sum and result are joined at the end.
+//
+// P enters P V as bf16: its roundings, up to 2^-8 each and independent from key to
+// key, leave an error of 1.9e-3 of the result where the result's own rounding
+// leaves 1.6e-3 (483 tokens of 8:4 x 64). Keeping 16 bits as run_bwd's FINE does
+// would make three products of two. The sum l is of the unrounded P, in fp32.
 // ===========================================================================
 template <int DP, int PARTS> struct Fwd {
   static constexpr int W = DP <= 160 ? 4 * PARTS : 8;    // waves
@@ -1049,11 +1054,12 @@ static hipError_t launch_bwd(PackedArgs& a, int* list, hipStream_t stream) {
 template <int DP>
 static hipError_t run_bwd(PackedArgs& a, int* list, hipStream_t stream) {
   // P and dS enter dV, dK and dQ as bf16; FINE adds what that rounding left over, in
-  // a second product. Small calls take it: the host needs 70 us for them anyway, and
-  // the roundings of few terms do not average out. Forward and gradient, without /
-  // with it: 52 tokens of 2:1 x 64 18.7 / 19.6 us with an error of dQ of 2.6e-3 /
-  // 1.9e-3 (the result's own rounding is 1.7e-3), 256 of 32:8 x 128 49.8 / 53.1,
-  // 2048 262 / 295, 8192 1084 / 1270 (2.4e-3 without).
+  // a second product. Small calls take it, as the roundings of few terms do not
+  // average out and an eager call is bound by the host's 70 us. Forward and gradient,
+  // without / with it: 52 tokens of 2:1 x 64 18.7 / 19.6 us with an error of dQ of
+  // 2.6e-3 / 1.9e-3 (the result's own rounding is 1.7e-3), 256 of 32:8 x 128 49.8 /
+  // 53.1, which a captured graph does pay, 2048 262 / 295, 8192 1084 / 1270 (2.4e-3
+  // without). So a sequence's gradients are rounded differently in a larger batch.
   if ((int64_t)a.T * a.H <= 8192) return launch_bwd<DP, true>(a, list, stream);
   return launch_bwd<DP, false>(a, list, stream);
 }

@@ -53,10 +53,10 @@ DEV_INLINE uint32_t pack_bf16(float lo, float hi) {
 // their chunks.
 //
 // Measured, join included: 64 rows of 32:8 heads x 128 with 1001 .. 32690 tokens,
-// 4.4 GB: 756 us, 5.8 TB/s (a large copy moves 5.1). Small calls wait for a chain
-// of loads (lengths, page number, K and V) and for the second launch: eight rows of
-// up to 4096 tokens, 52 MB: 16.3 us; one of 2041 with 12:4 x 159, 5 MB: 10.3, of
-// which the join takes 2.8.
+// 4.4 GB: 757 us, 5.8 TB/s (a plain read of as much 6.1 to 6.2). Small calls wait
+// for a chain of loads (lengths, page number, K and V) and for the second launch:
+// eight rows of up to 4096 tokens, 52 MB: 16.3 us (a plain read 11.3); one of 2041
+// with 12:4 x 159, 5 MB: 10.3, of which the join takes 3.
 // ===========================================================================
 struct PagedAttnArgs {
   const uint16_t* q;
@@ -624,8 +624,8 @@ extern "C" hipError_t lumina_paged_append(
 // two pools at once. The page numbers travel in the kernel's arguments, so a
 // call copies nothing to the device and may be captured. A workgroup moves
 // COPY_PIECE bytes of one page. Bound by bytes: 301 pages of 32 layers x 8 x 64 x
-// 128, keys and values, 5.0 GB: 970 us, 5.2 TB/s; 3 pages of 31 layers x 4 x 16 x
-// 160: 5.1 us, the launch.
+// 128, keys and values, 5.0 GB: 970 us, 5.2 TB/s (a plain copy of as much 5.5 to
+// 5.9); 3 pages of 31 layers x 4 x 16 x 160: 5.0 us, the launch.
 // ===========================================================================
 #define COPY_PAIRS 256
 #define COPY_PIECE 16384

@@ -26,7 +26,8 @@ def flash_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     strides), H a multiple of kv_heads, and at most 65536 sequences. Returns
     [T, H, D]. `scale` (positive) defaults to D ** -0.5. Rows behind the last
     sequence give zeros and get zero gradients. The gradient can be taken once
-    (on the GPU) and has one order of summation, so it is the same each time.
+    (on the GPU) and has one order of summation, so it is the same each time; its
+    probabilities are rounded to bf16, in calls of up to T * H = 8192 to 16 bits.
     The CPU refuses borders that fall or pass T; the GPU, which does not read
     them, cuts them to T and computes nothing outside the tensors, and what such
     borders give is not defined.
