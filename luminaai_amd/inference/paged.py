@@ -398,7 +398,8 @@ class PagedBatchingEngine:
 
     def _stops(self, cfg: GenerationConfig) -> set:
         """Checks a configuration; the tokens that end its answer."""
-        if cfg.logprobs is not None and not 0 <= cfg.logprobs <= 64:
+        if cfg.logprobs is not None and not (
+                isinstance(cfg.logprobs, int) and 0 <= cfg.logprobs <= 64):
             raise ValueError(f"logprobs must be 0 to 64, got {cfg.logprobs}")
         try:
             stops = {operator.index(t) for t in cfg.stop_token_ids}

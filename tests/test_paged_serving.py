@@ -598,6 +598,19 @@ def test_stop_tokens_of_any_integer_type(small_model, tokenizer):
         assert eng.slots[b].result == []
 
 
+@pytest.mark.parametrize("bad", [2.5, "3", 65, -1])
+def test_log_probabilities_of_one_row_do_not_end_the_others(
+        small_model, tokenizer, bad):
+    """One call computes those of all rows, so a bad number is refused before."""
+    eng = _engine(small_model, tokenizer)
+    a = eng.admit([1, 2, 3], _cfg(4, logprobs=1))
+    with pytest.raises(ValueError, match="logprobs"):
+        eng.admit([1, 2], _cfg(4, logprobs=bad))
+    while eng.n_active():
+        eng.step()
+    assert eng.slots[a].error is None and len(eng.slots[a].logprobs) == 4
+
+
 def test_engine_takes_nothing_for_a_request_it_refuses(small_model, tokenizer):
     eng = _engine(small_model, tokenizer)
     a = eng.admit([1, 2, 3], _cfg(4, logprobs=1))
