@@ -607,13 +607,12 @@ class MoEFFNLayer(nn.Module):
         route_idx = topi if placement is None else placement[topi]
         limit = None
         if seqs is not None and seqs.alone:
-            # a token's experts differ: no bucket takes more than all of them
+            # room for what all of them keep; a token's experts differ, so no
+            # bucket takes more than all tokens, and single ones lose none
             C = min(tokens, C + seqs.count)
             if seqs.lens is not None:
                 limit = (seqs.lens.double() * k / E * self.capacity_factor) \
                     .ceil().clamp(min=1).long()
-            else:
-                C = tokens
         plan = ops.interface.moe_routing_plan(
             route_idx, E, C, None if limit is None else seqs.seq, limit)
         counts = plan.counts if placement is None \
